@@ -49,7 +49,8 @@ int ksb_version(void);
 const char* ksb_last_error(void);
 /* Synchronises the device, returns the status words written by kernels whose bounded waits ran out
  * (code 0 = none; code 1 = a wait timed out, detail = kernel id << 16 | wait site; kernel ids: 1 FP8 GEMM,
- * 2 attention with one Q block per CTA, 3 attention with two, 4 FP8 GEMM with a split K, 15 the self-test) and clears them.
+ * 2 attention with one Q block per CTA, 3 attention with two, 4 FP8 GEMM with a split K, 5 gated projections and their
+ * gradients, 6 products with 4-bit weights, 15 the self-test) and clears them.
  * The words are sticky: from the moment a wait has run out, every later wait of every kernel on that GPU gives
  * up at once and leaves its outputs unwritten, until this call has read the words.  A caller that consumes
  * results should therefore check once per step, at a point where it synchronises anyway.
@@ -403,6 +404,22 @@ enum {
 };
 int64_t ksb_qwen_block_workspace(const ksb_qwen_block* block, int64_t text_tokens, int64_t img_tokens);
 int ksb_qwen_block_forward(const ksb_qwen_block* block, const ksb_qwen_call* call, int first, int last, void* workspace, ksb_stream_t stream);
+
+/* Operators of blocks whose halves are normed on both sides and whose feed-forward is gated, with the gradients that fine-tuning
+ * needs.  They have no counterpart in KsanaDiT, which runs such models through eager torch. ------------------------------------ */
+
+/* Products of a few rows with a weight held in 4 bits: the one-row Linears of a block (timestep embedding, modulation), whose time is
+ * the weight's way from memory.
+ *   out[m, n] = sum_g scale[n, g] * (sum_{k in g} (q[n, k] - zero[n, g]) * x[m, k]) + bias[n],  groups of 32, 64 or 128 columns
+ * x: [M, K] half (row stride ldx); out: [M, N] half (row stride ldo); bias: half [N] or NULL; K in whole groups, at most KSB_W4_MAX_K;
+ * sums of a group and over groups in fp32, one rounding at the end.  Up to 16 rows share one pass over the weight.
+ * weight: q packed as [ceil(N/16)][ceil(K/64)][512] bytes.  Byte ((r * 4 + t) * 16 + 8 * b + 4 * h + i) of tile (n, k) holds of
+ *   row 16 n + 8 h + r the columns 64 k + 32 b + 8 t + c with c = {0, 4, 1, 5}[i] in its low and c + 2 in its high four bits
+ * scale: half [ceil(N/16)][K/group][16]; zero: uint8 of the same layout, 0..15, or NULL for 8.
+ * Returns the number of kernels queued, or a negative code. */
+#define KSB_W4_MAX_K 65536
+int ksb_w4_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, const void* weight, const void* scale, const void* zero,
+                  int group, const void* bias, int64_t N, void* out, int64_t ldo, ksb_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -72,6 +72,8 @@ SIGNATURES = {
     "ksb_wan_block_forward": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p]),
     "ksb_qwen_block_workspace": (c_int64, [c_void_p, c_int64, c_int64]),
     "ksb_qwen_block_forward": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p]),
+    "ksb_w4_linear": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_void_p,
+                              c_int64, c_void_p]),
 }
 
 _lib = None

@@ -624,3 +624,63 @@ def qwen_rope_tables(img_grid, txt_len, axes=(16, 56, 56), theta=10000.0, scale_
     txt = torch.stack([torch.cos(tang), torch.sin(tang)], dim=-1).to(torch.float32).contiguous().to(device)
     _ROPE_TABLES[key] = ((img, axes[0] // 2, axes[1] // 2), (txt, axes[0] // 2, axes[1] // 2))
     return _ROPE_TABLES[key]
+
+
+# ----------------------------------------------------------------------------- gated halves of a block: 4-bit Linears, norms, projections
+
+
+def _elsewhere(device) -> bool:
+    """Whether a call's tensors are on another GPU than the current one (its launches then need that GPU, and its stream)."""
+    return device.index != torch.cuda.current_device()
+
+
+def _one_device(x, *ts):
+    if not x.is_cuda:
+        _cuda(x)
+    for t in ts:
+        if t is not None and t.device != x.device:
+            raise _lib.KsanaB200Error(f"all tensors of a call must be on one GPU: found {t.device} beside {x.device}")
+
+
+def _rows(x, K):
+    """x [..., K] as rows [M, K] with adjacent elements, a constant distance apart and on 16-byte boundaries (a copy where it is not)."""
+    x2 = x if x.dim() == 2 else x.reshape(-1, K)
+    if x2.stride(1) != 1 or (x2.shape[0] > 1 and (x2.stride(0) % 8 != 0 or x2.stride(0) < K)) or x2.data_ptr() % 16 != 0:
+        x2 = x2.clone(memory_format=torch.contiguous_format)
+    return x2
+
+
+def w4_linear(x, weight, weight_scale, weight_zero=None, bias=None, out_features=None):
+    """x [..., K] half times a packed 4-bit weight (``w4.quantize_w4``) -> [..., N] half.
+
+    out[m, n] = sum over groups of scale * sum (q - zero) x, plus bias; sums in fp32, one rounding.  N: ``out_features`` (default: 16
+    per tile row, or the bias's length).  The group is K / weight_scale.shape[1]: 32, 64 or 128.  Up to 16 rows of x share one pass over
+    the weight, more are taken 16 at a time: for many rows ``B200Fp8Linear`` is the faster class.  No gradients."""
+    dt, K = _dt(x), x.shape[-1]
+    if weight.dim() != 3 or weight.dtype != torch.uint8 or weight.shape[2] != 512 or not weight.is_contiguous():
+        raise _lib.KsanaB200Error("the packed weight must be a contiguous [ceil(N/16), ceil(K/64), 512] uint8 tensor")
+    nt, kt = weight.shape[:2]
+    N = out_features if out_features is not None else nt * 16 if bias is None else bias.numel()
+    groups = weight_scale.shape[1] if weight_scale.dim() == 3 else 0
+    group = K // groups if groups else 0
+    if kt != (K + 63) // 64 or nt != (N + 15) // 16 or group not in (32, 64, 128) or group * groups != K or N < 1:
+        raise _lib.KsanaB200Error(f"weight {tuple(weight.shape)} and scales {tuple(weight_scale.shape)} do not hold {N} x {K} values in groups of 32, 64 or 128")
+    if weight_scale.shape != (nt, groups, 16) or weight_scale.dtype != x.dtype or not weight_scale.is_contiguous():
+        raise _lib.KsanaB200Error(f"weight_scale must be a contiguous [{nt}, {groups}, 16] tensor of x's type, {x.dtype}")
+    if weight_zero is not None and (weight_zero.shape != weight_scale.shape or weight_zero.dtype != torch.uint8 or not weight_zero.is_contiguous()):
+        raise _lib.KsanaB200Error(f"weight_zero must be a contiguous [{nt}, {groups}, 16] uint8 tensor")
+    if bias is not None and (bias.shape != (N,) or bias.dtype != x.dtype or bias.stride(0) != 1):
+        raise _lib.KsanaB200Error(f"bias must hold {N} adjacent values of x's type, {x.dtype}")
+    if torch.is_grad_enabled() and (x.requires_grad or weight_scale.requires_grad or (bias is not None and bias.requires_grad)):
+        raise _lib.KsanaB200Error("w4_linear has no backward pass: call it under torch.no_grad() or on tensors that need no gradient")
+    _one_device(x, weight, weight_scale, weight_zero, bias)
+    if _elsewhere(x.device):
+        with torch.cuda.device(x.device):
+            return w4_linear(x, weight, weight_scale, weight_zero, bias, out_features)
+    x2 = _rows(x, K)
+    M = x2.shape[0]
+    out = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=x.device)
+    STATS.count(native.queued(_lib.load().ksb_w4_linear(
+        x2.data_ptr(), dt, M, K, x2.stride(0), weight.data_ptr(), weight_scale.data_ptr(), _p(weight_zero), group, _p(bias), N, out.data_ptr(), N,
+        _stream()), "ksb_w4_linear"))
+    return out
