@@ -417,7 +417,7 @@ int ksb_qwen_block_forward(const ksb_qwen_block* block, const ksb_qwen_call* cal
  *   row 16 n + 8 h + r the columns 64 k + 32 b + 8 t + c with c = {0, 4, 1, 5}[i] in its low and c + 2 in its high four bits
  * scale: half [ceil(N/16)][K/group][16]; zero: uint8 of the same layout, 0..15, or NULL for 8.
  * Returns the number of kernels queued, or a negative code. */
-#define KSB_W4_MAX_K 65536
+#define KSB_W4_MAX_K 32768
 int ksb_w4_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, const void* weight, const void* scale, const void* zero,
                   int group, const void* bias, int64_t N, void* out, int64_t ldo, ksb_stream_t stream);
 

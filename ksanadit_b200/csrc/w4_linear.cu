@@ -8,9 +8,11 @@
 // at most 15 in magnitude, exact in bf16 and fp16, so the products are exact and their sums are fp32 per group; the scale
 // multiplies a group's fp32 sum, it is never rounded into the weight.
 //
-// One CTA per SM, persistent over the row tiles: one thread copies the packed tiles of a row tile, up to CHUNK a stage, with their
-// scales and zero points into a ring in shared memory (bulk copies: consecutive bytes all the way), sixteen warps take the tiles
-// in turn, and their sums meet in shared memory in the order of the warps.  x waits in shared memory for all of it.
+// One CTA of sixteen warps per SM takes an even share of the row tiles, each warp an even share of that share's tiles: it copies
+// them, their scales and zero points into a ring of its own in shared memory, a few slots ahead (bulk copies; no warp waits for
+// another), and only at the end the sums of row tiles that several warps share are added up, in the order of the warps.  x
+// waits in shared memory.  Where it leaves no room for a ring, or there are few row tiles, the CTAs of a cluster share K: each
+// keeps its row tiles' sums, and in the end they are added up in the order of K through distributed shared memory.
 #include <algorithm>
 
 #include "../../include/ksana_b200.h"
@@ -22,11 +24,9 @@ namespace w4 {
 
 constexpr int KERNEL_ID = 6;
 constexpr int TILE_N = 16, TILE_K = 64, TILE_BYTES = 512;
-constexpr int WARPS = 16, CHUNK = 32;  // tiles per stage
-constexpr int THREADS = WARPS * 32 + 32;
-constexpr int MAX_STAGES = 12;
+constexpr int WARPS = 16, THREADS = WARPS * 32;
+constexpr int MAX_SLOTS = 4;  // of a warp's ring
 constexpr int SMEM_LIMIT = 232448;
-constexpr int BAR_BYTES = MAX_STAGES * 16;
 
 struct Params {
   const void* x;
@@ -37,41 +37,57 @@ struct Params {
   void* out;
   int64_t ldx, ldo;
   int M, N, K;
-  int units, tiles_k;    // row tiles, tiles of a row tile
-  int group, groups;     // columns per group, groups of a row
+  int split;             // CTAs of a cluster, which share K
+  int units_each, units_over;  // row tiles per cluster; the first clusters have one more
+  int steps, groups;     // of a row tile (a step: GT tiles)
   int pitch;             // bytes between rows of x in shared memory: 64 more than a multiple of 128, so that the eight 16-byte
                          // reads of a quarter warp (two rows, four neighbours each) are in different banks
-  int stages, stage_bytes, zero_at;  // of the ring; where a stage's zero points are (its scales are behind CHUNK tiles)
+  int slots, slot_steps, slot_bytes, scale_at, zero_at;  // a warp's ring
+  int x_at, sums_at;     // in shared memory, behind the rings
   int* status;
 };
 
+// (w & 0x000f000f) | c as one instruction
+__device__ __forceinline__ uint32_t take(uint32_t w, uint32_t c) {
+  uint32_t v;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(v) : "r"(w), "r"(0x000f000fu), "r"(c));
+  return v;
+}
 template <typename T> struct Nibbles;
 // 128 + q is the bf16 number 0x4300 | q, 1024 + q the fp16 number 0x6400 | q; 128 + z and 1024 + z are exact as well.
 template <> struct Nibbles<__nv_bfloat16> {
+  typedef uint16_t IsHalf;
   static __device__ __forceinline__ uint32_t offset(uint32_t z) { return (0x4300u | z) * 0x10001u; }
   static __device__ __forceinline__ uint32_t pair(uint32_t w, int i, uint32_t off) {
-    const uint32_t v = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+    const uint32_t v = take(w >> (4 * i), 0x43004300u);
     const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&off));
     return *reinterpret_cast<const uint32_t*>(&d);
   }
 };
 template <> struct Nibbles<__half> {
+  typedef uint8_t IsHalf;
   static __device__ __forceinline__ uint32_t offset(uint32_t z) { return (0x6400u | z) * 0x10001u; }
   static __device__ __forceinline__ uint32_t pair(uint32_t w, int i, uint32_t off) {
-    const uint32_t v = ((w >> (4 * i)) & 0x000f000fu) | 0x64006400u;
+    const uint32_t v = take(w >> (4 * i), 0x64006400u);
     const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&off));
     return *reinterpret_cast<const uint32_t*>(&d);
   }
 };
 
-template <typename T> __device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
-template <> __device__ __forceinline__ void mma16<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-template <> __device__ __forceinline__ void mma16<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// c = a * b + c; the first of a group's products starts from zeros
+#define KSB_MMA16(NAME, TYPE)                                                                                                              \
+  __device__ __forceinline__ void NAME(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0, float c1, float c2, float c3) { \
+    asm("mma.sync.aligned.m16n8k16.row.col.f32." TYPE "." TYPE ".f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"    \
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])                                                                                    \
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));                                \
+  }
+KSB_MMA16(mma_bf16, "bf16")
+KSB_MMA16(mma_f16, "f16")
+#undef KSB_MMA16
+template <typename T> __device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, bool first) {
+  const float c0 = first ? 0.f : c[0], c1 = first ? 0.f : c[1], c2 = first ? 0.f : c[2], c3 = first ? 0.f : c[3];
+  if constexpr (sizeof(typename Nibbles<T>::IsHalf) == 1) mma_f16(c, a, b0, b1, c0, c1, c2, c3);
+  else mma_bf16(c, a, b0, b1, c0, c1, c2, c3);
 }
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
@@ -79,160 +95,232 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                : "memory");
 }
 
-// NT: blocks of eight rows of x.  FINE: groups of 32 columns, a scale per half tile.
-template <typename T, int NT, bool ZEROS, bool FINE>
+__device__ __forceinline__ float load_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// NT: blocks of eight rows of x.  G: columns of a group.
+template <typename T, int NT, bool ZEROS, int G>
 __global__ void __launch_bounds__(THREADS, 1) w4_kernel(const __grid_constant__ Params p) {
   extern __shared__ __align__(128) uint8_t smem[];
-  constexpr int SUMS = TILE_N * 8 * NT;  // of a row tile
-  __shared__ __align__(16) float red[2][WARPS][SUMS];
-  __shared__ __align__(8) uint64_t bars[2 * MAX_STAGES];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t ring = smem_u32(smem), full0 = smem_u32(bars), empty0 = full0 + 8 * MAX_STAGES;
-  uint8_t* xs = smem + p.stages * p.stage_bytes;
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < p.stages; ++s) {
-      mbar_init(full0 + 8 * s, 1);
-      mbar_init(empty0 + 8 * s, WARPS);
+  constexpr int GT = G == 128 ? 2 : 1;        // tiles per step
+  constexpr int SCALES = G == 32 ? 2 : 1;     // groups per step
+  constexpr int SUMS = TILE_N * 8 * NT;       // of a row tile: [row of x][row of the weight]
+  // [0]: of the row tile that a warp comes into midway.  [1]: of the one it leaves midway, and on its way to memory any other's
+  __shared__ __align__(16) float parts[2][WARPS][SUMS];
+  __shared__ __align__(16) uint8_t nothing[256];  // x of the rows there are not
+  __shared__ __align__(8) uint64_t bars[WARPS * MAX_SLOTS + 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
+  const int split = p.split, rank = split > 1 ? (int)cluster_ctarank() : 0, cluster = blockIdx.x / split;
+  const int k0 = p.steps * rank / split, steps = p.steps * (rank + 1) / split - k0;  // this CTA's steps of every row tile
+  const int u0 = cluster * p.units_each + min(cluster, p.units_over), units = p.units_each + (cluster < p.units_over);
+  const int64_t share = static_cast<int64_t>(units) * steps;
+  const int begin = static_cast<int>(share * warp / WARPS), end = static_cast<int>(share * (warp + 1) / WARPS);
+  uint8_t* ring = smem + warp * p.slots * p.slot_bytes;
+  uint8_t* xs = smem + p.x_at;
+  float* sums = reinterpret_cast<float*>(smem + p.sums_at);  // split: [row tile][SUMS]
+  const uint32_t ring_at = smem_u32(ring), bar0 = smem_u32(bars + warp * MAX_SLOTS), x_bar = smem_u32(bars + WARPS * MAX_SLOTS);
+  int u = begin / steps, k = begin - u * steps;
+  int ahead = begin, ahead_u = u, ahead_k = k;  // of the next slot to ask for
+  const int x0 = k0 * GT * TILE_K, width = min(p.K - x0, steps * GT * TILE_K);  // this CTA's columns of x
+  // Up to a slot of steps, not past a row tile's end.
+  auto fetch = [&](int s) {
+    const int n = min(min(p.slot_steps, end - ahead), steps - ahead_k);
+    const int64_t row = u0 + ahead_u, kk = k0 + ahead_k, g0 = row * p.groups + kk * SCALES;
+    const uint32_t groups = SCALES == 1 ? n : min(2 * n, p.groups - 2 * (int)kk), bytes = n * GT * TILE_BYTES;
+    const uint32_t dst = ring_at + s * p.slot_bytes, bar = bar0 + 8 * s;
+    mbar_arrive_expect_tx(bar, bytes + groups * (ZEROS ? 48 : 32));
+    bulk_load(dst, p.weight + (row * p.steps + kk) * (GT * TILE_BYTES), bytes, bar);
+    bulk_load(dst + p.scale_at, p.scale + g0 * 32, groups * 32, bar);
+    if (ZEROS) bulk_load(dst + p.zero_at, p.zero + g0 * 16, groups * 16, bar);
+    ahead += n;
+    ahead_k += n;
+    if (ahead_k == steps) {
+      ahead_k = 0;
+      ++ahead_u;
     }
+  };
+  if (lane == 0) {
+    for (int s = 0; s < p.slots; ++s) mbar_init(bar0 + 8 * s, 1);
+    if (warp == 0) mbar_init(x_bar, 1);
     fence_barrier_init();
+    if (warp == 0) {
+      // Ahead of the weight: behind its slots a row of x took a round trip of microseconds.
+      mbar_arrive_expect_tx(x_bar, p.M * width * 2);
+      for (int m = 0; m < p.M; ++m) bulk_load(smem_u32(xs) + m * p.pitch, static_cast<const T*>(p.x) + m * p.ldx + x0, width * 2, x_bar);
+    }
+    for (int s = 0; s < p.slots && ahead < end; ++s) fetch(s);
   }
+  // zeros behind the last column of x, and in place of its missing rows
+  if (threadIdx.x < 16) reinterpret_cast<uint4*>(nothing)[threadIdx.x] = make_uint4(0, 0, 0, 0);
+  if (G == 32 && width < steps * TILE_K && threadIdx.x < 4 * p.M)
+    *reinterpret_cast<uint4*>(xs + (threadIdx.x >> 2) * p.pitch + width * 2 + (threadIdx.x & 3) * 16) = make_uint4(0, 0, 0, 0);
   __syncthreads();
-  const int chunks = (p.tiles_k + CHUNK - 1) / CHUNK;
-  const int chunk_groups = CHUNK * TILE_K / p.group;
-  if (warp == WARPS) {
-    if (lane == 0) {
-      uint32_t it = 0;
-      bool ok = true;
-      for (int u = blockIdx.x; u < p.units && ok; u += gridDim.x) {
-        for (int c = 0; c < chunks; ++c, ++it) {
-          const uint32_t s = it % p.stages, ph = (it / p.stages) & 1;
-          if (!mbar_wait(empty0 + 8 * s, ph ^ 1, p.status, (KERNEL_ID << 16) | 1)) { ok = false; break; }
-          const int tiles = min(CHUNK, p.tiles_k - c * CHUNK), groups = min(chunk_groups, p.groups - c * chunk_groups);
-          const int64_t g0 = static_cast<int64_t>(u) * p.groups + c * chunk_groups;
-          const uint32_t dst = ring + s * p.stage_bytes, bar = full0 + 8 * s;
-          mbar_arrive_expect_tx(bar, tiles * TILE_BYTES + groups * (ZEROS ? 48 : 32));
-          bulk_load(dst, p.weight + (static_cast<int64_t>(u) * p.tiles_k + c * CHUNK) * TILE_BYTES, tiles * TILE_BYTES, bar);
-          bulk_load(dst + CHUNK * TILE_BYTES, p.scale + g0 * 32, groups * 32, bar);
-          if (ZEROS) bulk_load(dst + p.zero_at, p.zero + g0 * 16, groups * 16, bar);
-        }
+  bool failed = !mbar_wait_warp(x_bar, 0, p.status, (KERNEL_ID << 16) | 3);
+
+  float acc[NT][4];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[nt][i] = 0.f;
+  // a row tile's sums on their way out
+  auto put = [&](int which) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        parts[which][warp][(nt * 8 + 2 * t + (i & 1)) * TILE_N + r + (i >> 1) * 8] = acc[nt][i];
+        acc[nt][i] = 0.f;
       }
-      // what is on its way lands before the block leaves
-      for (uint32_t i = it > (uint32_t)p.stages ? it - p.stages : 0; i < it; ++i)
-        mbar_wait(full0 + 8 * (i % p.stages), (i / p.stages) & 1, p.status, (KERNEL_ID << 16) | 3);
+    __syncwarp();
+  };
+  auto store = [&](int row_tile, int j, float v) {
+    const int m = j >> 4, n = (u0 + row_tile) * TILE_N + (j & 15);
+    if (n >= p.N) return;
+    if (p.bias) v += HalfOps<T>::to_f(static_cast<const T*>(p.bias)[n]);
+    static_cast<T*>(p.out)[m * p.ldo + n] = HalfOps<T>::from_f(v);
+  };
+  auto keep = [&](int row_tile, int j, float v) {
+    if (split > 1) sums[row_tile * SUMS + j] = v;
+    else store(row_tile, j, v);
+  };
+  const int live = p.M * TILE_N;  // sums that there are
+  // a lane's x: of a row that there is not, the same zeros at every step
+  const uint8_t* x_at[NT];
+  int x_step[NT];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const bool there = nt * 8 + r < p.M;
+    x_at[nt] = (there ? xs + (nt * 8 + r) * p.pitch : nothing) + t * 16;
+    x_step[nt] = there ? GT * 128 : 0;
+  }
+  bool entered = k != 0;  // the row tile was begun by an earlier warp
+  int slot = 0;
+  uint32_t phase = 0;
+  for (int at = begin; at < end;) {
+    if (failed || !mbar_wait_warp(bar0 + 8 * slot, phase, p.status, (KERNEL_ID << 16) | 1)) {
+      failed = true;
+      break;
     }
-  } else {
-    // x, zeros behind its last column
-    const int units16 = p.tiles_k * 8, width = p.K / 8;  // 16-byte units of a row
-    for (int i = threadIdx.x; i < p.M * units16; i += WARPS * 32) {
-      const int m = i / units16, u = i - m * units16;
-      const uint4 v = u < width ? reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) + m * p.ldx)[u] : make_uint4(0, 0, 0, 0);
-      *reinterpret_cast<uint4*>(xs + m * p.pitch + u * 16) = v;
-    }
-    asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory");
-    const int r = lane >> 2, t = lane & 3;
-    const int group_shift = p.group == 128 ? 1 : 0;
-    bool failed = false;
-    uint32_t it = 0;
-    int par = 0;
-    for (int u = blockIdx.x; u < p.units; u += gridDim.x, par ^= 1) {
-      float acc[NT][4];
+    const int n = min(min(p.slot_steps, end - at), steps - k);
+    const uint8_t* tiles = ring + slot * p.slot_bytes + lane * 16;
+    const T* scales = reinterpret_cast<const T*>(ring + slot * p.slot_bytes + p.scale_at) + r;
+    const uint8_t* zeros = ring + slot * p.slot_bytes + p.zero_at + r;
+    // a row's last half tile may be behind K: it has no group of its own, and zeros in x
+    const int lone = SCALES == 2 && (p.groups & 1) && k0 + k + n == p.steps ? n - 1 : -1;
+#pragma unroll(GT == 1 ? 2 : 1)
+    for (int j = 0; j < n; ++j) {
+      float part[NT][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int half = 0; half < 2 * GT; ++half) {
+        const uint4 a4 = *reinterpret_cast<const uint4*>(tiles + (half >> 1) * TILE_BYTES);
+        const uint32_t w0 = half & 1 ? a4.z : a4.x, w1 = half & 1 ? a4.w : a4.y;
+        const bool first = SCALES == 2 || half == 0, done = SCALES == 2 || half == 2 * GT - 1;
+        const int g = SCALES == 2 && half == 1 && j != lone ? TILE_N : 0;
+        uint32_t z0 = 8, z1 = 8;
+        if (ZEROS) {
+          z0 = zeros[g] & 15u;
+          z1 = zeros[g + 8] & 15u;
+        }
+        z0 = Nibbles<T>::offset(z0);
+        z1 = Nibbles<T>::offset(z1);
+        uint32_t a[2][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[nt][i] = 0.f;
-      for (int c = 0; c < chunks; ++c, ++it) {
-        const uint32_t s = it % p.stages, ph = (it / p.stages) & 1;
-        if (!failed && !mbar_wait_warp(full0 + 8 * s, ph, p.status, (KERNEL_ID << 16) | 2)) failed = true;
-        if (failed) continue;
-        const int tiles = min(CHUNK, p.tiles_k - c * CHUNK);
-        const uint8_t* stage = smem + s * p.stage_bytes;
-        const T* scales = reinterpret_cast<const T*>(stage + CHUNK * TILE_BYTES);
-        const uint8_t* zeros = stage + p.zero_at;
-        for (int j = warp; j < tiles; j += WARPS) {
-          const uint4 a4 = *reinterpret_cast<const uint4*>(stage + j * TILE_BYTES + lane * 16);
-          const uint32_t words[4] = {a4.x, a4.y, a4.z, a4.w};
-          float part[NT][4], s0 = 0.f, s1 = 0.f;
-          uint32_t z0 = Nibbles<T>::offset(8), z1 = z0;
+        for (int c = 0; c < 2; ++c) {
+          a[c][0] = Nibbles<T>::pair(w0, 2 * c, z0);
+          a[c][1] = Nibbles<T>::pair(w1, 2 * c, z1);
+          a[c][2] = Nibbles<T>::pair(w0, 2 * c + 1, z0);
+          a[c][3] = Nibbles<T>::pair(w1, 2 * c + 1, z1);
+        }
+        float s0 = 0.f, s1 = 0.f;
+        if (done) {
+          s0 = HalfOps<T>::to_f(scales[g]);
+          s1 = HalfOps<T>::to_f(scales[g + 8]);
+        }
 #pragma unroll
-          for (int kb = 0; kb < 2; ++kb) {
-            if (FINE || kb == 0) {
-              // a last half tile behind K has zeros in x: any group's scale will do
-              const int g = FINE ? min(2 * j + kb, p.groups - 1 - c * chunk_groups) : j >> group_shift;
-              s0 = HalfOps<T>::to_f(scales[g * 16 + r]);
-              s1 = HalfOps<T>::to_f(scales[g * 16 + r + 8]);
-              if (ZEROS) {
-                z0 = Nibbles<T>::offset(zeros[g * 16 + r] & 15u);
-                z1 = Nibbles<T>::offset(zeros[g * 16 + r + 8] & 15u);
-              }
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) part[nt][i] = 0.f;
-            }
-            uint32_t a[2][4];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              a[h][0] = Nibbles<T>::pair(words[2 * kb], 2 * h, z0);
-              a[h][1] = Nibbles<T>::pair(words[2 * kb + 1], 2 * h, z1);
-              a[h][2] = Nibbles<T>::pair(words[2 * kb], 2 * h + 1, z0);
-              a[h][3] = Nibbles<T>::pair(words[2 * kb + 1], 2 * h + 1, z1);
-            }
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              uint4 b = make_uint4(0, 0, 0, 0);
-              const int m = nt * 8 + r;
-              if (m < p.M) b = *reinterpret_cast<const uint4*>(xs + m * p.pitch + ((c * CHUNK + j) * 2 + kb) * 64 + t * 16);
-              mma16<T>(part[nt], a[0], b.x, b.y);
-              mma16<T>(part[nt], a[1], b.z, b.w);
-            }
-            if (FINE || kb == 1) {
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                acc[nt][0] = fmaf(s0, part[nt][0], acc[nt][0]);
-                acc[nt][1] = fmaf(s0, part[nt][1], acc[nt][1]);
-                acc[nt][2] = fmaf(s1, part[nt][2], acc[nt][2]);
-                acc[nt][3] = fmaf(s1, part[nt][3], acc[nt][3]);
-              }
-            }
+        for (int nt = 0; nt < NT; ++nt) {
+          const uint4 b = *reinterpret_cast<const uint4*>(x_at[nt] + (k + j) * x_step[nt] + half * 64);
+          mma16<T>(part[nt], a[0], b.x, b.y, first);
+          mma16<T>(part[nt], a[1], b.z, b.w, false);
+          if (done) {
+            acc[nt][0] = fmaf(s0, part[nt][0], acc[nt][0]);
+            acc[nt][1] = fmaf(s0, part[nt][1], acc[nt][1]);
+            acc[nt][2] = fmaf(s1, part[nt][2], acc[nt][2]);
+            acc[nt][3] = fmaf(s1, part[nt][3], acc[nt][3]);
           }
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(empty0 + 8 * s);
       }
-      // [row of x][row of the weight]
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) red[par][warp][(nt * 8 + 2 * t + (i & 1)) * TILE_N + r + (i >> 1) * 8] = acc[nt][i];
-      failed = named_bar_or(1, WARPS * 32, failed);
-      if (failed) break;
-      const int m = threadIdx.x >> 4, n = u * TILE_N + (threadIdx.x & 15);
-      if (threadIdx.x < SUMS && m < p.M && n < p.N) {
-        float v = 0.f;
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) v += red[par][w][threadIdx.x];
-        if (p.bias) v += HalfOps<T>::to_f(static_cast<const T*>(p.bias)[n]);
-        static_cast<T*>(p.out)[m * p.ldo + n] = HalfOps<T>::from_f(v);
-      }
+      tiles += GT * TILE_BYTES;
+      scales += SCALES * TILE_N;
+      zeros += SCALES * TILE_N;
     }
+    __syncwarp();
+    if (lane == 0 && ahead < end) fetch(slot);
+    if (++slot == p.slots) {
+      slot = 0;
+      phase ^= 1;
+    }
+    at += n;
+    k += n;
+    if (k == steps) {  // the end of a row tile
+      put(entered ? 0 : 1);
+      if (!entered) {
+#pragma unroll 1
+        for (int j = lane; j < live; j += 32) keep(u, j, parts[1][warp][j]);
+        __syncwarp();
+      }
+      entered = false;
+      k = 0;
+      ++u;
+    }
+  }
+  if (failed) {  // what is on its way lands before the block leaves
+    for (int s = slot; s < slot + p.slots; ++s) mbar_wait(bar0 + 8 * (s % p.slots), phase ^ (s >= p.slots), p.status, (KERNEL_ID << 16) | 2);
+  }
+  if (k != 0 && begin < end) put(entered ? 0 : 1);
+  __syncthreads();
+  // The warp that has begun a row tile and left it to others adds up its pieces.
+  const int tail = end / steps, start = tail * steps;  // the row tile that the end falls into
+  if (end != start && begin < end && begin <= start) {
+#pragma unroll 1
+    for (int j = lane; j < live; j += 32) {
+      float v = parts[1][warp][j];
+      for (int w = warp + 1, from = end; w < WARPS && from < start + steps; ++w) {
+        const int to = static_cast<int>(share * (w + 1) / WARPS);
+        if (to > from) v += parts[0][w][j];
+        from = to;
+      }
+      keep(tail, j, v);
+    }
+  }
+  if (split > 1) {
+    cluster_sync_all();  // every CTA's sums are there
+    const uint32_t mine = smem_u32(sums);
+    for (int i = rank * THREADS + threadIdx.x; i < units * live; i += split * THREADS) {
+      const int row_tile = i / live, j = i - row_tile * live;
+      float v = 0.f;
+      for (int c = 0; c < split; ++c) v += load_cluster(mapa_shared(mine, c) + (row_tile * SUMS + j) * 4);
+      store(row_tile, j, v);
+    }
+    cluster_sync_all();  // none leaves while another reads it
   }
 }
 
-template <typename T, int NT, bool ZEROS, bool FINE> static int launch(const Params& p, int grid, size_t smem, cudaStream_t st) {
-  auto kernel = w4_kernel<T, NT, ZEROS, FINE>;
+constexpr int fixed_bytes(int nt) { return 2 * WARPS * TILE_N * 8 * nt * 4 + 256 + WARPS * MAX_SLOTS * 8 + 128; }
+template <typename T, int NT, bool ZEROS, int G> static int launch(const Params& p, int grid, size_t smem, cudaStream_t st) {
+  auto kernel = w4_kernel<T, NT, ZEROS, G>;
   static DeviceOnce limit;
-  const int fixed = 2 * WARPS * TILE_N * 8 * NT * 4 + 16 * MAX_STAGES + 64;
-  if (int rc = limit.raise_smem(reinterpret_cast<const void*>(kernel), SMEM_LIMIT - fixed)) return rc;
-  return launch_kernel("w4 linear", reinterpret_cast<const void*>(kernel), dim3((unsigned)grid), dim3(THREADS), smem, st, 1, false, p);
+  if (int rc = limit.raise_smem(reinterpret_cast<const void*>(kernel), SMEM_LIMIT - fixed_bytes(NT))) return rc;
+  return launch_kernel("w4 linear", reinterpret_cast<const void*>(kernel), dim3((unsigned)grid), dim3(THREADS), smem, st, p.split, false, p);
 }
-template <typename T> static int dispatch(const Params& p, int grid, size_t smem, cudaStream_t st) {
-  const bool wide = p.M > 8, zeros = p.zero != nullptr, fine = p.group == 32;
-  if (wide) {
-    if (zeros) return fine ? launch<T, 2, true, true>(p, grid, smem, st) : launch<T, 2, true, false>(p, grid, smem, st);
-    return fine ? launch<T, 2, false, true>(p, grid, smem, st) : launch<T, 2, false, false>(p, grid, smem, st);
-  }
-  if (zeros) return fine ? launch<T, 1, true, true>(p, grid, smem, st) : launch<T, 1, true, false>(p, grid, smem, st);
-  return fine ? launch<T, 1, false, true>(p, grid, smem, st) : launch<T, 1, false, false>(p, grid, smem, st);
+template <typename T, int NT, bool ZEROS> static int with_group(const Params& p, int group, int grid, size_t smem, cudaStream_t st) {
+  return group == 32 ? launch<T, NT, ZEROS, 32>(p, grid, smem, st) : group == 64 ? launch<T, NT, ZEROS, 64>(p, grid, smem, st) : launch<T, NT, ZEROS, 128>(p, grid, smem, st);
+}
+template <typename T> static int dispatch(const Params& p, int group, int grid, size_t smem, cudaStream_t st) {
+  if (p.M > 8) return p.zero ? with_group<T, 2, true>(p, group, grid, smem, st) : with_group<T, 2, false>(p, group, grid, smem, st);
+  return p.zero ? with_group<T, 1, true>(p, group, grid, smem, st) : with_group<T, 1, false>(p, group, grid, smem, st);
 }
 
 }  // namespace w4
@@ -260,29 +348,49 @@ extern "C" int ksb_w4_linear(const void* x, int dtype, int64_t M, int64_t K, int
   p.bias = bias;
   p.ldx = ldx; p.ldo = ldo;
   p.N = (int)N; p.K = (int)K;
-  p.units = (int)((N + w4::TILE_N - 1) / w4::TILE_N);
-  p.tiles_k = (int)((K + w4::TILE_K - 1) / w4::TILE_K);
-  p.group = group; p.groups = (int)(K / group);
-  p.pitch = p.tiles_k * 128 + 64;
-  const int chunk_groups = w4::CHUNK * w4::TILE_K / group;
-  p.zero_at = w4::CHUNK * w4::TILE_BYTES + chunk_groups * 32;
-  p.stage_bytes = p.zero_at + (zero ? chunk_groups * 16 : 0);
-  const int grid = p.units < sm_count() ? p.units : sm_count();
+  const int units = (int)((N + w4::TILE_N - 1) / w4::TILE_N);
+  const int tiles = (int)((K + w4::TILE_K - 1) / w4::TILE_K), step_tiles = group == 128 ? 2 : 1;
+  p.steps = tiles / step_tiles;
+  p.groups = (int)(K / group);
+  // A slot: eight tiles and their scales, or four where x leaves less room.
+  auto slot = [&](int slot_tiles) {
+    const int groups = slot_tiles / step_tiles * (group == 32 ? 2 : 1);
+    p.slot_steps = slot_tiles / step_tiles;
+    p.scale_at = slot_tiles * w4::TILE_BYTES;
+    p.zero_at = p.scale_at + groups * 32;
+    p.slot_bytes = (p.zero_at + (zero ? groups * 16 : 0) + 127) / 128 * 128;
+  };
+  // K is shared by a cluster where that fills the GPU, or makes room for the rows of x.
+  auto plan = [&](int rows, int split) {
+    const int clusters = std::min(units, std::max(1, sm_count() / split)), sums = w4::TILE_N * (rows > 8 ? 16 : 8) * 4;
+    p.split = split;
+    p.units_each = units / clusters;
+    p.units_over = units % clusters;
+    p.pitch = ((p.steps + split - 1) / split) * step_tiles * 128 + 64;
+    const int64_t kept = split > 1 ? (int64_t)(p.units_each + 1) * sums : 0;
+    const int64_t room = (w4::SMEM_LIMIT - w4::fixed_bytes(rows > 8 ? 2 : 1) - (int64_t)rows * p.pitch - kept) / w4::WARPS;
+    slot(8);
+    if (room < 2 * p.slot_bytes) slot(4);
+    p.slots = (int)std::max<int64_t>(0, std::min<int64_t>(w4::MAX_SLOTS, room / p.slot_bytes));
+    p.x_at = w4::WARPS * p.slots * p.slot_bytes;
+    p.sums_at = p.x_at + rows * p.pitch;
+    return p.slots >= 2 ? p.sums_at + (int)kept : 0;
+  };
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   int launches = 0;
-  // Rows of one launch: what fits beside two stages and the sums.
-  for (int64_t m0 = 0; m0 < M;) {
-    const int room = w4::SMEM_LIMIT - 2 * w4::WARPS * w4::TILE_N * 16 * 4 - 16 * w4::MAX_STAGES - 64 - 2 * p.stage_bytes;
-    const int64_t rows = std::min<int64_t>({M - m0, 16, room / p.pitch});
-    p.M = (int)rows;
+  for (int64_t m0 = 0; m0 < M; ++launches) {
+    const int64_t left = M - m0, passes = (left + 15) / 16;
+    int rows = (int)((left + passes - 1) / passes), split = 1, smem = 0;
+    while (split < 8 && 2 * split * units <= sm_count() && 2 * split <= p.steps) split *= 2;
+    while ((smem = plan(rows, split)) == 0 && split < 8 && 2 * split <= p.steps) split *= 2;
+    while (smem == 0 && rows > 1) smem = plan(rows = (rows + 1) / 2, split = 1);  // the kept sums of very many row tiles
+    if (smem == 0) return fail(KSB_ERR_UNSUPPORTED, "no room for a row of %lld columns", (long long)K);
+    p.M = rows;
     p.x = static_cast<const uint8_t*>(x) + m0 * ldx * 2;
     p.out = static_cast<uint8_t*>(out) + m0 * ldo * 2;
-    const int fixed = 2 * w4::WARPS * w4::TILE_N * (rows > 8 ? 16 : 8) * 4 + 16 * w4::MAX_STAGES + 64;
-    p.stages = std::min(w4::MAX_STAGES, (w4::SMEM_LIMIT - fixed - (int)rows * p.pitch) / p.stage_bytes);
-    const size_t smem = (size_t)p.stages * p.stage_bytes + (size_t)rows * p.pitch;
-    if (int rc = dtype == KSB_BF16 ? w4::dispatch<__nv_bfloat16>(p, grid, smem, st) : w4::dispatch<__half>(p, grid, smem, st)) return rc;
+    const int grid = std::min(units, std::max(1, sm_count() / split)) * split;
+    if (int rc = dtype == KSB_BF16 ? w4::dispatch<__nv_bfloat16>(p, group, grid, smem, st) : w4::dispatch<__half>(p, group, grid, smem, st)) return rc;
     m0 += rows;
-    ++launches;
   }
   return launches;
 }

@@ -36,7 +36,7 @@ def _check(out, x, packed, scale, zero, bias, N, K):
 @pytest.mark.parametrize("M,N,K,group,zeros", [
     (1, 16, 32, 32, False), (1, 1, 64, 64, True), (2, 17, 96, 32, True), (3, 100, 128, 128, False), (8, 48, 2048, 64, True), (9, 33, 2176, 128, True),
     (16, 4000, 256, 32, False), (7, 2500, 4160, 32, True), (17, 50, 512, 64, False), (35, 24, 128, 64, True), (1, 9216, 1536, 128, False), (12, 40, 13824, 128, True),
-    (16, 64, 8960, 64, False), (5, 16, 65536, 128, False)])
+    (16, 64, 8960, 64, False), (5, 16, 32768, 32, True)])
 def test_products(dtype, M, N, K, group, zeros):
     x, packed, scale, zero, bias = _case(M, N, K, group, zeros, dtype, M + N + K)
     for b in (None, bias):

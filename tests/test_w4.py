@@ -88,4 +88,4 @@ def test_c_entry_refuses_before_any_launch():
     for bad in (dict(x=None), dict(w=None), dict(s=None), dict(out=None), dict(dtype=2), dict(group=16), dict(group=0), dict(K=100), dict(K=0), dict(N=0), dict(M=-1),
                 dict(x=p + 2), dict(w=p + 8), dict(z=p + 4), dict(M=2, ldx=64), dict(M=2, ldx=132), dict(M=2, ldo=8)):
         assert call(**bad) == -1, bad
-    assert call(K=65536 + 64) == -3
+    assert call(K=32768 + 64) == -3
