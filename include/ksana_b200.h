@@ -421,6 +421,35 @@ int ksb_qwen_block_forward(const ksb_qwen_block* block, const ksb_qwen_call* cal
 int ksb_w4_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, const void* weight, const void* scale, const void* zero,
                   int group, const void* bias, int64_t N, void* out, int64_t ldo, ksb_stream_t stream);
 
+/* Norms on both sides of a block's half:
+ *   r = x + residual_scale * gate * N(y) * post_w;   h = N(r) * pre_w * (1 + scale) + shift
+ * N: v * rsqrt(mean(v^2) + eps), with `layer` the same of v - mean(v).  fp32 throughout, each result rounded once (h is the norm of the
+ * unrounded r).  x, y, r, h: [M, C] half (row strides ldx, ldy; r and h contiguous); gate, scale, shift: half, mod_rows rows (mod_rows
+ * divides M; row m uses row m / (M / mod_rows)) `*_stride` elements apart (0: one row for all), each may be NULL; post_w, pre_w: fp32 [C]
+ * or NULL.  y NULL: r = x and is not written; h NULL: no norm behind the sum.  stats: fp32 [M, 4], written where given: what the
+ * backward pass needs besides its inputs.  C % 8 == 0, at most KSB_NORM_MAX_C.  Returns the number of kernels queued. */
+#define KSB_NORM_MAX_C 8192
+typedef struct ksb_sandwich_norm_args {
+  const void *x, *y, *gate, *scale, *shift;
+  const float *post_w, *pre_w;
+  float* stats;
+  int64_t M, C, mod_rows, ldx, ldy, gate_stride, scale_stride, shift_stride;
+  int dtype, layer;
+  float eps, residual_scale;
+} ksb_sandwich_norm_args;
+int ksb_sandwich_norm(const ksb_sandwich_norm_args* args, void* r, void* h, ksb_stream_t stream);
+/* Its gradients: from dr and dh (half, row strides lddr, lddh; one of them may be NULL = zeros) those asked for: dx, dy [M, C], dgate, dscale,
+ * dshift [mod_rows, C] half, contiguous; dpost_w, dpre_w fp32 [C].  args: as in the forward call, stats as it wrote them.  Sums over rows
+ * are fp32, in an order that depends on the shapes alone.  workspace: ksb_sandwich_norm_workspace bytes. */
+typedef struct ksb_sandwich_norm_grads {
+  const void *dr, *dh;
+  void *dx, *dy, *dgate, *dscale, *dshift;
+  float *dpost_w, *dpre_w;
+  int64_t lddr, lddh;
+} ksb_sandwich_norm_grads;
+int64_t ksb_sandwich_norm_workspace(int64_t M, int64_t C, int64_t mod_rows);
+int ksb_sandwich_norm_backward(const ksb_sandwich_norm_args* args, const ksb_sandwich_norm_grads* grads, void* workspace, ksb_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

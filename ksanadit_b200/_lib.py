@@ -74,6 +74,9 @@ SIGNATURES = {
     "ksb_qwen_block_forward": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p]),
     "ksb_w4_linear": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_void_p,
                               c_int64, c_void_p]),
+    "ksb_sandwich_norm": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p]),
+    "ksb_sandwich_norm_workspace": (c_int64, [c_int64, c_int64, c_int64]),
+    "ksb_sandwich_norm_backward": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p]),
 }
 
 _lib = None

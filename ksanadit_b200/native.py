@@ -225,3 +225,13 @@ def tile_lists(offsets, entries, order, n_blocks):
             pairs = 1
     keep = (offsets, entries, order)
     return TileLists(offsets.data_ptr(), entries.data_ptr(), None if order is None else order.data_ptr(), pairs), keep
+
+
+class NormArgs(ctypes.Structure):
+    _fields_ = [(n, c_void_p) for n in ("x", "y", "gate", "scale", "shift", "post_w", "pre_w", "stats")] + \
+        [(n, c_int64) for n in ("M", "C", "mod_rows", "ldx", "ldy", "gate_stride", "scale_stride", "shift_stride")] + \
+        [("dtype", c_int), ("layer", c_int), ("eps", c_float), ("residual_scale", c_float)]
+
+
+class NormGrads(ctypes.Structure):
+    _fields_ = [(n, c_void_p) for n in ("dr", "dh", "dx", "dy", "dgate", "dscale", "dshift", "dpost_w", "dpre_w")] + [("lddr", c_int64), ("lddh", c_int64)]

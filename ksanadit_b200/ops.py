@@ -684,3 +684,145 @@ def w4_linear(x, weight, weight_scale, weight_zero=None, bias=None, out_features
         x2.data_ptr(), dt, M, K, x2.stride(0), weight.data_ptr(), weight_scale.data_ptr(), _p(weight_zero), group, _p(bias), N, out.data_ptr(), N,
         _stream()), "ksb_w4_linear"))
     return out
+
+
+def _modulation(t, x):
+    """How many rows a modulation tensor has for x [..., C]: one for everything, or one for each index of x's leading axes up to some
+    axis.  [C], [1, C]; [B, 1, C], [B, C] or [B, L, C] for x [B, L, C]; any number that divides M for x [M, C]."""
+    C, lead = x.shape[-1], x.shape[:-1]
+    if t.dtype != x.dtype or t.dim() == 0 or t.shape[-1] != C:
+        raise _lib.KsanaB200Error(f"modulation must have {C} columns of x's type, {x.dtype}: got {tuple(t.shape)} {t.dtype}")
+    if t.numel() == C:
+        return 1
+    if t.dim() == 2:
+        n = t.shape[0]
+        if (len(lead) == 1 and n > 0 and lead[0] % n == 0) or (len(lead) > 1 and n == lead[0]) or n == lead[0] == 0:
+            return max(n, 1)
+    elif t.dim() == x.dim():
+        rows, i = 1, 0
+        while i < len(lead) and t.shape[i] == lead[i]:
+            rows *= lead[i]
+            i += 1
+        if all(s == 1 for s in t.shape[i:-1]):
+            return max(rows, 1)
+    raise _lib.KsanaB200Error(f"modulation {tuple(t.shape)} does not belong to rows {tuple(x.shape)}")
+
+
+def _modulation_rows(t, rows):
+    """(address, elements between rows, tensor) of a modulation tensor; a copy where its rows are not on 16-byte boundaries."""
+    if t is None:
+        return None, 0, None
+    t2 = t.reshape(-1, t.shape[-1])
+    n = t2.shape[0]
+    if t2.stride(1) != 1 or (n > 1 and t2.stride(0) % 8 != 0) or t2.data_ptr() % 16 != 0:
+        t2 = t2.clone(memory_format=torch.contiguous_format)
+    return t2.data_ptr(), t2.stride(0) if n == rows and n > 1 else 0, t2
+
+
+def _norm_launch(x, y, gate, scale, shift, post_weight, pre_weight, residual_scale, pre, layer, eps, mod_rows, want_stats):
+    C = x.shape[-1]
+    x2, y2 = _rows(x, C), None if y is None else _rows(y, C)
+    M = x2.shape[0]
+    (ga, gs, g2), (sa, ss, s2), (ha, hs, h2) = (_modulation_rows(t, mod_rows) for t in (gate, scale, shift))
+    stats = torch.empty(M, 4, dtype=torch.float32, device=x.device) if want_stats else None
+    r = x if y is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if pre else None
+    args = native.NormArgs(x2.data_ptr(), None if y2 is None else y2.data_ptr(), ga, sa, ha, _p(post_weight), _p(pre_weight), _p(stats), M, C, mod_rows,
+                           x2.stride(0), 0 if y2 is None else y2.stride(0), gs, ss, hs, _dt(x), int(layer), eps, residual_scale)
+    STATS.count(native.queued(_lib.load().ksb_sandwich_norm(ctypes.addressof(args), None if y is None else r.data_ptr(), _p(h), _stream()),
+                              "ksb_sandwich_norm"))
+    return r, h, stats, (x2, y2, g2, s2, h2)
+
+
+class _SandwichNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, y, gate, scale, shift, post_weight, pre_weight, residual_scale, pre, layer, eps, mod_rows):
+        r, h, stats, _ = _norm_launch(x, y, gate, scale, shift, post_weight, pre_weight, residual_scale, pre, layer, eps, mod_rows, True)
+        ctx.save_for_backward(x, y, gate, scale, shift, post_weight, pre_weight, stats)
+        ctx.plain = (residual_scale, pre, layer, eps, mod_rows)
+        ctx.set_materialize_grads(False)
+        return (None if y is None else r), h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dr, dh):
+        x, y, gate, scale, shift, post_weight, pre_weight, stats = ctx.saved_tensors
+        residual_scale, pre, layer, eps, mod_rows = ctx.plain
+        if dr is None and dh is None:
+            return (None,) * 12
+        C, device = x.shape[-1], x.device
+        with torch.cuda.device(device):
+            need = ctx.needs_input_grad
+            x2, y2 = _rows(x, C), None if y is None else _rows(y, C)
+            M = x2.shape[0]
+            mods = [_modulation_rows(t, mod_rows) for t in (gate, scale, shift)]
+            dr2, dh2 = (None if d is None else _rows(d, C) for d in (dr, dh))
+            dx = torch.empty(x.shape, dtype=x.dtype, device=device) if need[0] else None
+            dy = torch.empty(y.shape, dtype=x.dtype, device=device) if y is not None and need[1] else None
+            # without dh, what belongs to the norm behind the sum has no gradient
+            there = (y is not None, dh is not None, dh is not None)
+            dmods = [torch.empty(mod_rows, C, dtype=x.dtype, device=device) if n and t is not None and ok else None
+                     for n, t, ok in zip(need[2:5], (gate, scale, shift), there)]
+            dpost, dpre = (torch.empty(C, dtype=torch.float32, device=device) if n and w is not None and ok else None
+                           for n, w, ok in zip(need[5:7], (post_weight, pre_weight), there))
+            lib = _lib.load()
+            args = native.NormArgs(x2.data_ptr(), _p(y2), mods[0][0], mods[1][0], mods[2][0], _p(post_weight), _p(pre_weight), stats.data_ptr(), M, C, mod_rows,
+                                   x2.stride(0), 0 if y2 is None else y2.stride(0), mods[0][1], mods[1][1], mods[2][1], _dt(x), int(layer), eps, residual_scale)
+            grads = native.NormGrads(_p(dr2), _p(dh2), _p(dx), _p(dy), _p(dmods[0]), _p(dmods[1]), _p(dmods[2]), _p(dpost), _p(dpre),
+                                     0 if dr2 is None else dr2.stride(0), 0 if dh2 is None else dh2.stride(0))
+            ws = native.workspace(lib.ksb_sandwich_norm_workspace(M, C, mod_rows), device)
+            STATS.count(native.queued(lib.ksb_sandwich_norm_backward(ctypes.addressof(args), ctypes.addressof(grads), ws.data_ptr(), _stream()),
+                                      "ksb_sandwich_norm_backward"))
+            # a tensor with one row for rows that others of the call tell apart
+            out = []
+            for d, t in zip(dmods, (gate, scale, shift)):
+                if d is not None and d.numel() != t.numel():
+                    d = d.float().sum(0).to(t.dtype) if t.numel() else torch.empty_like(t)
+                out.append(None if d is None else d.view(t.shape))
+        return (dx, dy, *out, dpost, dpre, None, None, None, None, None)
+
+
+def sandwich_norm(x, y=None, *, gate=None, scale=None, shift=None, post_weight=None, pre_weight=None, residual_scale=1.0, pre=True, kind="rms", eps=1e-6):
+    """The norms on both sides of a block's half in one pass: behind it, with its gate and residual scale, and ahead of the next one.
+
+        r = x + residual_scale * gate * N(y) * post_weight
+        h = N(r) * pre_weight * (1 + scale) + shift              -> (r, h)
+
+    x, y [..., C] of one half type; N: RMSNorm (``kind="rms"``) or LayerNorm (``"layer"``) over the last axis.  gate, scale, shift: half,
+    [C], [1, C], or one row per leading index up to some axis ([B, 1, C], [B, C] or [B, L, C] for x [B, L, C]; any number that divides M
+    for x [M, C]).  post_weight, pre_weight: fp32 [C].  All optional; without y, r is x itself; with ``pre=False``, h is None.  C % 8 == 0, at
+    most 8192.  fp32 arithmetic, one rounding per result; h is the norm of the unrounded r.  Differentiable in all tensors."""
+    tensors = (x, y, gate, scale, shift, post_weight, pre_weight)
+    if kind not in ("rms", "layer"):
+        raise _lib.KsanaB200Error(f"kind must be 'rms' or 'layer', got {kind!r}")
+    _dt(x)
+    C = x.shape[-1] if x.dim() > 0 else 0
+    if x.dim() == 0 or C % 8 != 0 or not 0 < C <= 8192:
+        raise _lib.KsanaB200Error(f"the last axis must be a multiple of 8, at most 8192: got {tuple(x.shape)}")
+    if y is None and (not pre or gate is not None or post_weight is not None):
+        raise _lib.KsanaB200Error("without y there is only the norm of x: gate and post_weight belong to y")
+    if not pre and not (scale is None and shift is None and pre_weight is None):
+        raise _lib.KsanaB200Error("scale, shift and pre_weight belong to the norm that pre=False leaves out")
+    if y is not None and (y.shape != x.shape or y.dtype != x.dtype):
+        raise _lib.KsanaB200Error(f"y must be like x, {tuple(x.shape)} {x.dtype}: got {tuple(y.shape)} {y.dtype}")
+    for w in (post_weight, pre_weight):
+        if w is not None and (w.shape != (C,) or w.dtype != torch.float32 or w.stride(0) != 1 or w.data_ptr() % 16 != 0):
+            raise _lib.KsanaB200Error(f"norm weights must hold {C} adjacent fp32 values on a 16-byte boundary")
+    mod_rows = 1
+    for t in (gate, scale, shift):
+        if t is not None:
+            n = _modulation(t, x)
+            if n != 1 and mod_rows not in (1, n):
+                raise _lib.KsanaB200Error(f"gate, scale and shift have different numbers of rows: {mod_rows} and {n}")
+            mod_rows = max(mod_rows, n)
+    _one_device(*tensors)
+    if _elsewhere(x.device):
+        with torch.cuda.device(x.device):
+            return sandwich_norm(x, y, gate=gate, scale=scale, shift=shift, post_weight=post_weight, pre_weight=pre_weight, residual_scale=residual_scale,
+                                 pre=pre, kind=kind, eps=eps)
+    plain = (float(residual_scale), pre, kind == "layer", float(eps), mod_rows)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        r, h = _SandwichNorm.apply(*tensors, *plain)
+        return (x if y is None else r), h
+    r, h, _, _ = _norm_launch(*tensors, *plain, False)
+    return r, h
