@@ -1,0 +1,629 @@
+// The gated half of a feed-forward block, and its gradients, in 16-bit floating point on the Blackwell tensor cores:
+//
+//   g = x Wg^T + bg,  u = x Wu^T + bu,  h = act(g) u            act: SiLU or the tanh form of GELU, both v sigmoid(w(v))
+//   dg = dh u act'(g),  du = dh act(g)
+//   dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x,  dbg = sum of dg over rows,  dbu = sum of du
+//
+// Tensor-bound (4 M F K flop forward, 8 M F K more for the gradients) except for few rows, which only stream the weights.
+//
+// One persistent kernel does all three kinds of products: a thread copies tiles of A and B by TMA into a ring of stages, one thread issues
+// tcgen05.mma (kind::f16, fp32 accumulators in tensor memory, two of them so that one tile's output overlaps the next one's
+// products), the other warps take the accumulator through registers and shared memory to TMA stores.
+//   PROJECT  A = x, B = rows of Wg and, behind them, the same rows of Wu: a thread of the output holds g and u of the same element.
+//            In a CTA pair (cta_group::2, 256 x 256 tiles) the even CTA brings the rows of Wg, the odd one those of Wu.
+//   DX       two runs over F into one accumulator: A = dg, du as they lie, B = Wg, Wu read column by column (MN-major)
+//   DW       two problems of one launch: A = dg, du and B = x, all read column by column
+// A column-wise operand needs no transposed copy: a box of 64 columns x 64 rows lands in the layout that the tensor core reads as
+// MN-major with 128-byte swizzle.
+#include <algorithm>
+
+#include "../../include/ksana_b200.h"
+#include "common.cuh"
+#include "host_utils.h"
+
+namespace ksb {
+namespace gated {
+
+constexpr int KERNEL_ID = 5;
+constexpr int BM = 128, BK = 64, ROW_BYTES = BK * 2;  // a stage holds 64 columns of the sum: 128-byte rows
+enum Kind : int { PROJECT = 0, DX = 1, DW = 2 };
+
+// KIND: above.  CTAS: 1, or 2 = CTA pairs.  TN: columns of a tile's accumulator (PROJECT: half of them g, half u).  AR: rows of A that
+// are loaded (32 where M is no more: the products' other rows are of whatever lies there, and nobody reads them).
+template <int KIND, int CTAS, int TN, int AR> struct Cfg {
+  static constexpr int OUT_N = KIND == PROJECT ? TN / 2 : TN;  // columns of the output
+  static constexpr int PIECE_COLS = OUT_N < 64 ? OUT_N : 64;
+  static constexpr int PIECE_BYTES = 32 * PIECE_COLS * 2;
+  static constexpr int EW = 4 * (OUT_N / PIECE_COLS);  // output warps
+  static constexpr int THREADS = 64 + 32 * EW;
+  static constexpr int A_BYTES = AR * ROW_BYTES, B_ROWS = TN / CTAS, B_BYTES = B_ROWS * ROW_BYTES, STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int OUT_BYTES = EW * PIECE_BYTES;
+  static constexpr int SLACK = (BM - AR) * ROW_BYTES;  // what the last stage's products read behind the loaded rows
+  static constexpr int ROOM = 232448 - 1024 - (OUT_BYTES > SLACK ? OUT_BYTES : SLACK);
+  static constexpr int STAGES = ROOM / STAGE_BYTES > 24 ? 24 : ROOM / STAGE_BYTES;
+  static constexpr int TMEM_COLS = 2 * TN < 32 ? 32 : 2 * TN;
+  static constexpr int NUM_BARS = 2 * STAGES + 4;
+  // [STAGES x (A | B)][output pieces][barriers]
+  static constexpr int TAIL = OUT_BYTES > SLACK ? OUT_BYTES : SLACK;
+  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + TAIL + NUM_BARS * 8 + 16;
+  static_assert(SMEM_BYTES <= 232448 && STAGES >= 3, "shared memory");
+};
+
+struct Params {
+  CUtensorMap a[2], b[2], out[3];
+  int M, N;                       // of the output
+  int tiles_m, tiles_n, num_tiles, problem_tiles;
+  int steps, num_k;               // stages per run over the sum, and per tile
+  int group_m;                    // row tiles that go through all columns together
+  const void* b_gate;             // PROJECT: halves or null
+  const void* b_up;
+  int act, save;                  // PROJECT: save g and u as well
+  int* status;
+};
+
+__device__ __forceinline__ uint64_t mn_major_desc(uint32_t smem_addr) {
+  // blocks of 64 rows of the operand 8192 bytes apart (leading offset), groups of 8 columns of the sum 1024 bytes apart (stride offset)
+  uint64_t d = static_cast<uint64_t>((smem_addr & 0x3ffff) >> 4);
+  d |= static_cast<uint64_t>(8192 >> 4) << 16;
+  d |= static_cast<uint64_t>(1024 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(2) << 61;
+  return d;
+}
+// both operands of one type (0 = fp16, 1 = bf16), fp32 accumulator; bits 15 and 16: A, B column by column
+template <typename T> struct MmaType;
+template <> struct MmaType<__half> { static constexpr uint32_t value = 0; };
+template <> struct MmaType<__nv_bfloat16> { static constexpr uint32_t value = 1; };
+
+__device__ __forceinline__ void mma_f16_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// 16 consecutive columns
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+        "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+
+// Both activations are v s with s = sigmoid(w(v)): SiLU w = v; GELU (tanh form) w = 2 sqrt(2 / pi) (v + 0.044715 v^3), since
+// (1 + tanh z) / 2 = sigmoid(2 z).
+constexpr float GELU_C = 1.5957691216057308f, GELU_K = 0.044715f, NEG_LOG2E = -1.4426950408889634f;
+__device__ __forceinline__ float sigmoid_of(float w) {
+  float s;  // subnormal results kept: v s is a normal number where s is not any more
+  asm("rcp.approx.f32 %0, %1;" : "=f"(s) : "f"(1.f + fast_exp2(w * NEG_LOG2E)));
+  return s;
+}
+__device__ __forceinline__ float act_sigmoid(float v, int act) { return sigmoid_of(act == KSB_ACT_SILU ? v : GELU_C * fmaf(GELU_K * v * v, v, v)); }
+// act'(v) = s + v s (1 - s) w'(v); far out s (1 - s) is 0, and w' is kept finite
+__device__ __forceinline__ float act_slope(float v, float s, int act) {
+  const float c = fminf(fmaxf(v, -64.f), 64.f);
+  const float w = act == KSB_ACT_SILU ? 1.f : GELU_C * fmaf(3.f * GELU_K * c, c, 1.f);
+  return fmaf(c * s * (1.f - s), w, s);
+}
+
+__device__ __forceinline__ void tile_coords(const Params& p, int tile, int& problem, int& tm, int& tn) {
+  problem = tile / p.problem_tiles;
+  tile -= problem * p.problem_tiles;
+  const int per_group = p.group_m * p.tiles_n, rg = tile / per_group, first = rg * p.group_m;
+  const int rows = min(p.group_m, p.tiles_m - first), r = tile - rg * per_group;
+  tm = first + r % rows;
+  tn = r / rows;
+}
+
+template <typename T, int KIND, int CTAS, int TN, int AR>
+__global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, AR>::THREADS, 1) gemm_kernel(const __grid_constant__ Params p) {
+  using C = Cfg<KIND, CTAS, TN, AR>;
+  constexpr int STAGES = C::STAGES, STAGE_BYTES = C::STAGE_BYTES;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t base = smem_u32(smem);
+  const uint32_t pieces = base + STAGES * STAGE_BYTES, bars = pieces + C::TAIL;
+  const uint32_t full0 = bars, empty0 = full0 + 8 * STAGES, tfull0 = empty0 + 8 * STAGES, tempty0 = tfull0 + 16, tmem_slot = tempty0 + 16;
+  volatile uint32_t* tmem_slot_gen = reinterpret_cast<volatile uint32_t*>(smem + (tmem_slot - base));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t crank = CTAS == 2 ? cluster_ctarank() : 0u;
+  const int worker = CTAS == 2 ? blockIdx.x >> 1 : blockIdx.x, workers = CTAS == 2 ? gridDim.x >> 1 : gridDim.x;
+  if ((base & 1023u) != 0) {  // uniform over the grid
+    if (threadIdx.x == 0) report_error(p.status, KSB_ERR_BAD_SMEM_ALIGNMENT, (KERNEL_ID << 16) | 99);
+    return;
+  }
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(full0 + 8 * s, 1);   // the expecting arrival (of the even CTA in a pair) + the bytes
+      mbar_init(empty0 + 8 * s, 1);  // one commit
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(tfull0 + 8 * a, 1);
+      mbar_init(tempty0 + 8 * a, C::EW * CTAS);
+    }
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    if (CTAS == 2) {
+      tmem_alloc_pair(tmem_slot, C::TMEM_COLS);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(tmem_slot, C::TMEM_COLS);
+      tmem_relinquish();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (CTAS == 2) cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot_gen;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ loads
+    if (lane == 0) {
+      tma_prefetch_desc(&p.a[0]);
+      tma_prefetch_desc(&p.b[KIND == PROJECT ? crank : 0]);
+      pdl_wait();
+      uint32_t it = 0;
+      bool ok = true;
+      for (int tile = worker; tile < p.num_tiles && ok; tile += workers) {
+        int problem, tm, tn;
+        tile_coords(p, tile, problem, tm, tn);
+        const int row = (tm * CTAS + (int)crank) * BM;
+        for (int k = 0; k < p.num_k; ++k, ++it) {
+          const uint32_t s = it % STAGES, ph = (it / STAGES) & 1;
+          if (!mbar_wait(empty0 + 8 * s, ph ^ 1, p.status, (KERNEL_ID << 16) | 1)) { ok = false; break; }
+          if (CTAS == 1) mbar_arrive_expect_tx(full0 + 8 * s, STAGE_BYTES);
+          else if (crank == 0) mbar_arrive_expect_tx(full0 + 8 * s, 2 * STAGE_BYTES);
+          const uint32_t sa = base + s * STAGE_BYTES, sb = sa + C::A_BYTES;
+          auto load = [&](const CUtensorMap* map, uint32_t dst, int x, int y) {
+            if (CTAS == 2) tma_load_2d_pair(dst, map, mapa_shared(full0 + 8 * s, 0), x, y);
+            else tma_load_2d(dst, map, full0 + 8 * s, x, y);
+          };
+          if (KIND == PROJECT) {
+            load(&p.a[0], sa, k * BK, row);
+            if (CTAS == 2) {
+              load(&p.b[crank], sb, k * BK, tn * C::OUT_N);
+            } else {
+              load(&p.b[0], sb, k * BK, tn * C::OUT_N);
+              load(&p.b[1], sb + C::B_BYTES / 2, k * BK, tn * C::OUT_N);
+            }
+          } else {
+            const int run = KIND == DX && k >= p.steps, kk = (run ? k - p.steps : k) * BK, col = tn * TN + (int)crank * C::B_ROWS;
+            if (KIND == DX) {
+              load(&p.a[run], sa, kk, row);
+            } else {
+              load(&p.a[problem], sa, row, kk);
+              load(&p.a[problem], sa + 8192, row + 64, kk);
+            }
+#pragma unroll
+            for (int i = 0; i < C::B_ROWS / 64; ++i) load(&p.b[run], sb + i * 8192, col + 64 * i, kk);
+          }
+        }
+      }
+      // what is on its way lands before the block leaves (of a pair, the even CTA hears of it)
+      if (crank == 0)
+        for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i)
+          if (!mbar_wait(full0 + 8 * (i % STAGES), (i / STAGES) & 1, p.status, (KERNEL_ID << 16) | 5)) break;
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ products (in a pair: the even CTA's)
+    if (lane == 0 && crank == 0) {
+      constexpr bool a_mn = KIND == DW, b_mn = KIND != PROJECT;
+      constexpr uint32_t idesc = make_idesc(1, MmaType<T>::value, MmaType<T>::value, CTAS * BM, TN) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u);
+      uint32_t it = 0, count = 0;
+      bool ok = true;
+      for (int tile = worker; tile < p.num_tiles && ok; tile += workers, ++count) {
+        const uint32_t acc = count & 1, aph = (count >> 1) & 1;
+        if (!mbar_wait(tempty0 + 8 * acc, aph ^ 1, p.status, (KERNEL_ID << 16) | 2)) break;
+        tc_fence_after();
+        const uint32_t d = tmem_base + acc * TN;
+        for (int k = 0; k < p.num_k; ++k, ++it) {
+          const uint32_t s = it % STAGES, ph = (it / STAGES) & 1;
+          if (!mbar_wait(full0 + 8 * s, ph, p.status, (KERNEL_ID << 16) | 3)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t sa = base + s * STAGE_BYTES, sb = sa + C::A_BYTES;
+          const uint64_t da = a_mn ? mn_major_desc(sa) : make_kmajor_sw128_desc(sa), db = b_mn ? mn_major_desc(sb) : make_kmajor_sw128_desc(sb);
+#pragma unroll
+          for (int kk = 0; kk < BK / 16; ++kk) {  // 16 columns of the sum: 32 bytes of a row, or 16 rows of 128 bytes
+            const uint64_t ak = da + kk * (a_mn ? 128 : 2), bk = db + kk * (b_mn ? 128 : 2);
+            if (CTAS == 2) mma_f16_pair(d, ak, bk, idesc, (k | kk) != 0);
+            else mma_bf16_ss(d, ak, bk, idesc, (k | kk) != 0);
+          }
+          if (CTAS == 2) mma_commit_pair(empty0 + 8 * s); else mma_commit(empty0 + 8 * s);
+        }
+        if (ok) {
+          if (CTAS == 2) mma_commit_pair(tfull0 + 8 * acc); else mma_commit(tfull0 + 8 * acc);
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ output
+    pdl_wait();
+    pdl_release();
+    const int q = warp & 3, ew = warp - 2, col0 = (ew >> 2) * C::PIECE_COLS;  // lanes of tensor memory; the warp's columns of a tile
+    const uint32_t piece = pieces + ew * C::PIECE_BYTES;
+    constexpr int UNITS = C::PIECE_COLS / 8;  // of 16 bytes in a row of a piece
+    const int swizzle = UNITS == 8 ? lane & 7 : UNITS == 4 ? (lane >> 1) & 3 : 0;
+    const uint32_t piece_row = piece + lane * (C::PIECE_COLS * 2);
+    const uint32_t tempty_even = CTAS == 2 ? mapa_shared(tempty0, 0) : 0u;
+    uint32_t count = 0;
+    for (int tile = worker; tile < p.num_tiles; tile += workers, ++count) {
+      int problem, tm, tn;
+      tile_coords(p, tile, problem, tm, tn);
+      const uint32_t acc = count & 1, aph = (count >> 1) & 1;
+      if (!mbar_wait_warp(tfull0 + 8 * acc, aph, p.status, (KERNEL_ID << 16) | 4)) break;
+      tc_fence_after();
+      const int row0 = (tm * CTAS + (int)crank) * BM + q * 32, n0 = tn * C::OUT_N + col0;
+      if (row0 < p.M && n0 < p.N) {  // uniform over the warp
+        const uint32_t t_row = tmem_base + acc * TN + (static_cast<uint32_t>(q * 32) << 16) + col0;
+        // `f`(columns' values of the accumulator: 16 of g, or of the output; 16 of u; first column)
+        auto each16 = [&](bool second, auto&& f) {
+#pragma unroll
+          for (int c = 0; c < C::PIECE_COLS; c += 16) {
+            uint32_t v[16], w[16];
+            tmem_ld16(t_row + c, v);
+            if (KIND == PROJECT && second) tmem_ld16(t_row + TN / 2 + c, w);
+            tmem_wait_ld();
+            f(v, w, c);
+          }
+        };
+        auto put = [&](int c, const float (&y)[8]) {
+          st_shared_v4(piece_row + (((c >> 3) ^ swizzle) << 4), make_uint4(HalfOps<T>::pack2(make_float2(y[0], y[1])), HalfOps<T>::pack2(make_float2(y[2], y[3])),
+                                                                          HalfOps<T>::pack2(make_float2(y[4], y[5])), HalfOps<T>::pack2(make_float2(y[6], y[7]))));
+        };
+        auto open = [&]() {  // the piece's last store has read it
+          if (lane == 0) bulk_wait_source_read<0>();
+          __syncwarp();
+        };
+        auto close = [&](const CUtensorMap* map) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) tma_store_2d(map, piece, n0, row0);
+        };
+        if (KIND == PROJECT) {
+          // eight columns with their bias; the same for all lanes
+          auto with_bias = [&](const uint32_t* v, const void* bias, int c, float (&y)[8]) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = __uint_as_float(v[i]);
+            if (bias && n0 + c < p.N) {
+              const uint4 b = *reinterpret_cast<const uint4*>(static_cast<const T*>(bias) + n0 + c);
+              const uint32_t w[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float2 f = HalfOps<T>::unpack2(w[i]);
+                y[2 * i] += f.x;
+                y[2 * i + 1] += f.y;
+              }
+            }
+          };
+          if (p.save) {
+#pragma unroll 1
+            for (int which = 0; which < 2; ++which) {
+              open();
+#pragma unroll
+              for (int c = 0; c < C::PIECE_COLS; c += 16) {
+                uint32_t v[16];
+                tmem_ld16(t_row + which * (TN / 2) + c, v);
+                tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 16; e += 8) {
+                  float y[8];
+                  with_bias(v + e, which ? p.b_up : p.b_gate, c + e, y);
+                  put(c + e, y);
+                }
+              }
+              close(&p.out[1 + which]);
+            }
+          }
+          open();
+          each16(true, [&](const uint32_t (&v)[16], const uint32_t (&w)[16], int c) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 8) {
+              float g[8], u[8];
+              with_bias(v + e, p.b_gate, c + e, g);
+              with_bias(w + e, p.b_up, c + e, u);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) g[i] = g[i] * act_sigmoid(g[i], p.act) * u[i];
+              put(c + e, g);
+            }
+          });
+          close(&p.out[0]);
+        } else {
+          open();
+          each16(false, [&](const uint32_t (&v)[16], const uint32_t (&)[16], int c) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 8) {
+              float y[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) y[i] = __uint_as_float(v[e + i]);
+              put(c + e, y);
+            }
+          });
+          close(&p.out[problem]);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (CTAS == 2) mbar_arrive_cluster_relaxed(tempty_even + 8 * acc); else mbar_arrive(tempty0 + 8 * acc);
+      }
+    }
+    bulk_wait_all();  // no store of this thread may outlive the kernel's shared memory
+  }
+
+  // ------------------------------------------------------------------ common exit
+  tc_fence_before();
+  __syncthreads();
+  if (CTAS == 2) cluster_sync_all();
+  if (warp == 1) {
+    tc_fence_after();
+    if (CTAS == 2) tmem_dealloc_pair(tmem_base, C::TMEM_COLS); else tmem_dealloc(tmem_base, C::TMEM_COLS);
+  }
+}
+
+// dg and du, element by element, and a stretch of rows' sums of them: bound by HBM, 10 bytes per element.
+struct ActParams {
+  const void* dh;
+  const void* g;
+  const void* u;
+  void* dg;
+  void* du;
+  float* parts;  // [row stretches][2][F], or null
+  int64_t lddh, M, stretch;
+  int F, act;
+};
+template <typename T> __global__ void __launch_bounds__(256) act_grad_kernel(const __grid_constant__ ActParams p) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c * 8 >= p.F) return;
+  const int64_t first = blockIdx.y * p.stretch, last = first + p.stretch < p.M ? first + p.stretch : p.M;
+  float sg[8], su[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sg[i] = su[i] = 0.f;
+#pragma unroll 2
+  for (int64_t row = first; row < last; ++row) {
+    const int64_t at = row * p.F + c * 8;
+    const uint4 dv = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.dh) + row * p.lddh + c * 8);
+    const uint4 gv = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.g) + at), uv = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.u) + at);
+    const uint32_t dw[4] = {dv.x, dv.y, dv.z, dv.w}, gw[4] = {gv.x, gv.y, gv.z, gv.w}, uw[4] = {uv.x, uv.y, uv.z, uv.w};
+    uint32_t og[4], ou[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 d = HalfOps<T>::unpack2(dw[i]), g = HalfOps<T>::unpack2(gw[i]), u = HalfOps<T>::unpack2(uw[i]);
+      const float sx = act_sigmoid(g.x, p.act), sy = act_sigmoid(g.y, p.act);
+      const float2 dg = make_float2(d.x * u.x * act_slope(g.x, sx, p.act), d.y * u.y * act_slope(g.y, sy, p.act));
+      const float2 du = make_float2(d.x * g.x * sx, d.y * g.y * sy);
+      og[i] = HalfOps<T>::pack2(dg);
+      ou[i] = HalfOps<T>::pack2(du);
+      sg[2 * i] += dg.x;
+      sg[2 * i + 1] += dg.y;
+      su[2 * i] += du.x;
+      su[2 * i + 1] += du.y;
+    }
+    *reinterpret_cast<uint4*>(static_cast<T*>(p.dg) + at) = make_uint4(og[0], og[1], og[2], og[3]);
+    *reinterpret_cast<uint4*>(static_cast<T*>(p.du) + at) = make_uint4(ou[0], ou[1], ou[2], ou[3]);
+  }
+  if (p.parts) {
+    float* to = p.parts + static_cast<int64_t>(blockIdx.y) * 2 * p.F + c * 8;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float* s = h ? su : sg;
+      *reinterpret_cast<float4*>(to + h * p.F) = make_float4(s[0], s[1], s[2], s[3]);
+      *reinterpret_cast<float4*>(to + h * p.F + 4) = make_float4(s[4], s[5], s[6], s[7]);
+    }
+  }
+}
+// The bias gradients from the stretches' sums, in their order: 32 columns and 8 takers of turns per CTA.
+template <typename T> __global__ void __launch_bounds__(256) bias_grad_kernel(const float* parts, int stretches, int F, void* dbg, void* dbu) {
+  __shared__ float sums[8][33];
+  const int lane = threadIdx.x & 31, j = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
+  pdl_wait();
+  pdl_release();
+  float s = 0.f;
+  if (col < 2 * F)
+    for (int i = j; i < stretches; i += 8) s += parts[static_cast<int64_t>(i) * 2 * F + col];
+  sums[j][lane] = s;
+  __syncthreads();
+  if (j != 0 || col >= 2 * F) return;
+  s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s += sums[i][lane];
+  void* to = col < F ? dbg : dbu;
+  if (to) static_cast<T*>(to)[col < F ? col : col - F] = HalfOps<T>::from_f(s);
+}
+
+// ---------------------------------------------------------------------------------------------------------------- host side
+
+struct Operand {
+  const void* ptr;
+  int64_t rows, cols, ld;
+};
+static int map_of(CUtensorMap* m, const Operand& o, int box_cols, int box_rows) {
+  return encode_tmap_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, o.ptr, (uint64_t)o.cols, (uint64_t)o.rows, (uint64_t)o.ld * 2, (uint32_t)box_cols, (uint32_t)box_rows);
+}
+
+template <typename T, int KIND, int CTAS, int TN, int AR> static int launch_as(const Params& p, bool chained, cudaStream_t st) {
+  using C = Cfg<KIND, CTAS, TN, AR>;
+  auto kernel = gemm_kernel<T, KIND, CTAS, TN, AR>;
+  static DeviceOnce smem_limit;
+  if (int rc = smem_limit.raise_smem(reinterpret_cast<const void*>(kernel), C::SMEM_BYTES)) return rc;
+  const int workers = std::max(1, sm_count() / CTAS), grid = CTAS * std::min(p.num_tiles, workers);
+  return launch_kernel("gated linear", reinterpret_cast<const void*>(kernel), dim3((unsigned)grid), dim3(C::THREADS), C::SMEM_BYTES, st, CTAS, chained, p);
+}
+
+// A launch: operands as the kernel's kind wants them, outputs, and the columns that are summed over.
+struct Job {
+  Operand a[2], b[2], out[3];
+  int outs;
+  int64_t M, N, sum;
+  int problems;
+  Params p;
+};
+
+template <int KIND, int CTAS, int TN, int AR> static int launch_form(Job& j, int dtype, bool chained, cudaStream_t st) {
+  using C = Cfg<KIND, CTAS, TN, AR>;
+  Params& p = j.p;
+  p.status = status_words();
+  if (!p.status) return fail(KSB_ERR_CUDA, "status words unavailable");
+  const bool a_mn = KIND == DW, b_mn = KIND != PROJECT;
+  for (int i = 0; i < (KIND == PROJECT ? 1 : 2); ++i)
+    if (int rc = map_of(&p.a[i], j.a[i], BK, a_mn ? BK : AR)) return rc;
+  for (int i = 0; i < (KIND == DW ? 1 : 2); ++i)
+    if (int rc = map_of(&p.b[i], j.b[i], BK, b_mn ? BK : (KIND == PROJECT && CTAS == 1 ? TN / 2 : C::B_ROWS))) return rc;
+  for (int i = 0; i < j.outs; ++i)
+    if (int rc = map_of(&p.out[i], j.out[i], C::PIECE_COLS, 32)) return rc;
+  p.M = (int)j.M;
+  p.N = (int)j.N;
+  p.tiles_m = (int)((j.M + CTAS * BM - 1) / (CTAS * BM));
+  p.tiles_n = (int)((j.N + C::OUT_N - 1) / C::OUT_N);
+  const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n * j.problems;
+  if (tiles > INT32_MAX) return fail(KSB_ERR_UNSUPPORTED, "too many tiles");
+  p.problem_tiles = p.tiles_m * p.tiles_n;
+  p.num_tiles = (int)tiles;
+  p.steps = (int)((j.sum + BK - 1) / BK);
+  p.num_k = p.steps * (KIND == DX ? 2 : 1);
+  // Row tiles that share each column tile's operand while it is in L2; their own operand's rows are to take about 32 MB of it.
+  const int64_t row_bytes = (int64_t)CTAS * BM * p.num_k * ROW_BYTES;
+  p.group_m = (int)std::max<int64_t>(KIND == DW ? 8 : 4, std::min<int64_t>(64, (32ll << 20) / row_bytes));
+  return dtype == KSB_BF16 ? launch_as<__nv_bfloat16, KIND, CTAS, TN, AR>(p, chained, st) : launch_as<__half, KIND, CTAS, TN, AR>(p, chained, st);
+}
+
+static double waves(int64_t M, int64_t N, int tm, int tn, int workers, int problems) {
+  return (double)((((M + tm - 1) / tm) * ((N + tn - 1) / tn) * problems + workers - 1) / workers);
+}
+
+static int project(Job& j, int dtype, cudaStream_t st) {
+  if (j.M <= 32) return launch_form<PROJECT, 1, 32, 32>(j, dtype, false, st);
+  if (j.M <= 128) return launch_form<PROJECT, 1, 64, 128>(j, dtype, false, st);
+  const int sms = sm_count();
+  const double pair = sms < 2 ? 1e30 : waves(j.M, j.N, 256, 128, sms / 2, 1) * 2.0, single = waves(j.M, j.N, 128, 64, sms, 1) * 1.2;
+  return single < pair ? launch_form<PROJECT, 1, 128, 128>(j, dtype, false, st) : launch_form<PROJECT, 2, 256, 128>(j, dtype, false, st);
+}
+template <int KIND> static int gradient(Job& j, int dtype, cudaStream_t st) {
+  const int sms = sm_count();
+  const double pair = sms < 2 ? 1e30 : waves(j.M, j.N, 256, 256, sms / 2, j.problems) * 2.0, single = waves(j.M, j.N, 128, 128, sms, j.problems) * 1.2;
+  return single < pair ? launch_form<KIND, 1, 128, 128>(j, dtype, true, st) : launch_form<KIND, 2, 256, 128>(j, dtype, true, st);
+}
+
+static int64_t row_stretch(int64_t M, int64_t F) {
+  // rows per CTA: enough CTAs for four waves of eight per SM, at least 8 rows each
+  const int64_t columns = (F / 8 + 255) / 256, want = std::max<int64_t>(1, (int64_t)sm_count() * 32 / columns);
+  return std::max<int64_t>(8, (M + want - 1) / want);
+}
+
+}  // namespace gated
+}  // namespace ksb
+
+using namespace ksb;
+
+static int check_gated(int dtype, int64_t M, int64_t F, int64_t K, int act) {
+  if (dtype != KSB_BF16 && dtype != KSB_FP16) return fail(KSB_ERR_INVALID, "dtype must be KSB_BF16 or KSB_FP16");
+  if (act != KSB_ACT_SILU && act != KSB_ACT_GELU_TANH) return fail(KSB_ERR_INVALID, "unknown activation %d", act);
+  if (M < 0 || F <= 0 || K <= 0 || M > (1 << 30) || F > (1 << 30) || K > (1 << 30)) return fail(KSB_ERR_INVALID, "bad shape M=%lld F=%lld K=%lld", (long long)M, (long long)F, (long long)K);
+  if (F % 8 != 0 || K % 8 != 0) return fail(KSB_ERR_INVALID, "F and K must be multiples of 8 (F=%lld K=%lld)", (long long)F, (long long)K);
+  return 0;
+}
+static bool rows_ok(const void* p, int64_t ld, int64_t cols, int64_t rows) { return p && aligned16(p) && (rows <= 1 || (ld >= cols && ld % 8 == 0)); }
+
+extern "C" int ksb_gated_linear(const void* x, int64_t ldx, const void* w_gate, int64_t ldg, const void* w_up, int64_t ldu, const void* b_gate, const void* b_up,
+                                int dtype, int64_t M, int64_t F, int64_t K, int act, void* h, void* g, void* u, ksb_stream_t stream) {
+  if (int rc = check_gated(dtype, M, F, K, act)) return rc;
+  if (M == 0) return 0;
+  if (!rows_ok(x, ldx, K, M) || !rows_ok(w_gate, ldg, K, F) || !rows_ok(w_up, ldu, K, F) || !h || !aligned16(h) || !aligned16(b_gate) || !aligned16(b_up) || !aligned16(g) ||
+      !aligned16(u) || (!g) != (!u))
+    return fail(KSB_ERR_INVALID, "null or unaligned pointer, or rows not a multiple of 8 elements apart");
+  gated::Job j{};
+  j.a[0] = {x, M, K, M > 1 ? ldx : K};
+  j.b[0] = {w_gate, F, K, ldg};
+  j.b[1] = {w_up, F, K, ldu};
+  j.out[0] = {h, M, F, F};
+  j.out[1] = {g, M, F, F};
+  j.out[2] = {u, M, F, F};
+  j.outs = g ? 3 : 1;
+  j.M = M; j.N = F; j.sum = K; j.problems = 1;
+  j.p.b_gate = b_gate; j.p.b_up = b_up; j.p.act = act; j.p.save = g != nullptr;
+  if (int rc = gated::project(j, dtype, static_cast<cudaStream_t>(stream))) return rc;
+  return 1;
+}
+
+// [dg][du][sums of the bias gradients]
+static int64_t gated_bytes(int64_t M, int64_t F) { return (M * F * 2 + 255) / 256 * 256; }
+extern "C" int64_t ksb_gated_linear_workspace(int64_t M, int64_t F) {
+  if (M <= 0 || F <= 0 || F % 8 != 0) return 0;
+  const int64_t stretch = gated::row_stretch(M, F);
+  return 2 * gated_bytes(M, F) + (M + stretch - 1) / stretch * 2 * F * 4;
+}
+
+extern "C" int ksb_gated_linear_backward(const ksb_gated_linear_grads* a, void* workspace, ksb_stream_t stream) {
+  if (!a) return fail(KSB_ERR_INVALID, "null pointer");
+  const int64_t M = a->M, F = a->F, K = a->K;
+  if (int rc = check_gated(a->dtype, M, F, K, a->act)) return rc;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (M == 0) {  // sums over no rows
+    for (void* w : {a->dw_gate, a->dw_up})
+      if (w && cudaMemsetAsync(w, 0, (size_t)F * K * 2, st) != cudaSuccess) return fail(KSB_ERR_CUDA, "cannot clear the gradients");
+    for (void* b : {a->db_gate, a->db_up})
+      if (b && cudaMemsetAsync(b, 0, (size_t)F * 2, st) != cudaSuccess) return fail(KSB_ERR_CUDA, "cannot clear the gradients");
+    return 0;
+  }
+  const bool weights = a->dw_gate || a->dw_up;
+  if (!rows_ok(a->dh, a->lddh, F, M) || !rows_ok(a->g, F, F, M) || !rows_ok(a->u, F, F, M) || !workspace || !aligned16(workspace) ||
+      (weights && !rows_ok(a->x, a->ldx, K, M)) || (a->dx && (!rows_ok(a->w_gate, a->ldg, K, F) || !rows_ok(a->w_up, a->ldu, K, F))))
+    return fail(KSB_ERR_INVALID, "null or unaligned pointer, or rows not a multiple of 8 elements apart");
+  for (const void* t : {a->dx, a->dw_gate, a->dw_up})
+    if (!aligned16(t)) return fail(KSB_ERR_INVALID, "unaligned pointer");
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  void *dg = ws, *du = ws + gated_bytes(M, F);
+  const bool biases = a->db_gate || a->db_up;
+  const int before = launch_count();
+  gated::ActParams e{};
+  e.dh = a->dh; e.lddh = M > 1 ? a->lddh : F; e.g = a->g; e.u = a->u; e.dg = dg; e.du = du;
+  e.parts = biases ? reinterpret_cast<float*>(ws + 2 * gated_bytes(M, F)) : nullptr;
+  e.M = M; e.F = (int)F; e.act = a->act;
+  e.stretch = gated::row_stretch(M, F);
+  const int stretches = (int)((M + e.stretch - 1) / e.stretch);
+  const bool bf16 = a->dtype == KSB_BF16;
+  const dim3 grid((unsigned)((F / 8 + 255) / 256), (unsigned)stretches);
+  if (int rc = launch_kernel("gated linear", bf16 ? reinterpret_cast<const void*>(gated::act_grad_kernel<__nv_bfloat16>) : reinterpret_cast<const void*>(gated::act_grad_kernel<__half>),
+                             grid, dim3(256), 0, st, 1, false, e))
+    return rc;
+  if (biases) {
+    const float* parts = e.parts;
+    const int cols = (int)F;
+    void *dbg = a->db_gate, *dbu = a->db_up;
+    if (int rc = launch_kernel("gated linear", bf16 ? reinterpret_cast<const void*>(gated::bias_grad_kernel<__nv_bfloat16>) : reinterpret_cast<const void*>(gated::bias_grad_kernel<__half>),
+                               dim3((unsigned)((2 * F + 31) / 32)), dim3(256), 0, st, 1, true, parts, stretches, cols, dbg, dbu))
+      return rc;
+  }
+  if (a->dx) {
+    gated::Job j{};
+    j.a[0] = {dg, M, F, F};
+    j.a[1] = {du, M, F, F};
+    j.b[0] = {a->w_gate, F, K, a->ldg};
+    j.b[1] = {a->w_up, F, K, a->ldu};
+    j.out[0] = {a->dx, M, K, K};
+    j.outs = 1;
+    j.M = M; j.N = K; j.sum = F; j.problems = 1;
+    if (int rc = gated::gradient<gated::DX>(j, a->dtype, st)) return rc;
+  }
+  if (weights) {
+    gated::Job j{};
+    j.problems = 0;
+    for (int i = 0; i < 2; ++i) {
+      void* to = i ? a->dw_up : a->dw_gate;
+      if (!to) continue;
+      j.a[j.problems] = {i ? du : dg, M, F, F};
+      j.out[j.problems] = {to, F, K, K};
+      ++j.problems;
+    }
+    j.a[1] = j.problems == 2 ? j.a[1] : j.a[0];
+    j.outs = j.problems;
+    j.b[0] = {a->x, M, K, M > 1 ? a->ldx : K};
+    j.M = F; j.N = K; j.sum = M;
+    if (int rc = gated::gradient<gated::DW>(j, a->dtype, st)) return rc;
+  }
+  return launch_count() - before;
+}

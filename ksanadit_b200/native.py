@@ -235,3 +235,8 @@ class NormArgs(ctypes.Structure):
 
 class NormGrads(ctypes.Structure):
     _fields_ = [(n, c_void_p) for n in ("dr", "dh", "dx", "dy", "dgate", "dscale", "dshift", "dpost_w", "dpre_w")] + [("lddr", c_int64), ("lddh", c_int64)]
+
+
+class GatedGrads(ctypes.Structure):
+    _fields_ = [(n, c_void_p) for n in ("x", "w_gate", "w_up", "g", "u", "dh", "dx", "dw_gate", "dw_up", "db_gate", "db_up")] + \
+        [(n, c_int64) for n in ("M", "F", "K", "ldx", "ldg", "ldu", "lddh")] + [("dtype", c_int), ("act", c_int)]

@@ -826,3 +826,74 @@ def sandwich_norm(x, y=None, *, gate=None, scale=None, shift=None, post_weight=N
         return (x if y is None else r), h
     r, h, _, _ = _norm_launch(*tensors, *plain, False)
     return r, h
+
+
+ACTIVATIONS = {"silu": 0, "gelu_tanh": 1}
+
+
+def _gated_launch(x, w_gate, w_up, b_gate, b_up, act, save):
+    F, K = w_gate.shape
+    x2, wg, wu = _rows(x, K), _rows(w_gate, K), _rows(w_up, K)
+    M = x2.shape[0]
+    h = torch.empty(x.shape[:-1] + (F,), dtype=x.dtype, device=x.device)
+    g, u = (torch.empty(M, F, dtype=x.dtype, device=x.device) for _ in range(2)) if save else (None, None)
+    STATS.count(native.queued(_lib.load().ksb_gated_linear(
+        x2.data_ptr(), x2.stride(0), wg.data_ptr(), wg.stride(0), wu.data_ptr(), wu.stride(0), _p(b_gate), _p(b_up), _dt(x), M, F, K, act, h.data_ptr(),
+        _p(g), _p(u), _stream()), "ksb_gated_linear"))
+    return h, g, u
+
+
+class _GatedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, b_gate, b_up, act):
+        h, g, u = _gated_launch(x, w_gate, w_up, b_gate, b_up, act, True)
+        ctx.save_for_backward(x, w_gate, w_up, g, u)
+        ctx.act = act
+        return h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh):
+        x, w_gate, w_up, g, u = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        F, K = w_gate.shape
+        with torch.cuda.device(x.device):
+            x2, wg, wu, dh2 = _rows(x, K), _rows(w_gate, K), _rows(w_up, K), _rows(dh, F)
+            M = x2.shape[0]
+            out = [torch.empty(shape, dtype=x.dtype, device=x.device) if n else None
+                   for n, shape in zip(need, (x.shape, (F, K), (F, K), (F,), (F,)))]
+            lib = _lib.load()
+            args = native.GatedGrads(x2.data_ptr(), wg.data_ptr(), wu.data_ptr(), g.data_ptr(), u.data_ptr(), dh2.data_ptr(), *(_p(t) for t in out), M, F, K,
+                                     x2.stride(0), wg.stride(0), wu.stride(0), dh2.stride(0), _dt(x), ctx.act)
+            ws = native.workspace(lib.ksb_gated_linear_workspace(M, F), x.device)
+            STATS.count(native.queued(lib.ksb_gated_linear_backward(ctypes.addressof(args), ws.data_ptr(), _stream()), "ksb_gated_linear_backward"))
+        return (*out, None)
+
+
+def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, act="silu"):
+    """The gated half of a feed-forward block in one kernel: h = act(x w_gate^T + b_gate) * (x w_up^T + b_up).
+
+    x [..., K], w_gate and w_up [F, K], b_gate and b_up [F] or None, all of one half type -> h [..., F].  act: ``"silu"`` or ``"gelu_tanh"``.
+    K and F must be multiples of 8.  fp32 sums, one rounding of h.  Differentiable in all tensors: the two projections are kept in the half
+    type for the backward pass, whose products take their gradients in the half type too."""
+    if act not in ACTIVATIONS:
+        raise _lib.KsanaB200Error(f"act must be one of {sorted(ACTIVATIONS)}, got {act!r}")
+    _dt(x)
+    if w_gate.dim() != 2 or w_up.shape != w_gate.shape or x.dim() == 0 or x.shape[-1] != w_gate.shape[1]:
+        raise _lib.KsanaB200Error(f"gated_linear needs x [..., K] and two [F, K] weights: got {tuple(x.shape)}, {tuple(w_gate.shape)}, {tuple(w_up.shape)}")
+    F, K = w_gate.shape
+    if F % 8 != 0 or K % 8 != 0 or F == 0 or K == 0:
+        raise _lib.KsanaB200Error(f"K and F must be multiples of 8, got K={K} F={F}")
+    if w_gate.dtype != x.dtype or w_up.dtype != x.dtype:
+        raise _lib.KsanaB200Error(f"weights must be of x's type, {x.dtype}: got {w_gate.dtype} and {w_up.dtype}")
+    for b in (b_gate, b_up):
+        if b is not None and (b.shape != (F,) or b.dtype != x.dtype or b.stride(0) != 1 or b.data_ptr() % 16 != 0):
+            raise _lib.KsanaB200Error(f"biases must hold {F} adjacent values of x's type, {x.dtype}, on a 16-byte boundary")
+    tensors = (x, w_gate, w_up, b_gate, b_up)
+    _one_device(*tensors)
+    if _elsewhere(x.device):
+        with torch.cuda.device(x.device):
+            return gated_linear(x, w_gate, w_up, b_gate, b_up, act)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return _GatedLinear.apply(*tensors, ACTIVATIONS[act])
+    return _gated_launch(*tensors, ACTIVATIONS[act], False)[0]
