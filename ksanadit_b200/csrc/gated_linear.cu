@@ -6,7 +6,8 @@
 //
 // Tensor-bound (4 M F K flop forward, 8 M F K more for the gradients) except for few rows, which only stream the weights.
 //
-// One persistent kernel does all three kinds of products: a thread copies tiles of A and B by TMA into a ring of stages, one thread issues
+// One persistent kernel does all three kinds of products: a few threads, one per box of a stage, copy tiles of A and B by TMA into a ring
+// of stages (one thread for all boxes was the bound of narrow and of column-wise tiles: some 80 ns per box), one thread issues
 // tcgen05.mma (kind::f16, fp32 accumulators in tensor memory, two of them so that one tile's output overlaps the next one's
 // products), the other warps take the accumulator through registers and shared memory to TMA stores.
 //   PROJECT  A = x, B = rows of Wg and, behind them, the same rows of Wu: a thread of the output holds g and u of the same element.
@@ -17,8 +18,7 @@
 // MN-major with 128-byte swizzle.
 #include <algorithm>
 
-#include "../../include/ksana_b200.h"
-#include "common.cuh"
+#include "gated.h"
 #include "host_utils.h"
 
 namespace ksb {
@@ -35,7 +35,8 @@ template <int KIND, int CTAS, int TN, int AR> struct Cfg {
   static constexpr int PIECE_COLS = OUT_N < 64 ? OUT_N : 64;
   static constexpr int PIECE_BYTES = 32 * PIECE_COLS * 2;
   static constexpr int EW = 4 * (OUT_N / PIECE_COLS);  // output warps
-  static constexpr int THREADS = 64 + 32 * EW;
+  static constexpr int LOADS = KIND == PROJECT ? (CTAS == 2 ? 2 : 3) : KIND == DX ? 1 + TN / CTAS / 64 : 2 + TN / CTAS / 64;  // TMA boxes per stage
+  static constexpr int THREADS = 32 * (LOADS + 1 + EW);
   static constexpr int A_BYTES = AR * ROW_BYTES, B_ROWS = TN / CTAS, B_BYTES = B_ROWS * ROW_BYTES, STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int OUT_BYTES = EW * PIECE_BYTES;
   static constexpr int SLACK = (BM - AR) * ROW_BYTES;  // what the last stage's products read behind the loaded rows
@@ -94,22 +95,6 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
       : "memory");
 }
 
-// Both activations are v s with s = sigmoid(w(v)): SiLU w = v; GELU (tanh form) w = 2 sqrt(2 / pi) (v + 0.044715 v^3), since
-// (1 + tanh z) / 2 = sigmoid(2 z).
-constexpr float GELU_C = 1.5957691216057308f, GELU_K = 0.044715f, NEG_LOG2E = -1.4426950408889634f;
-__device__ __forceinline__ float sigmoid_of(float w) {
-  float s;  // subnormal results kept: v s is a normal number where s is not any more
-  asm("rcp.approx.f32 %0, %1;" : "=f"(s) : "f"(1.f + fast_exp2(w * NEG_LOG2E)));
-  return s;
-}
-__device__ __forceinline__ float act_sigmoid(float v, int act) { return sigmoid_of(act == KSB_ACT_SILU ? v : GELU_C * fmaf(GELU_K * v * v, v, v)); }
-// act'(v) = s + v s (1 - s) w'(v); far out s (1 - s) is 0, and w' is kept finite
-__device__ __forceinline__ float act_slope(float v, float s, int act) {
-  const float c = fminf(fmaxf(v, -64.f), 64.f);
-  const float w = act == KSB_ACT_SILU ? 1.f : GELU_C * fmaf(3.f * GELU_K * c, c, 1.f);
-  return fmaf(c * s * (1.f - s), w, s);
-}
-
 __device__ __forceinline__ void tile_coords(const Params& p, int tile, int& problem, int& tm, int& tn) {
   problem = tile / p.problem_tiles;
   tile -= problem * p.problem_tiles;
@@ -137,8 +122,8 @@ __global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, AR>::THREADS, 1) gemm_kern
   }
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(full0 + 8 * s, 1);   // the expecting arrival (of the even CTA in a pair) + the bytes
-      mbar_init(empty0 + 8 * s, 1);  // one commit
+      mbar_init(full0 + 8 * s, C::LOADS);  // the loaders' expecting arrivals (of the even CTA in a pair) + the bytes
+      mbar_init(empty0 + 8 * s, 1);         // one commit
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(tfull0 + 8 * a, 1);
@@ -146,7 +131,7 @@ __global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, AR>::THREADS, 1) gemm_kern
     }
     fence_barrier_init();
   }
-  if (warp == 1) {
+  if (warp == C::LOADS) {
     if (CTAS == 2) {
       tmem_alloc_pair(tmem_slot, C::TMEM_COLS);
       tmem_relinquish_pair();
@@ -161,47 +146,42 @@ __global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, AR>::THREADS, 1) gemm_kern
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot_gen;
 
-  if (warp == 0) {
-    // ------------------------------------------------------------------ loads
+  if (warp < C::LOADS) {
+    // ------------------------------------------------------------------ loads: box `warp` of every stage
     if (lane == 0) {
-      tma_prefetch_desc(&p.a[0]);
-      tma_prefetch_desc(&p.b[KIND == PROJECT ? crank : 0]);
+      constexpr int A_BOXES = KIND == DW ? 2 : 1, B_BOXES = C::LOADS - A_BOXES;
+      constexpr uint32_t BOX_A = C::A_BYTES / A_BOXES, BOX_B = C::B_BYTES / B_BOXES;
+      const bool of_a = warp < A_BOXES;
+      const int box = of_a ? warp : warp - A_BOXES;
+      const uint32_t bytes = of_a ? BOX_A : BOX_B, offset = of_a ? box * BOX_A : C::A_BYTES + box * BOX_B;
       pdl_wait();
       uint32_t it = 0;
       bool ok = true;
       for (int tile = worker; tile < p.num_tiles && ok; tile += workers) {
         int problem, tm, tn;
         tile_coords(p, tile, problem, tm, tn);
-        const int row = (tm * CTAS + (int)crank) * BM;
+        const int row = (tm * CTAS + (int)crank) * BM, col = tn * TN + (int)crank * C::B_ROWS;
         for (int k = 0; k < p.num_k; ++k, ++it) {
           const uint32_t s = it % STAGES, ph = (it / STAGES) & 1;
           if (!mbar_wait(empty0 + 8 * s, ph ^ 1, p.status, (KERNEL_ID << 16) | 1)) { ok = false; break; }
-          if (CTAS == 1) mbar_arrive_expect_tx(full0 + 8 * s, STAGE_BYTES);
-          else if (crank == 0) mbar_arrive_expect_tx(full0 + 8 * s, 2 * STAGE_BYTES);
-          const uint32_t sa = base + s * STAGE_BYTES, sb = sa + C::A_BYTES;
-          auto load = [&](const CUtensorMap* map, uint32_t dst, int x, int y) {
-            if (CTAS == 2) tma_load_2d_pair(dst, map, mapa_shared(full0 + 8 * s, 0), x, y);
-            else tma_load_2d(dst, map, full0 + 8 * s, x, y);
-          };
-          if (KIND == PROJECT) {
-            load(&p.a[0], sa, k * BK, row);
-            if (CTAS == 2) {
-              load(&p.b[crank], sb, k * BK, tn * C::OUT_N);
-            } else {
-              load(&p.b[0], sb, k * BK, tn * C::OUT_N);
-              load(&p.b[1], sb + C::B_BYTES / 2, k * BK, tn * C::OUT_N);
-            }
+          if (CTAS == 1) mbar_arrive_expect_tx(full0 + 8 * s, bytes);
+          else if (crank == 0) mbar_arrive_expect_tx(full0 + 8 * s, 2 * bytes);
+          const int run = KIND == DX && k >= p.steps;
+          const int kk = (run ? k - p.steps : k) * BK;
+          const CUtensorMap* map;
+          int x, y;
+          if (of_a) {
+            map = &p.a[KIND == DW ? problem : run];
+            x = KIND == DW ? row + 64 * box : kk;
+            y = KIND == DW ? kk : row;
           } else {
-            const int run = KIND == DX && k >= p.steps, kk = (run ? k - p.steps : k) * BK, col = tn * TN + (int)crank * C::B_ROWS;
-            if (KIND == DX) {
-              load(&p.a[run], sa, kk, row);
-            } else {
-              load(&p.a[problem], sa, row, kk);
-              load(&p.a[problem], sa + 8192, row + 64, kk);
-            }
-#pragma unroll
-            for (int i = 0; i < C::B_ROWS / 64; ++i) load(&p.b[run], sb + i * 8192, col + 64 * i, kk);
+            map = &p.b[KIND == PROJECT ? (CTAS == 2 ? (int)crank : box) : run];
+            x = KIND == PROJECT ? kk : col + 64 * box;
+            y = KIND == PROJECT ? tn * C::OUT_N : kk;
           }
+          const uint32_t dst = base + s * STAGE_BYTES + offset;
+          if (CTAS == 2) tma_load_2d_pair(dst, map, mapa_shared(full0 + 8 * s, 0), x, y);
+          else tma_load_2d(dst, map, full0 + 8 * s, x, y);
         }
       }
       // what is on its way lands before the block leaves (of a pair, the even CTA hears of it)
@@ -209,7 +189,7 @@ __global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, AR>::THREADS, 1) gemm_kern
         for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i)
           if (!mbar_wait(full0 + 8 * (i % STAGES), (i / STAGES) & 1, p.status, (KERNEL_ID << 16) | 5)) break;
     }
-  } else if (warp == 1) {
+  } else if (warp == C::LOADS) {
     // ------------------------------------------------------------------ products (in a pair: the even CTA's)
     if (lane == 0 && crank == 0) {
       constexpr bool a_mn = KIND == DW, b_mn = KIND != PROJECT;
@@ -244,7 +224,7 @@ __global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, AR>::THREADS, 1) gemm_kern
     // ------------------------------------------------------------------ output
     pdl_wait();
     pdl_release();
-    const int q = warp & 3, ew = warp - 2, col0 = (ew >> 2) * C::PIECE_COLS;  // lanes of tensor memory; the warp's columns of a tile
+    const int q = warp & 3, ew = warp - C::LOADS - 1, col0 = (ew >> 2) * C::PIECE_COLS;  // lanes of tensor memory; the warp's columns of a tile
     const uint32_t piece = pieces + ew * C::PIECE_BYTES;
     constexpr int UNITS = C::PIECE_COLS / 8;  // of 16 bytes in a row of a piece
     const int swizzle = UNITS == 8 ? lane & 7 : UNITS == 4 ? (lane >> 1) & 3 : 0;
@@ -260,16 +240,12 @@ __global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, AR>::THREADS, 1) gemm_kern
       const int row0 = (tm * CTAS + (int)crank) * BM + q * 32, n0 = tn * C::OUT_N + col0;
       if (row0 < p.M && n0 < p.N) {  // uniform over the warp
         const uint32_t t_row = tmem_base + acc * TN + (static_cast<uint32_t>(q * 32) << 16) + col0;
-        // `f`(columns' values of the accumulator: 16 of g, or of the output; 16 of u; first column)
-        auto each16 = [&](bool second, auto&& f) {
+        auto take16 = [&](uint32_t at, float (&v)[16]) {
+          uint32_t w[16];
+          tmem_ld16(at, w);
+          tmem_wait_ld();
 #pragma unroll
-          for (int c = 0; c < C::PIECE_COLS; c += 16) {
-            uint32_t v[16], w[16];
-            tmem_ld16(t_row + c, v);
-            if (KIND == PROJECT && second) tmem_ld16(t_row + TN / 2 + c, w);
-            tmem_wait_ld();
-            f(v, w, c);
-          }
+          for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(w[i]);
         };
         auto put = [&](int c, const float (&y)[8]) {
           st_shared_v4(piece_row + (((c >> 3) ^ swizzle) << 4), make_uint4(HalfOps<T>::pack2(make_float2(y[0], y[1])), HalfOps<T>::pack2(make_float2(y[2], y[3])),
@@ -286,9 +262,9 @@ __global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, AR>::THREADS, 1) gemm_kern
         };
         if (KIND == PROJECT) {
           // eight columns with their bias; the same for all lanes
-          auto with_bias = [&](const uint32_t* v, const void* bias, int c, float (&y)[8]) {
+          auto with_bias = [&](const float* v, const void* bias, int c, float (&y)[8]) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = __uint_as_float(v[i]);
+            for (int i = 0; i < 8; ++i) y[i] = v[i];
             if (bias && n0 + c < p.N) {
               const uint4 b = *reinterpret_cast<const uint4*>(static_cast<const T*>(bias) + n0 + c);
               const uint32_t w[4] = {b.x, b.y, b.z, b.w};
@@ -306,9 +282,8 @@ __global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, AR>::THREADS, 1) gemm_kern
               open();
 #pragma unroll
               for (int c = 0; c < C::PIECE_COLS; c += 16) {
-                uint32_t v[16];
-                tmem_ld16(t_row + which * (TN / 2) + c, v);
-                tmem_wait_ld();
+                float v[16];
+                take16(t_row + which * (TN / 2) + c, v);
 #pragma unroll
                 for (int e = 0; e < 16; e += 8) {
                   float y[8];
@@ -320,7 +295,11 @@ __global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, AR>::THREADS, 1) gemm_kern
             }
           }
           open();
-          each16(true, [&](const uint32_t (&v)[16], const uint32_t (&w)[16], int c) {
+#pragma unroll
+          for (int c = 0; c < C::PIECE_COLS; c += 16) {
+            float v[16], w[16];
+            take16(t_row + c, v);
+            take16(t_row + TN / 2 + c, w);
 #pragma unroll
             for (int e = 0; e < 16; e += 8) {
               float g[8], u[8];
@@ -330,19 +309,22 @@ __global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, AR>::THREADS, 1) gemm_kern
               for (int i = 0; i < 8; ++i) g[i] = g[i] * act_sigmoid(g[i], p.act) * u[i];
               put(c + e, g);
             }
-          });
+          }
           close(&p.out[0]);
         } else {
           open();
-          each16(false, [&](const uint32_t (&v)[16], const uint32_t (&)[16], int c) {
+#pragma unroll
+          for (int c = 0; c < C::PIECE_COLS; c += 16) {
+            float v[16];
+            take16(t_row + c, v);
 #pragma unroll
             for (int e = 0; e < 16; e += 8) {
               float y[8];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) y[i] = __uint_as_float(v[e + i]);
+              for (int i = 0; i < 8; ++i) y[i] = v[e + i];
               put(c + e, y);
             }
-          });
+          }
           close(&p.out[problem]);
         }
       }
@@ -359,7 +341,7 @@ __global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, AR>::THREADS, 1) gemm_kern
   tc_fence_before();
   __syncthreads();
   if (CTAS == 2) cluster_sync_all();
-  if (warp == 1) {
+  if (warp == C::LOADS) {
     tc_fence_after();
     if (CTAS == 2) tmem_dealloc_pair(tmem_base, C::TMEM_COLS); else tmem_dealloc(tmem_base, C::TMEM_COLS);
   }
@@ -496,10 +478,9 @@ static double waves(int64_t M, int64_t N, int tm, int tn, int workers, int probl
 }
 
 static int project(Job& j, int dtype, cudaStream_t st) {
-  if (j.M <= 32) return launch_form<PROJECT, 1, 32, 32>(j, dtype, false, st);
-  if (j.M <= 128) return launch_form<PROJECT, 1, 64, 128>(j, dtype, false, st);
   const int sms = sm_count();
   const double pair = sms < 2 ? 1e30 : waves(j.M, j.N, 256, 128, sms / 2, 1) * 2.0, single = waves(j.M, j.N, 128, 64, sms, 1) * 1.2;
+  if (j.M <= 128) return launch_form<PROJECT, 1, 256, 128>(j, dtype, false, st);
   return single < pair ? launch_form<PROJECT, 1, 128, 128>(j, dtype, false, st) : launch_form<PROJECT, 2, 256, 128>(j, dtype, false, st);
 }
 template <int KIND> static int gradient(Job& j, int dtype, cudaStream_t st) {
@@ -535,6 +516,12 @@ extern "C" int ksb_gated_linear(const void* x, int64_t ldx, const void* w_gate, 
   if (!rows_ok(x, ldx, K, M) || !rows_ok(w_gate, ldg, K, F) || !rows_ok(w_up, ldu, K, F) || !h || !aligned16(h) || !aligned16(b_gate) || !aligned16(b_up) || !aligned16(g) ||
       !aligned16(u) || (!g) != (!u))
     return fail(KSB_ERR_INVALID, "null or unaligned pointer, or rows not a multiple of 8 elements apart");
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (M <= gated::MAX_ROWS && !g) {
+    const gated::RowsCall call{x, w_gate, w_up, b_gate, b_up, h, ldx, ldg, ldu, (int)M, (int)F, (int)K, act};
+    const int rc = gated::run_rows(call, dtype, st);
+    if (rc != KSB_ERR_UNSUPPORTED) return rc ? rc : 1;  // else: no room for so many columns
+  }
   gated::Job j{};
   j.a[0] = {x, M, K, M > 1 ? ldx : K};
   j.b[0] = {w_gate, F, K, ldg};
@@ -545,7 +532,7 @@ extern "C" int ksb_gated_linear(const void* x, int64_t ldx, const void* w_gate, 
   j.outs = g ? 3 : 1;
   j.M = M; j.N = F; j.sum = K; j.problems = 1;
   j.p.b_gate = b_gate; j.p.b_up = b_up; j.p.act = act; j.p.save = g != nullptr;
-  if (int rc = gated::project(j, dtype, static_cast<cudaStream_t>(stream))) return rc;
+  if (int rc = gated::project(j, dtype, st)) return rc;
   return 1;
 }
 

@@ -91,7 +91,7 @@ def _call(t, act):
 
 # (rows, K, F): one row, the forms for few rows with ragged columns, one tile and its edges, single and paired tiles, odd sizes
 FORWARD = [(1, 8, 8), (1, 1536, 8960), (2, 72, 24), (31, 520, 136), (32, 64, 16), (33, 128, 264), (77, 1032, 1000), (128, 256, 64), (129, 64, 128), (200, 200, 1544),
-           (257, 328, 136), (1101, 136, 392), (1500, 264, 4616), (5000, 72, 1160), (3, 8200, 40)]
+           (257, 328, 136), (1, 5120, 13824), (5, 13824, 72), (16, 5120, 1504), (8, 1536, 1208), (9, 16400, 208), (1101, 136, 392), (1500, 264, 4616), (5000, 72, 1160), (3, 8200, 40)]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
@@ -119,7 +119,9 @@ def test_gradients(M, K, F, act, bias, dtype):
     ref, off = _reference(t, act, True)
     _compare("h", h, ref["h"], off["h"])
     with torch.no_grad():
-        assert torch.equal(_call(t, act), h)  # the same bits with and without what the backward pass keeps
+        alone = _call(t, act)
+    _compare("h", alone, ref["h"], off["h"])
+    assert M <= 16 or torch.equal(alone, h)  # the same kernel with and without what the backward pass keeps, but for few rows
     for name, g in zip(leaves, grads):
         assert g.shape == t[name].shape and g.dtype == dtype
         _compare(name, g, ref[name], off[name])
