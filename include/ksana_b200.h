@@ -453,17 +453,19 @@ int ksb_sandwich_norm_backward(const ksb_sandwich_norm_args* args, const ksb_san
 /* The gated half of a feed-forward block, both projections, the activation and the product in one kernel:
  *   h = act(x w_gate^T + b_gate) * (x w_up^T + b_up)
  * x: [M, K] half (row stride ldx); w_gate, w_up: [F, K] half (row strides ldg, ldu); b_gate, b_up: half [F] or NULL; h: [M, F] contiguous;
- * g, u: both NULL, or both [M, F] contiguous: the two projections with their biases, rounded, as the backward pass wants them.  fp32 sums;
- * h is formed from the unrounded projections and rounded once.  F % 8 == 0, K % 8 == 0.  Returns the number of kernels queued. */
+ * saved: NULL, or ksb_gated_linear_saved bytes for what the backward pass needs besides the inputs: the two projections with their
+ * biases, in 24 bits each.  fp32 sums; h is formed from the unrounded projections and rounded once.  F % 8 == 0, K % 8 == 0.  Returns the
+ * number of kernels queued. */
 #define KSB_ACT_SILU 0
 #define KSB_ACT_GELU_TANH 1
 int ksb_gated_linear(const void* x, int64_t ldx, const void* w_gate, int64_t ldg, const void* w_up, int64_t ldu, const void* b_gate, const void* b_up,
-                     int dtype, int64_t M, int64_t F, int64_t K, int act, void* h, void* g, void* u, ksb_stream_t stream);
+                     int dtype, int64_t M, int64_t F, int64_t K, int act, void* h, void* saved, ksb_stream_t stream);
+int64_t ksb_gated_linear_saved(int64_t M, int64_t F);
 /* Its gradients from dh [M, F] (row stride lddh), those that are asked for: dx [M, K], dw_gate, dw_up [F, K], db_gate, db_up [F], half,
- * contiguous.  g, u: as the forward call wrote them.  The gradients of the two projections are rounded to the half type, which is what the
+ * contiguous.  saved: as the forward call wrote it.  The gradients of the two projections are rounded to the half type, which is what the
  * tensor cores multiply; all sums are fp32.  workspace: ksb_gated_linear_workspace bytes.  Returns the number of kernels queued. */
 typedef struct ksb_gated_linear_grads {
-  const void *x, *w_gate, *w_up, *g, *u, *dh;
+  const void *x, *w_gate, *w_up, *saved, *dh;
   void *dx, *dw_gate, *dw_up, *db_gate, *db_up;
   int64_t M, F, K, ldx, ldg, ldu, lddh;
   int dtype, act;

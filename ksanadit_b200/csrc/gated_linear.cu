@@ -28,30 +28,27 @@ constexpr int KERNEL_ID = 5;
 constexpr int BM = 128, BK = 64, ROW_BYTES = BK * 2;  // a stage holds 64 columns of the sum: 128-byte rows
 enum Kind : int { PROJECT = 0, DX = 1, DW = 2 };
 
-// KIND: above.  CTAS: 1, or 2 = CTA pairs.  TN: columns of a tile's accumulator (PROJECT: half of them g, half u).  AR: rows of A that
-// are loaded (32 where M is no more: the products' other rows are of whatever lies there, and nobody reads them).
-template <int KIND, int CTAS, int TN, int AR> struct Cfg {
+// KIND: above.  CTAS: 1, or 2 = CTA pairs.  TN: columns of a tile's accumulator (PROJECT: half of them g, half u).  FLEX (PROJECT, single
+// CTAs): at most TN columns, how many is the launch's choice.
+template <int KIND, int CTAS, int TN, bool FLEX> struct Cfg {
   static constexpr int OUT_N = KIND == PROJECT ? TN / 2 : TN;  // columns of the output
-  static constexpr int PIECE_COLS = OUT_N < 64 ? OUT_N : 64;
-  static constexpr int PIECE_BYTES = 32 * PIECE_COLS * 2;
-  static constexpr int EW = 4 * (OUT_N / PIECE_COLS);  // output warps
+  static constexpr int PIECE_COLS = 64, PIECE_BYTES = 32 * PIECE_COLS * (KIND == PROJECT ? 3 : 2);  // PROJECT: a half's piece, and a byte's
+  static constexpr int EW = FLEX ? 4 : 4 * (OUT_N / PIECE_COLS);  // output warps
   static constexpr int LOADS = KIND == PROJECT ? (CTAS == 2 ? 2 : 3) : KIND == DX ? 1 + TN / CTAS / 64 : 2 + TN / CTAS / 64;  // TMA boxes per stage
   static constexpr int THREADS = 32 * (LOADS + 1 + EW);
-  static constexpr int A_BYTES = AR * ROW_BYTES, B_ROWS = TN / CTAS, B_BYTES = B_ROWS * ROW_BYTES, STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int OUT_BYTES = EW * PIECE_BYTES;
-  static constexpr int SLACK = (BM - AR) * ROW_BYTES;  // what the last stage's products read behind the loaded rows
-  static constexpr int ROOM = 232448 - 1024 - (OUT_BYTES > SLACK ? OUT_BYTES : SLACK);
-  static constexpr int STAGES = ROOM / STAGE_BYTES > 24 ? 24 : ROOM / STAGE_BYTES;
-  static constexpr int TMEM_COLS = 2 * TN < 32 ? 32 : 2 * TN;
-  static constexpr int NUM_BARS = 2 * STAGES + 4;
-  // [STAGES x (A | B)][output pieces][barriers]
-  static constexpr int TAIL = OUT_BYTES > SLACK ? OUT_BYTES : SLACK;
-  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + TAIL + NUM_BARS * 8 + 16;
+  static constexpr int A_BYTES = BM * ROW_BYTES, B_ROWS = TN / CTAS, B_BYTES = B_ROWS * ROW_BYTES, STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int OUT_BYTES = FLEX ? 0 : EW * PIECE_BYTES;
+  static constexpr int MOST = FLEX ? 10 : 6;  // stages
+  static constexpr int ROOM = 232448 - OUT_BYTES - (2 * MOST + 4) * 8 - 16;
+  static constexpr int STAGES = ROOM / STAGE_BYTES > MOST ? MOST : ROOM / STAGE_BYTES;
+  static constexpr int TMEM_COLS = 2 * TN;
+  // [stages x (A | B)][output pieces][barriers]
+  static constexpr int SMEM_BYTES = FLEX ? 232448 : STAGES * STAGE_BYTES + OUT_BYTES + (2 * STAGES + 4) * 8 + 16;
   static_assert(SMEM_BYTES <= 232448 && STAGES >= 3, "shared memory");
 };
 
 struct Params {
-  CUtensorMap a[2], b[2], out[3];
+  CUtensorMap a[2], b[2], out[5];  // PROJECT with `save`: h, upper and lower part of g, of u
   int M, N;                       // of the output
   int tiles_m, tiles_n, num_tiles, problem_tiles;
   int steps, num_k;               // stages per run over the sum, and per tile
@@ -59,6 +56,8 @@ struct Params {
   const void* b_gate;             // PROJECT: halves or null
   const void* b_up;
   int act, save;                  // PROJECT: save g and u as well
+  int flex_cols, stages;          // FLEX: columns of the output per tile, stages
+  void* h;                        // FLEX
   int* status;
 };
 
@@ -95,6 +94,37 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
       : "memory");
 }
 
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(taddr) : "memory");
+}
+
+// g and u are kept for the backward pass as the upper 24 bits of their fp32 values, rounded (a plane of the upper 16, one of the next 8):
+// kept in the half type they would put as much into the gradients' error as the rounding of dg and du that the tensor cores ask for.
+__device__ __forceinline__ uint32_t round24(float v) { return v != v ? 0x7fc00000u : __float_as_uint(v) + 0x80u; }
+__device__ __forceinline__ uint32_t high2(const uint32_t* r) { return __byte_perm(r[0], r[1], 0x7632); }
+__device__ __forceinline__ uint32_t low4(const uint32_t* r) { return __byte_perm(__byte_perm(r[0], r[1], 0x0051), __byte_perm(r[2], r[3], 0x0051), 0x5410); }
+// eight of them back
+__device__ __forceinline__ void from24(const uint4& high, const uint2& low, float (&v)[8]) {
+  const uint32_t h[4] = {high.x, high.y, high.z, high.w}, l[2] = {low.x, low.y};
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    v[i] = __uint_as_float(h[i / 2] << 16 | (l[i / 4] >> (i % 4 * 8) & 0xffu) << 8);
+    v[i + 1] = __uint_as_float((h[i / 2] & 0xffff0000u) | (l[i / 4] >> (i % 4 * 8 + 8) & 0xffu) << 8);
+  }
+}
+struct Saved {  // offsets of the planes, bytes
+  int64_t low_ld, low, u, bytes;
+};
+static Saved saved_layout(int64_t M, int64_t F) {
+  Saved s;
+  s.low_ld = (F + 15) / 16 * 16;
+  s.low = (M * F * 2 + 255) / 256 * 256;
+  s.u = s.low + (M * s.low_ld + 255) / 256 * 256;
+  s.bytes = 2 * s.u;
+  return s;
+}
+
 __device__ __forceinline__ void tile_coords(const Params& p, int tile, int& problem, int& tm, int& tn) {
   problem = tile / p.problem_tiles;
   tile -= problem * p.problem_tiles;
@@ -104,13 +134,14 @@ __device__ __forceinline__ void tile_coords(const Params& p, int tile, int& prob
   tn = r / rows;
 }
 
-template <typename T, int KIND, int CTAS, int TN, int AR>
-__global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, AR>::THREADS, 1) gemm_kernel(const __grid_constant__ Params p) {
-  using C = Cfg<KIND, CTAS, TN, AR>;
-  constexpr int STAGES = C::STAGES, STAGE_BYTES = C::STAGE_BYTES;
+template <typename T, int KIND, int CTAS, int TN, bool FLEX>
+__global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, FLEX>::THREADS, 1) gemm_kernel(const __grid_constant__ Params p) {
+  using C = Cfg<KIND, CTAS, TN, FLEX>;
+  const int OUT_N = FLEX ? p.flex_cols : C::OUT_N;
+  const uint32_t STAGES = FLEX ? p.stages : C::STAGES, B_BYTES = FLEX ? p.flex_cols * 2 * ROW_BYTES : C::B_BYTES, STAGE_BYTES = C::A_BYTES + B_BYTES;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t base = smem_u32(smem);
-  const uint32_t pieces = base + STAGES * STAGE_BYTES, bars = pieces + C::TAIL;
+  const uint32_t pieces = base + STAGES * STAGE_BYTES, bars = pieces + C::OUT_BYTES;
   const uint32_t full0 = bars, empty0 = full0 + 8 * STAGES, tfull0 = empty0 + 8 * STAGES, tempty0 = tfull0 + 16, tmem_slot = tempty0 + 16;
   volatile uint32_t* tmem_slot_gen = reinterpret_cast<volatile uint32_t*>(smem + (tmem_slot - base));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -150,20 +181,19 @@ __global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, AR>::THREADS, 1) gemm_kern
     // ------------------------------------------------------------------ loads: box `warp` of every stage
     if (lane == 0) {
       constexpr int A_BOXES = KIND == DW ? 2 : 1, B_BOXES = C::LOADS - A_BOXES;
-      constexpr uint32_t BOX_A = C::A_BYTES / A_BOXES, BOX_B = C::B_BYTES / B_BOXES;
+      const uint32_t BOX_A = C::A_BYTES / A_BOXES, BOX_B = B_BYTES / B_BOXES;
       const bool of_a = warp < A_BOXES;
       const int box = of_a ? warp : warp - A_BOXES;
       const uint32_t bytes = of_a ? BOX_A : BOX_B, offset = of_a ? box * BOX_A : C::A_BYTES + box * BOX_B;
       pdl_wait();
-      uint32_t it = 0;
+      uint32_t it = 0, s = 0, ph = 1;
       bool ok = true;
       for (int tile = worker; tile < p.num_tiles && ok; tile += workers) {
         int problem, tm, tn;
         tile_coords(p, tile, problem, tm, tn);
         const int row = (tm * CTAS + (int)crank) * BM, col = tn * TN + (int)crank * C::B_ROWS;
         for (int k = 0; k < p.num_k; ++k, ++it) {
-          const uint32_t s = it % STAGES, ph = (it / STAGES) & 1;
-          if (!mbar_wait(empty0 + 8 * s, ph ^ 1, p.status, (KERNEL_ID << 16) | 1)) { ok = false; break; }
+          if (!mbar_wait(empty0 + 8 * s, ph, p.status, (KERNEL_ID << 16) | 1)) { ok = false; break; }
           if (CTAS == 1) mbar_arrive_expect_tx(full0 + 8 * s, bytes);
           else if (crank == 0) mbar_arrive_expect_tx(full0 + 8 * s, 2 * bytes);
           const int run = KIND == DX && k >= p.steps;
@@ -177,11 +207,15 @@ __global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, AR>::THREADS, 1) gemm_kern
           } else {
             map = &p.b[KIND == PROJECT ? (CTAS == 2 ? (int)crank : box) : run];
             x = KIND == PROJECT ? kk : col + 64 * box;
-            y = KIND == PROJECT ? tn * C::OUT_N : kk;
+            y = KIND == PROJECT ? tn * OUT_N : kk;
           }
           const uint32_t dst = base + s * STAGE_BYTES + offset;
           if (CTAS == 2) tma_load_2d_pair(dst, map, mapa_shared(full0 + 8 * s, 0), x, y);
           else tma_load_2d(dst, map, full0 + 8 * s, x, y);
+          if (++s == STAGES) {
+            s = 0;
+            ph ^= 1;
+          }
         }
       }
       // what is on its way lands before the block leaves (of a pair, the even CTA hears of it)
@@ -193,16 +227,15 @@ __global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, AR>::THREADS, 1) gemm_kern
     // ------------------------------------------------------------------ products (in a pair: the even CTA's)
     if (lane == 0 && crank == 0) {
       constexpr bool a_mn = KIND == DW, b_mn = KIND != PROJECT;
-      constexpr uint32_t idesc = make_idesc(1, MmaType<T>::value, MmaType<T>::value, CTAS * BM, TN) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u);
-      uint32_t it = 0, count = 0;
+      const uint32_t idesc = make_idesc(1, MmaType<T>::value, MmaType<T>::value, CTAS * BM, FLEX ? 2 * OUT_N : TN) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u);
+      uint32_t s = 0, ph = 0, count = 0;
       bool ok = true;
       for (int tile = worker; tile < p.num_tiles && ok; tile += workers, ++count) {
         const uint32_t acc = count & 1, aph = (count >> 1) & 1;
         if (!mbar_wait(tempty0 + 8 * acc, aph ^ 1, p.status, (KERNEL_ID << 16) | 2)) break;
         tc_fence_after();
         const uint32_t d = tmem_base + acc * TN;
-        for (int k = 0; k < p.num_k; ++k, ++it) {
-          const uint32_t s = it % STAGES, ph = (it / STAGES) & 1;
+        for (int k = 0; k < p.num_k; ++k) {
           if (!mbar_wait(full0 + 8 * s, ph, p.status, (KERNEL_ID << 16) | 3)) { ok = false; break; }
           tc_fence_after();
           const uint32_t sa = base + s * STAGE_BYTES, sb = sa + C::A_BYTES;
@@ -214,6 +247,10 @@ __global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, AR>::THREADS, 1) gemm_kern
             else mma_bf16_ss(d, ak, bk, idesc, (k | kk) != 0);
           }
           if (CTAS == 2) mma_commit_pair(empty0 + 8 * s); else mma_commit(empty0 + 8 * s);
+          if (++s == STAGES) {
+            s = 0;
+            ph ^= 1;
+          }
         }
         if (ok) {
           if (CTAS == 2) mma_commit_pair(tfull0 + 8 * acc); else mma_commit(tfull0 + 8 * acc);
@@ -226,8 +263,6 @@ __global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, AR>::THREADS, 1) gemm_kern
     pdl_release();
     const int q = warp & 3, ew = warp - C::LOADS - 1, col0 = (ew >> 2) * C::PIECE_COLS;  // lanes of tensor memory; the warp's columns of a tile
     const uint32_t piece = pieces + ew * C::PIECE_BYTES;
-    constexpr int UNITS = C::PIECE_COLS / 8;  // of 16 bytes in a row of a piece
-    const int swizzle = UNITS == 8 ? lane & 7 : UNITS == 4 ? (lane >> 1) & 3 : 0;
     const uint32_t piece_row = piece + lane * (C::PIECE_COLS * 2);
     const uint32_t tempty_even = CTAS == 2 ? mapa_shared(tempty0, 0) : 0u;
     uint32_t count = 0;
@@ -237,7 +272,7 @@ __global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, AR>::THREADS, 1) gemm_kern
       const uint32_t acc = count & 1, aph = (count >> 1) & 1;
       if (!mbar_wait_warp(tfull0 + 8 * acc, aph, p.status, (KERNEL_ID << 16) | 4)) break;
       tc_fence_after();
-      const int row0 = (tm * CTAS + (int)crank) * BM + q * 32, n0 = tn * C::OUT_N + col0;
+      const int row0 = (tm * CTAS + (int)crank) * BM + q * 32, n0 = tn * OUT_N + col0;
       if (row0 < p.M && n0 < p.N) {  // uniform over the warp
         const uint32_t t_row = tmem_base + acc * TN + (static_cast<uint32_t>(q * 32) << 16) + col0;
         auto take16 = [&](uint32_t at, float (&v)[16]) {
@@ -248,7 +283,7 @@ __global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, AR>::THREADS, 1) gemm_kern
           for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(w[i]);
         };
         auto put = [&](int c, const float (&y)[8]) {
-          st_shared_v4(piece_row + (((c >> 3) ^ swizzle) << 4), make_uint4(HalfOps<T>::pack2(make_float2(y[0], y[1])), HalfOps<T>::pack2(make_float2(y[2], y[3])),
+          st_shared_v4(piece_row + (((c >> 3) ^ (lane & 7)) << 4), make_uint4(HalfOps<T>::pack2(make_float2(y[0], y[1])), HalfOps<T>::pack2(make_float2(y[2], y[3])),
                                                                           HalfOps<T>::pack2(make_float2(y[4], y[5])), HalfOps<T>::pack2(make_float2(y[6], y[7]))));
         };
         auto open = [&]() {  // the piece's last store has read it
@@ -276,22 +311,53 @@ __global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, AR>::THREADS, 1) gemm_kern
               }
             }
           };
+          if constexpr (FLEX) {
+            // few rows: straight to memory
+            const int row = row0 + lane;
+            for (int c = 0; c < OUT_N; c += 8) {
+              uint32_t v[8], w[8];
+              tmem_ld8(t_row + c, v);
+              tmem_ld8(t_row + OUT_N + c, w);
+              tmem_wait_ld();
+              if (row >= p.M || n0 + c >= p.N) continue;
+              float fv[8], fw[8], g[8], u[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                fv[i] = __uint_as_float(v[i]);
+                fw[i] = __uint_as_float(w[i]);
+              }
+              with_bias(fv, p.b_gate, c, g);
+              with_bias(fw, p.b_up, c, u);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) g[i] = g[i] * act_sigmoid(g[i], p.act) * u[i];
+              *reinterpret_cast<uint4*>(static_cast<T*>(p.h) + static_cast<int64_t>(row) * p.N + n0 + c) =
+                  make_uint4(HalfOps<T>::pack2(make_float2(g[0], g[1])), HalfOps<T>::pack2(make_float2(g[2], g[3])), HalfOps<T>::pack2(make_float2(g[4], g[5])),
+                             HalfOps<T>::pack2(make_float2(g[6], g[7])));
+            }
+          } else {
           if (p.save) {
+            // the upper 24 bits of each fp32 value, as two planes
+            const uint32_t low_row = piece + 32 * C::PIECE_COLS * 2 + lane * 64;
 #pragma unroll 1
-            for (int which = 0; which < 2; ++which) {
+            for (int up = 0; up < 2; ++up) {
               open();
 #pragma unroll
               for (int c = 0; c < C::PIECE_COLS; c += 16) {
                 float v[16];
-                take16(t_row + which * (TN / 2) + c, v);
+                take16(t_row + up * (TN / 2) + c, v);
+                uint32_t r[16];
 #pragma unroll
                 for (int e = 0; e < 16; e += 8) {
                   float y[8];
-                  with_bias(v + e, which ? p.b_up : p.b_gate, c + e, y);
-                  put(c + e, y);
+                  with_bias(v + e, up ? p.b_up : p.b_gate, c + e, y);
+#pragma unroll
+                  for (int i = 0; i < 8; ++i) r[e + i] = round24(y[i]);
+                  st_shared_v4(piece_row + ((((c + e) >> 3) ^ (lane & 7)) << 4), make_uint4(high2(r + e), high2(r + e + 2), high2(r + e + 4), high2(r + e + 6)));
                 }
+                st_shared_v4(low_row + (((c >> 4) ^ ((lane >> 1) & 3)) << 4), make_uint4(low4(r), low4(r + 4), low4(r + 8), low4(r + 12)));
               }
-              close(&p.out[1 + which]);
+              close(&p.out[1 + 2 * up]);
+              if (lane == 0) tma_store_2d(&p.out[2 + 2 * up], piece + 32 * C::PIECE_COLS * 2, n0, row0);
             }
           }
           open();
@@ -311,6 +377,7 @@ __global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, AR>::THREADS, 1) gemm_kern
             }
           }
           close(&p.out[0]);
+          }
         } else {
           open();
 #pragma unroll
@@ -347,15 +414,15 @@ __global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, AR>::THREADS, 1) gemm_kern
   }
 }
 
-// dg and du, element by element, and a stretch of rows' sums of them: bound by HBM, 10 bytes per element.
+// dg and du, element by element, and a stretch of rows' sums of them: bound by HBM, 12 bytes per element.
 struct ActParams {
   const void* dh;
-  const void* g;
-  const void* u;
+  const uint8_t* saved;
   void* dg;
   void* du;
   float* parts;  // [row stretches][2][F], or null
   int64_t lddh, M, stretch;
+  int64_t low_ld, low, u;  // planes of what is saved
   int F, act;
 };
 template <typename T> __global__ void __launch_bounds__(256) act_grad_kernel(const __grid_constant__ ActParams p) {
@@ -369,12 +436,15 @@ template <typename T> __global__ void __launch_bounds__(256) act_grad_kernel(con
   for (int64_t row = first; row < last; ++row) {
     const int64_t at = row * p.F + c * 8;
     const uint4 dv = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.dh) + row * p.lddh + c * 8);
-    const uint4 gv = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.g) + at), uv = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.u) + at);
-    const uint32_t dw[4] = {dv.x, dv.y, dv.z, dv.w}, gw[4] = {gv.x, gv.y, gv.z, gv.w}, uw[4] = {uv.x, uv.y, uv.z, uv.w};
+    const uint8_t *hp = p.saved + at * 2, *lp = p.saved + p.low + row * p.low_ld + c * 8;
+    float gf[8], uf[8];
+    from24(*reinterpret_cast<const uint4*>(hp), *reinterpret_cast<const uint2*>(lp), gf);
+    from24(*reinterpret_cast<const uint4*>(hp + p.u), *reinterpret_cast<const uint2*>(lp + p.u), uf);
+    const uint32_t dw[4] = {dv.x, dv.y, dv.z, dv.w};
     uint32_t og[4], ou[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2 d = HalfOps<T>::unpack2(dw[i]), g = HalfOps<T>::unpack2(gw[i]), u = HalfOps<T>::unpack2(uw[i]);
+      const float2 d = HalfOps<T>::unpack2(dw[i]), g = make_float2(gf[2 * i], gf[2 * i + 1]), u = make_float2(uf[2 * i], uf[2 * i + 1]);
       const float sx = act_sigmoid(g.x, p.act), sy = act_sigmoid(g.y, p.act);
       const float2 dg = make_float2(d.x * u.x * act_slope(g.x, sx, p.act), d.y * u.y * act_slope(g.y, sy, p.act));
       const float2 du = make_float2(d.x * g.x * sx, d.y * g.y * sy);
@@ -423,13 +493,14 @@ struct Operand {
   const void* ptr;
   int64_t rows, cols, ld;
 };
-static int map_of(CUtensorMap* m, const Operand& o, int box_cols, int box_rows) {
-  return encode_tmap_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, o.ptr, (uint64_t)o.cols, (uint64_t)o.rows, (uint64_t)o.ld * 2, (uint32_t)box_cols, (uint32_t)box_rows);
+static int map_of(CUtensorMap* m, const Operand& o, int box_cols, int box_rows, int elem = 2) {
+  return encode_tmap_2d(m, elem == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, elem, o.ptr, (uint64_t)o.cols, (uint64_t)o.rows, (uint64_t)o.ld * elem,
+                        (uint32_t)box_cols, (uint32_t)box_rows);
 }
 
-template <typename T, int KIND, int CTAS, int TN, int AR> static int launch_as(const Params& p, bool chained, cudaStream_t st) {
-  using C = Cfg<KIND, CTAS, TN, AR>;
-  auto kernel = gemm_kernel<T, KIND, CTAS, TN, AR>;
+template <typename T, int KIND, int CTAS, int TN, bool FLEX> static int launch_as(const Params& p, bool chained, cudaStream_t st) {
+  using C = Cfg<KIND, CTAS, TN, FLEX>;
+  auto kernel = gemm_kernel<T, KIND, CTAS, TN, FLEX>;
   static DeviceOnce smem_limit;
   if (int rc = smem_limit.raise_smem(reinterpret_cast<const void*>(kernel), C::SMEM_BYTES)) return rc;
   const int workers = std::max(1, sm_count() / CTAS), grid = CTAS * std::min(p.num_tiles, workers);
@@ -438,55 +509,68 @@ template <typename T, int KIND, int CTAS, int TN, int AR> static int launch_as(c
 
 // A launch: operands as the kernel's kind wants them, outputs, and the columns that are summed over.
 struct Job {
-  Operand a[2], b[2], out[3];
+  Operand a[2], b[2], out[5];
   int outs;
   int64_t M, N, sum;
   int problems;
   Params p;
 };
 
-template <int KIND, int CTAS, int TN, int AR> static int launch_form(Job& j, int dtype, bool chained, cudaStream_t st) {
-  using C = Cfg<KIND, CTAS, TN, AR>;
+template <int KIND, int CTAS, int TN, bool FLEX = false> static int launch_form(Job& j, int dtype, bool chained, cudaStream_t st, int flex_cols = 0) {
+  using C = Cfg<KIND, CTAS, TN, FLEX>;
   Params& p = j.p;
   p.status = status_words();
   if (!p.status) return fail(KSB_ERR_CUDA, "status words unavailable");
   const bool a_mn = KIND == DW, b_mn = KIND != PROJECT;
+  const int out_n = FLEX ? flex_cols : C::OUT_N;
   for (int i = 0; i < (KIND == PROJECT ? 1 : 2); ++i)
-    if (int rc = map_of(&p.a[i], j.a[i], BK, a_mn ? BK : AR)) return rc;
+    if (int rc = map_of(&p.a[i], j.a[i], BK, a_mn ? BK : BM)) return rc;
   for (int i = 0; i < (KIND == DW ? 1 : 2); ++i)
-    if (int rc = map_of(&p.b[i], j.b[i], BK, b_mn ? BK : (KIND == PROJECT && CTAS == 1 ? TN / 2 : C::B_ROWS))) return rc;
-  for (int i = 0; i < j.outs; ++i)
-    if (int rc = map_of(&p.out[i], j.out[i], C::PIECE_COLS, 32)) return rc;
+    if (int rc = map_of(&p.b[i], j.b[i], BK, b_mn ? BK : out_n)) return rc;
+  for (int i = 0; i < j.outs && !FLEX; ++i)
+    if (int rc = map_of(&p.out[i], j.out[i], C::PIECE_COLS, 32, KIND == PROJECT && i > 0 && i % 2 == 0 ? 1 : 2)) return rc;
   p.M = (int)j.M;
   p.N = (int)j.N;
   p.tiles_m = (int)((j.M + CTAS * BM - 1) / (CTAS * BM));
-  p.tiles_n = (int)((j.N + C::OUT_N - 1) / C::OUT_N);
+  p.tiles_n = (int)((j.N + out_n - 1) / out_n);
   const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n * j.problems;
   if (tiles > INT32_MAX) return fail(KSB_ERR_UNSUPPORTED, "too many tiles");
   p.problem_tiles = p.tiles_m * p.tiles_n;
   p.num_tiles = (int)tiles;
   p.steps = (int)((j.sum + BK - 1) / BK);
   p.num_k = p.steps * (KIND == DX ? 2 : 1);
+  p.flex_cols = out_n;
+  p.stages = std::min<int>(C::MOST, C::ROOM / (C::A_BYTES + 2 * out_n * ROW_BYTES));  // FLEX
   // Row tiles that share each column tile's operand while it is in L2; their own operand's rows are to take about 32 MB of it.
   const int64_t row_bytes = (int64_t)CTAS * BM * p.num_k * ROW_BYTES;
   p.group_m = (int)std::max<int64_t>(KIND == DW ? 8 : 4, std::min<int64_t>(64, (32ll << 20) / row_bytes));
-  return dtype == KSB_BF16 ? launch_as<__nv_bfloat16, KIND, CTAS, TN, AR>(p, chained, st) : launch_as<__half, KIND, CTAS, TN, AR>(p, chained, st);
+  return dtype == KSB_BF16 ? launch_as<__nv_bfloat16, KIND, CTAS, TN, FLEX>(p, chained, st) : launch_as<__half, KIND, CTAS, TN, FLEX>(p, chained, st);
 }
 
 static double waves(int64_t M, int64_t N, int tm, int tn, int workers, int problems) {
   return (double)((((M + tm - 1) / tm) * ((N + tn - 1) / tn) * problems + workers - 1) / workers);
 }
 
+// The form of a projection: by estimated time, waves x stages of a tile x time of a stage (us).
 static int project(Job& j, int dtype, cudaStream_t st) {
   const int sms = sm_count();
-  const double pair = sms < 2 ? 1e30 : waves(j.M, j.N, 256, 128, sms / 2, 1) * 2.0, single = waves(j.M, j.N, 128, 64, sms, 1) * 1.2;
-  if (j.M <= 128) return launch_form<PROJECT, 1, 256, 128>(j, dtype, false, st);
-  return single < pair ? launch_form<PROJECT, 1, 128, 128>(j, dtype, false, st) : launch_form<PROJECT, 2, 256, 128>(j, dtype, false, st);
+  const double pair = sms < 2 ? 1e30 : waves(j.M, j.N, 256, 128, sms / 2, 1) * 0.285, wide = waves(j.M, j.N, 128, 128, sms, 1) * 0.30;
+  double flex = 1e30;
+  int cols = 0;
+  if (!j.p.save && j.M <= BM)
+    for (int c = 8; c <= 128; c += 8) {
+      const double t = waves(j.M, j.N, 128, c, sms, 1) * std::max(0.25, 0.285 * c / 128);
+      if (t <= flex) flex = t, cols = c;
+    }
+  if (flex < wide && flex < pair) return launch_form<PROJECT, 1, 256, true>(j, dtype, false, st, cols);
+  return wide < pair ? launch_form<PROJECT, 1, 256>(j, dtype, false, st) : launch_form<PROJECT, 2, 256>(j, dtype, false, st);
 }
 template <int KIND> static int gradient(Job& j, int dtype, cudaStream_t st) {
   const int sms = sm_count();
-  const double pair = sms < 2 ? 1e30 : waves(j.M, j.N, 256, 256, sms / 2, j.problems) * 2.0, single = waves(j.M, j.N, 128, 128, sms, j.problems) * 1.2;
-  return single < pair ? launch_form<KIND, 1, 128, 128>(j, dtype, true, st) : launch_form<KIND, 2, 256, 128>(j, dtype, true, st);
+  const double pair = sms < 2 ? 1e30 : waves(j.M, j.N, 256, 256, sms / 2, j.problems) * 0.285, wide = waves(j.M, j.N, 128, 256, sms, j.problems) * 0.30;
+  const double narrow = waves(j.M, j.N, 128, 128, sms, j.problems) * 0.25;
+  if (narrow < wide && narrow < pair) return launch_form<KIND, 1, 128>(j, dtype, true, st);
+  return wide < pair ? launch_form<KIND, 1, 256>(j, dtype, true, st) : launch_form<KIND, 2, 256>(j, dtype, true, st);
 }
 
 static int64_t row_stretch(int64_t M, int64_t F) {
@@ -510,14 +594,14 @@ static int check_gated(int dtype, int64_t M, int64_t F, int64_t K, int act) {
 static bool rows_ok(const void* p, int64_t ld, int64_t cols, int64_t rows) { return p && aligned16(p) && (rows <= 1 || (ld >= cols && ld % 8 == 0)); }
 
 extern "C" int ksb_gated_linear(const void* x, int64_t ldx, const void* w_gate, int64_t ldg, const void* w_up, int64_t ldu, const void* b_gate, const void* b_up,
-                                int dtype, int64_t M, int64_t F, int64_t K, int act, void* h, void* g, void* u, ksb_stream_t stream) {
+                                int dtype, int64_t M, int64_t F, int64_t K, int act, void* h, void* saved, ksb_stream_t stream) {
   if (int rc = check_gated(dtype, M, F, K, act)) return rc;
   if (M == 0) return 0;
-  if (!rows_ok(x, ldx, K, M) || !rows_ok(w_gate, ldg, K, F) || !rows_ok(w_up, ldu, K, F) || !h || !aligned16(h) || !aligned16(b_gate) || !aligned16(b_up) || !aligned16(g) ||
-      !aligned16(u) || (!g) != (!u))
+  if (!rows_ok(x, ldx, K, M) || !rows_ok(w_gate, ldg, K, F) || !rows_ok(w_up, ldu, K, F) || !h || !aligned16(h) || !aligned16(b_gate) || !aligned16(b_up) ||
+      !aligned16(saved))
     return fail(KSB_ERR_INVALID, "null or unaligned pointer, or rows not a multiple of 8 elements apart");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (M <= gated::MAX_ROWS && !g) {
+  if (M <= gated::MAX_ROWS && !saved) {
     const gated::RowsCall call{x, w_gate, w_up, b_gate, b_up, h, ldx, ldg, ldu, (int)M, (int)F, (int)K, act};
     const int rc = gated::run_rows(call, dtype, st);
     if (rc != KSB_ERR_UNSUPPORTED) return rc ? rc : 1;  // else: no room for so many columns
@@ -527,14 +611,20 @@ extern "C" int ksb_gated_linear(const void* x, int64_t ldx, const void* w_gate, 
   j.b[0] = {w_gate, F, K, ldg};
   j.b[1] = {w_up, F, K, ldu};
   j.out[0] = {h, M, F, F};
-  j.out[1] = {g, M, F, F};
-  j.out[2] = {u, M, F, F};
-  j.outs = g ? 3 : 1;
+  const gated::Saved lay = gated::saved_layout(M, F);
+  uint8_t* planes = static_cast<uint8_t*>(saved);
+  for (int i = 0; i < 2; ++i) {
+    j.out[1 + 2 * i] = {planes + i * lay.u, M, F, F};
+    j.out[2 + 2 * i] = {planes + i * lay.u + lay.low, M, F, lay.low_ld};
+  }
+  j.outs = saved ? 5 : 1;
   j.M = M; j.N = F; j.sum = K; j.problems = 1;
-  j.p.b_gate = b_gate; j.p.b_up = b_up; j.p.act = act; j.p.save = g != nullptr;
+  j.p.b_gate = b_gate; j.p.b_up = b_up; j.p.act = act; j.p.save = saved != nullptr; j.p.h = h;
   if (int rc = gated::project(j, dtype, st)) return rc;
   return 1;
 }
+
+extern "C" int64_t ksb_gated_linear_saved(int64_t M, int64_t F) { return M <= 0 || F <= 0 || F % 8 != 0 ? 0 : gated::saved_layout(M, F).bytes; }
 
 // [dg][du][sums of the bias gradients]
 static int64_t gated_bytes(int64_t M, int64_t F) { return (M * F * 2 + 255) / 256 * 256; }
@@ -557,7 +647,7 @@ extern "C" int ksb_gated_linear_backward(const ksb_gated_linear_grads* a, void* 
     return 0;
   }
   const bool weights = a->dw_gate || a->dw_up;
-  if (!rows_ok(a->dh, a->lddh, F, M) || !rows_ok(a->g, F, F, M) || !rows_ok(a->u, F, F, M) || !workspace || !aligned16(workspace) ||
+  if (!rows_ok(a->dh, a->lddh, F, M) || !a->saved || !aligned16(a->saved) || !workspace || !aligned16(workspace) ||
       (weights && !rows_ok(a->x, a->ldx, K, M)) || (a->dx && (!rows_ok(a->w_gate, a->ldg, K, F) || !rows_ok(a->w_up, a->ldu, K, F))))
     return fail(KSB_ERR_INVALID, "null or unaligned pointer, or rows not a multiple of 8 elements apart");
   for (const void* t : {a->dx, a->dw_gate, a->dw_up})
@@ -567,7 +657,9 @@ extern "C" int ksb_gated_linear_backward(const ksb_gated_linear_grads* a, void* 
   const bool biases = a->db_gate || a->db_up;
   const int before = launch_count();
   gated::ActParams e{};
-  e.dh = a->dh; e.lddh = M > 1 ? a->lddh : F; e.g = a->g; e.u = a->u; e.dg = dg; e.du = du;
+  e.dh = a->dh; e.lddh = M > 1 ? a->lddh : F; e.dg = dg; e.du = du;
+  const gated::Saved lay = gated::saved_layout(M, F);
+  e.saved = static_cast<const uint8_t*>(a->saved); e.low_ld = lay.low_ld; e.low = lay.low; e.u = lay.u;
   e.parts = biases ? reinterpret_cast<float*>(ws + 2 * gated_bytes(M, F)) : nullptr;
   e.M = M; e.F = (int)F; e.act = a->act;
   e.stretch = gated::row_stretch(M, F);

@@ -238,5 +238,5 @@ class NormGrads(ctypes.Structure):
 
 
 class GatedGrads(ctypes.Structure):
-    _fields_ = [(n, c_void_p) for n in ("x", "w_gate", "w_up", "g", "u", "dh", "dx", "dw_gate", "dw_up", "db_gate", "db_up")] + \
+    _fields_ = [(n, c_void_p) for n in ("x", "w_gate", "w_up", "saved", "dh", "dx", "dw_gate", "dw_up", "db_gate", "db_up")] + \
         [(n, c_int64) for n in ("M", "F", "K", "ldx", "ldg", "ldu", "lddh")] + [("dtype", c_int), ("act", c_int)]

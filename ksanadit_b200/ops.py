@@ -836,25 +836,26 @@ def _gated_launch(x, w_gate, w_up, b_gate, b_up, act, save):
     x2, wg, wu = _rows(x, K), _rows(w_gate, K), _rows(w_up, K)
     M = x2.shape[0]
     h = torch.empty(x.shape[:-1] + (F,), dtype=x.dtype, device=x.device)
-    g, u = (torch.empty(M, F, dtype=x.dtype, device=x.device) for _ in range(2)) if save else (None, None)
-    STATS.count(native.queued(_lib.load().ksb_gated_linear(
+    lib = _lib.load()
+    saved = native.workspace(lib.ksb_gated_linear_saved(M, F), x.device) if save else None
+    STATS.count(native.queued(lib.ksb_gated_linear(
         x2.data_ptr(), x2.stride(0), wg.data_ptr(), wg.stride(0), wu.data_ptr(), wu.stride(0), _p(b_gate), _p(b_up), _dt(x), M, F, K, act, h.data_ptr(),
-        _p(g), _p(u), _stream()), "ksb_gated_linear"))
-    return h, g, u
+        _p(saved), _stream()), "ksb_gated_linear"))
+    return h, saved
 
 
 class _GatedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, b_gate, b_up, act):
-        h, g, u = _gated_launch(x, w_gate, w_up, b_gate, b_up, act, True)
-        ctx.save_for_backward(x, w_gate, w_up, g, u)
+        h, saved = _gated_launch(x, w_gate, w_up, b_gate, b_up, act, True)
+        ctx.save_for_backward(x, w_gate, w_up, saved)
         ctx.act = act
         return h
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dh):
-        x, w_gate, w_up, g, u = ctx.saved_tensors
+        x, w_gate, w_up, saved = ctx.saved_tensors
         need = ctx.needs_input_grad
         F, K = w_gate.shape
         with torch.cuda.device(x.device):
@@ -863,7 +864,7 @@ class _GatedLinear(torch.autograd.Function):
             out = [torch.empty(shape, dtype=x.dtype, device=x.device) if n else None
                    for n, shape in zip(need, (x.shape, (F, K), (F, K), (F,), (F,)))]
             lib = _lib.load()
-            args = native.GatedGrads(x2.data_ptr(), wg.data_ptr(), wu.data_ptr(), g.data_ptr(), u.data_ptr(), dh2.data_ptr(), *(_p(t) for t in out), M, F, K,
+            args = native.GatedGrads(x2.data_ptr(), wg.data_ptr(), wu.data_ptr(), saved.data_ptr(), dh2.data_ptr(), *(_p(t) for t in out), M, F, K,
                                      x2.stride(0), wg.stride(0), wu.stride(0), dh2.stride(0), _dt(x), ctx.act)
             ws = native.workspace(lib.ksb_gated_linear_workspace(M, F), x.device)
             STATS.count(native.queued(lib.ksb_gated_linear_backward(ctypes.addressof(args), ws.data_ptr(), _stream()), "ksb_gated_linear_backward"))
@@ -874,8 +875,8 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, act="silu"):
     """The gated half of a feed-forward block in one kernel: h = act(x w_gate^T + b_gate) * (x w_up^T + b_up).
 
     x [..., K], w_gate and w_up [F, K], b_gate and b_up [F] or None, all of one half type -> h [..., F].  act: ``"silu"`` or ``"gelu_tanh"``.
-    K and F must be multiples of 8.  fp32 sums, one rounding of h.  Differentiable in all tensors: the two projections are kept in the half
-    type for the backward pass, whose products take their gradients in the half type too."""
+    K and F must be multiples of 8.  fp32 sums, one rounding of h.  Differentiable in all tensors: for the backward pass the two projections are
+    kept in 24 bits each; its products take their gradients in the half type."""
     if act not in ACTIVATIONS:
         raise _lib.KsanaB200Error(f"act must be one of {sorted(ACTIVATIONS)}, got {act!r}")
     _dt(x)

@@ -33,21 +33,21 @@ P = 0x1000  # never read
 def test_c_entries_refuse_before_any_launch():
     lib = _lib.load()
 
-    def forward(x=P, ldx=16, wg=P, ldg=16, wu=P, ldu=16, bg=None, bu=None, dtype=0, M=4, F=8, K=16, act=0, h=P, g=None, u=None):
-        return lib.ksb_gated_linear(x, ldx, wg, ldg, wu, ldu, bg, bu, dtype, M, F, K, act, h, g, u, None)
+    def forward(x=P, ldx=16, wg=P, ldg=16, wu=P, ldu=16, bg=None, bu=None, dtype=0, M=4, F=8, K=16, act=0, h=P, saved=None):
+        return lib.ksb_gated_linear(x, ldx, wg, ldg, wu, ldu, bg, bu, dtype, M, F, K, act, h, saved, None)
 
     assert forward(M=0) == 0
     for kw in (dict(x=None), dict(wg=None), dict(wu=None), dict(h=None), dict(x=P + 2), dict(wg=P + 8), dict(wu=P + 4), dict(bg=P + 2), dict(bu=P + 2), dict(h=P + 2), dict(ldx=8),
-               dict(ldx=20), dict(ldg=8), dict(ldu=18), dict(dtype=2), dict(M=-1), dict(F=12), dict(K=20), dict(F=0), dict(K=0), dict(act=2), dict(g=P), dict(u=P), dict(g=P, u=P + 2)):
+               dict(ldx=20), dict(ldg=8), dict(ldu=18), dict(dtype=2), dict(M=-1), dict(F=12), dict(K=20), dict(F=0), dict(K=0), dict(act=2), dict(saved=P + 2)):
         assert forward(**kw) == -1, kw
 
     def backward(ws=P, **kw):
-        a = native.GatedGrads(P, P, P, P, P, P, P, P, P, P, P, 4, 8, 16, 16, 16, 16, 8, 0, 0)
+        a = native.GatedGrads(P, P, P, P, P, P, P, P, P, P, 4, 8, 16, 16, 16, 16, 8, 0, 0)
         for k, v in kw.items():
             setattr(a, k, v)
         return lib.ksb_gated_linear_backward(ctypes.byref(a), ws, None)
 
-    for kw in (dict(x=None), dict(w_gate=None), dict(w_up=None), dict(g=None), dict(u=None), dict(dh=None), dict(ws=None), dict(dx=P + 2), dict(dw_gate=P + 2), dict(dw_up=P + 8),
+    for kw in (dict(x=None), dict(w_gate=None), dict(w_up=None), dict(saved=None), dict(saved=P + 2), dict(dh=None), dict(ws=None), dict(dx=P + 2), dict(dw_gate=P + 2), dict(dw_up=P + 8),
                dict(lddh=4), dict(ldx=12), dict(ldg=8), dict(ldu=17), dict(M=-1), dict(F=4), dict(K=4), dict(dtype=3), dict(act=-1)):
         assert backward(**kw) == -1, kw
     assert lib.ksb_gated_linear_backward(None, P, None) == -1
