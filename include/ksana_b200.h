@@ -427,8 +427,9 @@ int ksb_w4_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, c
  * unrounded r).  x, y, r, h: [M, C] half (row strides ldx, ldy; r and h contiguous); gate, scale, shift: half, mod_rows rows (mod_rows
  * divides M; row m uses row m / (M / mod_rows)) `*_stride` elements apart (0: one row for all), each may be NULL; post_w, pre_w: fp32 [C]
  * or NULL.  y NULL: r = x and is not written; h NULL: no norm behind the sum.  stats: fp32 [M, 4], written where given: what the
- * backward pass needs besides its inputs.  C % 8 == 0, at most KSB_NORM_MAX_C.  Returns the number of kernels queued. */
+ * backward pass needs besides its inputs.  C % 8 == 0, at most KSB_NORM_MAX_C; M at most KSB_NORM_MAX_M.  Returns the number of kernels queued. */
 #define KSB_NORM_MAX_C 8192
+#define KSB_NORM_MAX_M (1 << 30)
 typedef struct ksb_sandwich_norm_args {
   const void *x, *y, *gate, *scale, *shift;
   const float *post_w, *pre_w;

@@ -13,8 +13,10 @@
 // dr, dh in and dx, dy out, 12 C bytes.  r is formed anew from x and y in the backward pass, which costs no more bytes than reading it
 // would and is not rounded.  All arithmetic is fp32, each result is rounded once: h is the norm of the unrounded r.
 //
-// Columns are taken in chunks of 8 (one 128-bit access per tensor); a row is owned by a group of warps whose threads hold one chunk
-// or two, and the next row's loads are issued before the present row's sums are exchanged.
+// Columns are taken in chunks of 8 (one 128-bit access per tensor).  A row is owned by a group of warps whose threads hold one chunk or
+// two, always the same columns, so that what the modulation and the weights make of them stays in registers as long as the modulation
+// row does.  A thread copies what it will read itself (cp.async) some rows ahead into a ring in shared memory: HBM is kept busy
+// through the exchanges of a row's sums, of which there are two to four, one after the other.
 #include <algorithm>
 
 #include "../../include/ksana_b200.h"
@@ -24,19 +26,21 @@
 namespace ksb {
 namespace norms {
 
-constexpr int MAX_WARPS = 32, MAX_GROUPS = 12;
+template <int NC> constexpr int backward_depth = NC == 4 ? 2 : 4;       // rows of the backward pass's ring
+template <int NC> constexpr int backward_threads = NC == 4 ? 256 : 640;  // of a CTA, one per SM
 
 struct Params {
   const void* x;
   const void* y;  // null: r = x
-  int64_t ldx, ldy, M;
-  int C;
+  int64_t ldx, ldy;
+  int M, C;
   float eps, a;
   // modulation row of row m: rows m / rows_per_mod, `stride` elements apart; each may be null
   const void* gate;
   const void* scale;
   const void* shift;
-  int64_t gate_stride, scale_stride, shift_stride, rows_per_mod;
+  int64_t gate_stride, scale_stride, shift_stride;
+  int rows_per_mod;
   const float* post_w;  // or null
   const float* pre_w;
   float4* stats;  // per row: mean and 1 / std of y, of r; or null
@@ -56,387 +60,589 @@ struct Grads {
   float* dpost_w;  // [C] or null
   float* dpre_w;
   float* parts;    // workspace
-  int64_t chunk_rows;
+  int chunk_rows;
   int chunks;      // of the rows that share a modulation row
   int samples;     // modulation rows
 };
 
 __device__ __forceinline__ uint4 load8(const void* base, int64_t offset_bytes) { return *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(base) + offset_bytes); }
 
-template <typename T> __device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
+// Two fp32 numbers in one register pair; one instruction works on both (bound by issue slots, the backward pass took a third longer
+// without: 75600 x 5120 921 us against PLACE).
+typedef unsigned long long F2;
+__device__ __forceinline__ F2 pair(float x, float y) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ F2 both(float x) { return pair(x, x); }
+__device__ __forceinline__ float2 split(F2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ F2 add(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ F2 mul(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ float total(F2 v) {
+  const float2 f = split(v);
+  return f.x + f.y;
+}
+// a thread's chunk: eight columns
+struct V8 {
+  F2 v[4];
+  __device__ __forceinline__ F2& operator[](int i) { return v[i]; }
+  __device__ __forceinline__ const F2& operator[](int i) const { return v[i]; }
+};
+__device__ __forceinline__ V8 fill8(float x) { return {both(x), both(x), both(x), both(x)}; }
+
+template <typename T> __device__ __forceinline__ V8 unpack8(const uint4& v) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  V8 r;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 p = HalfOps<T>::unpack2(w[i]);
-    f[2 * i] = p.x;
-    f[2 * i + 1] = p.y;
+    r[i] = pair(p.x, p.y);
   }
+  return r;
 }
-template <typename T> __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
-  return make_uint4(HalfOps<T>::pack2(make_float2(f[0], f[1])), HalfOps<T>::pack2(make_float2(f[2], f[3])), HalfOps<T>::pack2(make_float2(f[4], f[5])),
-                    HalfOps<T>::pack2(make_float2(f[6], f[7])));
+template <typename T> __device__ __forceinline__ uint4 pack8(const V8& f) {
+  return make_uint4(HalfOps<T>::pack2(split(f[0])), HalfOps<T>::pack2(split(f[1])), HalfOps<T>::pack2(split(f[2])), HalfOps<T>::pack2(split(f[3])));
 }
-__device__ __forceinline__ void weight8(const float* w, int c, float (&f)[8]) {
-  if (!w) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = 1.f;
-    return;
-  }
+__device__ __forceinline__ V8 weight8(const float* w, int c) {
+  if (!w) return fill8(1.f);
   const float4 a = *reinterpret_cast<const float4*>(w + c * 8), b = *reinterpret_cast<const float4*>(w + c * 8 + 4);
-  f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-  f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+  return {pair(a.x, a.y), pair(a.z, a.w), pair(b.x, b.y), pair(b.z, b.w)};
 }
 // A = a gate wp of chunk c
-template <typename T> __device__ __forceinline__ void post_factor(const Params& p, int64_t mod, int c, float (&f)[8]) {
-  weight8(p.post_w, c, f);
+template <typename T> __device__ __forceinline__ V8 post_factor(const Params& p, int64_t mod, int c) {
+  V8 f = weight8(p.post_w, c);
+  const F2 a = both(p.a);
   if (p.gate) {
-    float g[8];
-    unpack8<T>(load8(p.gate, (mod * p.gate_stride + c * 8) * 2), g);
+    const V8 g = unpack8<T>(load8(p.gate, (mod * p.gate_stride + c * 8) * 2));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] *= p.a * g[i];
+    for (int i = 0; i < 4; ++i) f[i] = mul(f[i], mul(a, g[i]));
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] *= p.a;
+    for (int i = 0; i < 4; ++i) f[i] = mul(f[i], a);
   }
+  return f;
 }
 // B = (1 + scale) wn of chunk c
-template <typename T> __device__ __forceinline__ void pre_factor(const Params& p, int64_t mod, int c, float (&f)[8]) {
-  weight8(p.pre_w, c, f);
+template <typename T> __device__ __forceinline__ V8 pre_factor(const Params& p, int64_t mod, int c) {
+  V8 f = weight8(p.pre_w, c);
   if (p.scale) {
-    float s[8];
-    unpack8<T>(load8(p.scale, (mod * p.scale_stride + c * 8) * 2), s);
+    const V8 s = unpack8<T>(load8(p.scale, (mod * p.scale_stride + c * 8) * 2));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] *= 1.f + s[i];
+    for (int i = 0; i < 4; ++i) f[i] = mul(f[i], add(both(1.f), s[i]));
   }
+  return f;
 }
 
+__device__ __forceinline__ void copy8(uint32_t dst, const void* base, int64_t offset_bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(static_cast<const uint8_t*>(base) + offset_bytes) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
 // A group of warps that owns a row: sums over its threads.  Each of a row's sums has its own place, and rows take turns between two
-// sets of places, so that one barrier per sum is enough.
+// sets of places, so that one barrier per exchange is enough.  The places behind the last warp's hold zeros.
+constexpr int PLACES = 8;
+constexpr int RED_FLOATS = 2 * PLACES * 64;  // groups x warps, in fours, are at most 64
 struct Group {
-  float2* red;  // [2][4][warps]
+  float* red;  // [2][PLACES][warps, in fours]
   int id, warps, warp, lane, par;
-  __device__ __forceinline__ float2 sum(float2 v, int place) {
+  __device__ __forceinline__ Group(float* all, int group, int threads, int t)
+      : id(group), warps(threads / 32), warp(t >> 5), lane(t & 31), par(0) {
+    red = all + group * 2 * PLACES * four();
+    if (warps > 1)
+      for (int i = t; i < 2 * PLACES * four(); i += threads) red[i] = 0.f;
+    barrier();
+  }
+  __device__ __forceinline__ int four() const { return (warps + 3) / 4 * 4; }
+  __device__ __forceinline__ void barrier() const {
+    if (warps > 1) asm volatile("bar.sync %0, %1;" ::"r"(id + 1), "r"(warps * 32) : "memory");
+  }
+  __device__ __forceinline__ float collect(const float* at) const {
+    float v = 0.f;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
-      v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
-    }
-    if (warps == 1) return v;
-    float2* at = red + (par * 4 + place) * warps;
-    if (lane == 0) at[warp] = v;
-    asm volatile("bar.sync %0, %1;" ::"r"(id + 1), "r"(warps * 32) : "memory");
-    v = at[0];
-    for (int w = 1; w < warps; ++w) {
-      const float2 o = at[w];
-      v.x += o.x;
-      v.y += o.y;
-    }
+    for (int i = 0; i < 5; ++i)  // at most 20 warps
+      if (i * 4 < warps) {
+        const float4 f = reinterpret_cast<const float4*>(at)[i];
+        v += (f.x + f.y) + (f.z + f.w);
+      }
     return v;
   }
-  __device__ __forceinline__ float sum(float v, int place) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __device__ __forceinline__ float sum(float v, int place) const {
+    v = warp_sum(v);
     if (warps == 1) return v;
-    float2* at = red + (par * 4 + place) * warps;
-    if (lane == 0) at[warp].x = v;
-    asm volatile("bar.sync %0, %1;" ::"r"(id + 1), "r"(warps * 32) : "memory");
-    v = at[0].x;
-    for (int w = 1; w < warps; ++w) v += at[w].x;
-    return v;
+    float* at = red + (par * PLACES + place) * four();
+    if (lane == 0) at[warp] = v;
+    barrier();
+    return collect(at);
+  }
+  // N sums in one exchange.  Of eight, lanes first share out the sums and only then add up one each, the warps' sums as well: 9 and 2 shuffles
+  // instead of 40, and 5 loads instead of 40 (32760 x 2 x 5120: 936 us instead of 1090).  Of three that would only lengthen the way (903 -> 1133).
+  template <int N> __device__ __forceinline__ void sums(float (&v)[N]) const {
+    constexpr bool SHARED_OUT = N == 8;
+    if (SHARED_OUT) {
+      int off = 16;
+#pragma unroll
+      for (int n = 4; n > 0; n /= 2, off /= 2) {
+        const bool upper = lane & off;
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+          const float keep = upper ? v[i + n] : v[i], give = upper ? v[i] : v[i + n];
+          v[i] = keep + __shfl_xor_sync(0xffffffffu, give, off);
+        }
+      }
+#pragma unroll
+      for (int o = 2; o > 0; o /= 2) v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+    } else {
+#pragma unroll
+      for (int o = 16; o > 0; o /= 2)
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+    }
+    if (warps > 1) {
+      float* at = red + par * PLACES * four();
+      if (SHARED_OUT) {
+        if ((lane & 3) == 0) at[(lane >> 2) * four() + warp] = v[0];
+      } else if (lane == 0) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) at[i * four() + warp] = v[i];
+      }
+      barrier();
+      if (SHARED_OUT) {
+        v[0] = 0.f;
+#pragma unroll
+        for (int w = 0; w < 20; w += 4)
+          if (w < four()) v[0] += at[(lane >> 2) * four() + w + (lane & 3)];
+#pragma unroll
+        for (int o = 2; o > 0; o /= 2) v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = collect(at + i * four());
+      }
+    }
+    if (SHARED_OUT) {
+      const float mine = v[0];
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = __shfl_sync(0xffffffffu, mine, i * 4);
+    }
   }
 };
 
-// 1 / std of a row of which this thread holds NC chunks, and the row's mean
-template <int NC, bool LAYER>
-__device__ __forceinline__ float2 row_stats(Group& g, const float (&v)[NC][8], const bool (&live)[NC], float inv_c, float eps, int place) {
+// 1 / std of a row of which this thread holds NC chunks, and the row's mean; `chunk`(c) gives chunk c (zeros where there is none)
+template <int NC, bool LAYER, typename Chunk>
+__device__ __forceinline__ float2 row_stats(Group& g, const Chunk& chunk, const bool (&live)[NC], float inv_c, float eps, int place) {
   float mean = 0.f;
   if (LAYER) {
-    float s = 0.f;
+    F2 s = both(0.f);
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
+    for (int c = 0; c < NC; ++c) {
+      const V8 f = chunk(c);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s += v[c][i];
-    mean = g.sum(s, place) * inv_c;
+      for (int i = 0; i < 4; ++i) s = add(s, f[i]);
+    }
+    mean = g.sum(total(s), place) * inv_c;
   }
-  float s = 0.f;
+  F2 s = both(0.f);
+  const F2 minus = both(-mean);
 #pragma unroll
   for (int c = 0; c < NC; ++c)
     if (live[c]) {
+      const V8 f = chunk(c);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float d = LAYER ? v[c][i] - mean : v[c][i];
-        s = fmaf(d, d, s);
+      for (int i = 0; i < 4; ++i) {
+        const F2 d = LAYER ? add(f[i], minus) : f[i];
+        s = fma2(d, d, s);
       }
     }
-  return make_float2(mean, rsqrtf(g.sum(s, place + 1) * inv_c + eps));
+  return make_float2(mean, rsqrtf(g.sum(total(s), place + 1) * inv_c + eps));
 }
 
+constexpr int FORWARD_DEPTH = 4;
 template <typename T, int NC, bool LAYER, int THREADS, int CTAS>
 __global__ void __launch_bounds__(THREADS, CTAS) forward_kernel(const __grid_constant__ Params p) {
-  __shared__ float2 red[2 * 4 * MAX_WARPS];
-  const int t = threadIdx.x, nt = blockDim.x, chunks = p.C / 8;
-  Group g{red + threadIdx.y * (2 * 4 * (nt / 32)), (int)threadIdx.y, nt / 32, t >> 5, t & 31, 0};
+  extern __shared__ __align__(16) uint8_t ring_bytes[];  // [FORWARD_DEPTH][x, y][NC][threads] 16 bytes
+  __shared__ __align__(16) float red[RED_FLOATS];
+  constexpr int DEPTH = FORWARD_DEPTH;
+  const int t = threadIdx.x, nt = blockDim.x, chunks = p.C / 8, all = nt * blockDim.y;
+  Group g(red, threadIdx.y, nt, t);
   const float inv_c = 1.f / static_cast<float>(p.C);
   bool live[NC];
 #pragma unroll
   for (int c = 0; c < NC; ++c) live[c] = t + c * nt < chunks;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.y;
-  uint4 nx[NC], ny[NC];
-  auto fetch = [&](int64_t row) {
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      nx[c] = ny[c] = make_uint4(0, 0, 0, 0);
-      if (row < p.M && live[c]) {
-        nx[c] = load8(p.x, (row * p.ldx + (t + c * nt) * 8) * 2);
-        if (p.y) ny[c] = load8(p.y, (row * p.ldy + (t + c * nt) * 8) * 2);
-      }
-    }
-  };
-  int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
-  fetch(row);
-  for (; row < p.M; row += step, g.par ^= 1) {
-    float x[NC][8], y[NC][8];
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      unpack8<T>(nx[c], x[c]);
-      unpack8<T>(ny[c], y[c]);
-    }
-    fetch(row + step);
-    const int64_t mod = row / p.rows_per_mod;
-    float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (p.y) {
-      const float2 s = row_stats<NC, LAYER>(g, y, live, inv_c, p.eps, 0);
-      st.x = s.x;
-      st.y = s.y;
+  const int step = gridDim.x * blockDim.y;  // rows are below 2^31, and so is a row and DEPTH steps: see the launch
+  const uint32_t mine = smem_u32(ring_bytes) + (threadIdx.y * nt + t) * 16;
+  int ahead = blockIdx.x * blockDim.y + threadIdx.y;
+  auto fetch = [&](int slot) {
+    if (ahead < p.M) {
 #pragma unroll
       for (int c = 0; c < NC; ++c)
         if (live[c]) {
-          float f[8];
-          post_factor<T>(p, mod, t + c * nt, f);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[c][i] = fmaf(f[i], (LAYER ? y[c][i] - s.x : y[c][i]) * s.y, x[c][i]);
-          *reinterpret_cast<uint4*>(static_cast<T*>(p.r) + row * p.C + (t + c * nt) * 8) = pack8<T>(x[c]);
+          copy8(mine + ((slot * 2) * NC + c) * all * 16, p.x, (static_cast<int64_t>(ahead) * p.ldx + (t + c * nt) * 8) * 2);
+          if (p.y) copy8(mine + ((slot * 2 + 1) * NC + c) * all * 16, p.y, (static_cast<int64_t>(ahead) * p.ldy + (t + c * nt) * 8) * 2);
         }
     }
-    if (p.h) {
-      const float2 s = row_stats<NC, LAYER>(g, x, live, inv_c, p.eps, 2);
-      st.z = s.x;
-      st.w = s.y;
+    ahead += step;
+    copies_commit();
+  };
+  int row = ahead;
+#pragma unroll
+  for (int d = 0; d < DEPTH - 1; ++d) fetch(d);
+  V8 A[NC], B[NC];
+  uint4 S[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    S[c] = make_uint4(0, 0, 0, 0);
+    A[c] = B[c] = fill8(0.f);
+  }
+  int mod_end = 0, slot = 0;
+  for (; row < p.M; row += step, g.par ^= 1) {
+    if (row >= mod_end) {
+      const int mod = row / p.rows_per_mod;
+      mod_end = (mod + 1) * p.rows_per_mod;
 #pragma unroll
       for (int c = 0; c < NC; ++c)
         if (live[c]) {
-          float f[8], b[8];
-          pre_factor<T>(p, mod, t + c * nt, f);
+          if (p.y) A[c] = post_factor<T>(p, mod, t + c * nt);
+          if (p.h) {
+            B[c] = pre_factor<T>(p, mod, t + c * nt);
+            if (p.shift) S[c] = load8(p.shift, (mod * p.shift_stride + (t + c * nt) * 8) * 2);
+          }
+        }
+    }
+    copies_wait<DEPTH - 2>();
+    // as halves for as long as that will do: registers are what limits the rows in flight
+    uint4 vx[NC], vy[NC];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) b[i] = 0.f;
-          if (p.shift) unpack8<T>(load8(p.shift, (mod * p.shift_stride + (t + c * nt) * 8) * 2), b);
+    for (int c = 0; c < NC; ++c) {
+      vx[c] = vy[c] = make_uint4(0, 0, 0, 0);
+      if (live[c]) {
+        vx[c] = ld_shared_v4(mine + ((slot * 2) * NC + c) * all * 16);
+        if (p.y) vy[c] = ld_shared_v4(mine + ((slot * 2 + 1) * NC + c) * all * 16);
+      }
+    }
+    fetch(slot == 0 ? DEPTH - 1 : slot - 1);  // the slot that was read one row ago
+    if (++slot == DEPTH) slot = 0;
+    float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
+    V8 x[NC];
+    if (p.y) {
+      const float2 s = row_stats<NC, LAYER>(g, [&](int c) { return unpack8<T>(vy[c]); }, live, inv_c, p.eps, 0);
+      st.x = s.x;
+      st.y = s.y;
+      const F2 minus = both(-s.x), rstd = both(s.y);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) b[i] = fmaf((LAYER ? x[c][i] - s.x : x[c][i]) * s.y, f[i], b[i]);
-          *reinterpret_cast<uint4*>(static_cast<T*>(p.h) + row * p.C + (t + c * nt) * 8) = pack8<T>(b);
+      for (int c = 0; c < NC; ++c) {
+        const V8 y = unpack8<T>(vy[c]);
+        x[c] = unpack8<T>(vx[c]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[c][i] = fma2(A[c][i], mul(LAYER ? add(y[i], minus) : y[i], rstd), x[c][i]);
+        if (live[c]) *reinterpret_cast<uint4*>(static_cast<T*>(p.r) + static_cast<int64_t>(row) * p.C + (t + c * nt) * 8) = pack8<T>(x[c]);
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < NC; ++c) x[c] = unpack8<T>(vx[c]);
+    }
+    if (p.h) {
+      const float2 s = row_stats<NC, LAYER>(g, [&](int c) { return x[c]; }, live, inv_c, p.eps, 2);
+      st.z = s.x;
+      st.w = s.y;
+      const F2 minus = both(-s.x), rstd = both(s.y);
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+        if (live[c]) {
+          V8 o = unpack8<T>(S[c]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[i] = fma2(mul(LAYER ? add(x[c][i], minus) : x[c][i], rstd), B[c][i], o[i]);
+          *reinterpret_cast<uint4*>(static_cast<T*>(p.h) + static_cast<int64_t>(row) * p.C + (t + c * nt) * 8) = pack8<T>(o);
         }
     }
     if (p.stats && t == 0) p.stats[row] = st;
   }
 }
 
-// Sums over rows that a thread keeps for its chunk: of D yh, dh rh and dh.
+// Sums over rows that a thread keeps for a chunk: of D yh, dh rh and dh.
 struct Sums {
-  float p[8], q[8], s[8];
-  __device__ __forceinline__ void clear() {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) p[i] = q[i] = s[i] = 0.f;
-  }
+  V8 p, q, s;
 };
 
-// One chunk per thread.  WHOLE: a group takes all rows of a modulation row, and writes the modulation's gradients itself; else a CTA takes
-// a stretch of them and leaves its sums to finish_kernel.
-template <typename T, bool LAYER, bool WHOLE, int THREADS>
-__global__ void __launch_bounds__(THREADS, 1) backward_kernel(const __grid_constant__ Params p, const __grid_constant__ Grads q) {
-  extern __shared__ __align__(16) float shared_sums[];  // [3][C], [2][C] with WHOLE
-  __shared__ float2 red[2 * 4 * MAX_WARPS];
-  const int t = threadIdx.x, nt = blockDim.x;
-  Group g{red + threadIdx.y * (2 * 4 * (nt / 32)), (int)threadIdx.y, nt / 32, t >> 5, t & 31, 0};
+// NC chunks per thread.  WHOLE: a group takes all rows of some modulation rows, and writes the modulation's gradients itself; else a CTA takes
+// a stretch of the rows of one and leaves its sums to finish_kernel.
+//
+// With w = dr + rstd_r t and z = A yh, D = w - a1 rh - a0 is linear in its row's a1 = rstd_r mean(t rh) and a0 = rstd_r mean(t), and so are the sums
+// that dy takes: sum(e yh) = sum(w z) - a1 sum(rh z) - a0 sum(z), sum(e) = sum(w A) - a1 sum(rh A) - a0 sum(A).  So a row has one exchange, of
+// three sums for RMS norms (a0 = 0) and of eight for layer norms, instead of two, one after the other.
+//
+// Up to 5120 columns a thread has one chunk and up to twenty warps share a row: eight warps of three chunks, which leaves the exchanges less to do
+// but the schedulers two warps each, took 1040 us for 75600 x 5120, twelve of two 1058, twenty of one 903.
+template <typename T, int NC, bool LAYER, bool WHOLE>
+__global__ void __launch_bounds__(backward_threads<NC>, 1) backward_kernel(const __grid_constant__ Params p, const __grid_constant__ Grads q) {
+  extern __shared__ __align__(16) uint8_t ring_bytes[];  // [DEPTH][x, y, dr, dh][NC][threads] 16 bytes and the factors; in the end the groups' sums
+  __shared__ __align__(16) float red[RED_FLOATS];
+  constexpr int DEPTH = backward_depth<NC>;
+  const int t = threadIdx.x, nt = blockDim.x, all = nt * blockDim.y;
+  Group g(red, threadIdx.y, nt, t);
   const float inv_c = 1.f / static_cast<float>(p.C);
-  const bool live = t < p.C / 8;
-  Sums acc;
-  acc.clear();
-  float wp[8], wn[8];  // WHOLE: of the weights' gradients
+  bool live[NC];
+  Sums acc[NC];
+  V8 wp[NC], wn[NC];  // WHOLE: of the weights' gradients
 #pragma unroll
-  for (int i = 0; i < 8; ++i) wp[i] = wn[i] = 0.f;
-
-  uint4 nx, ny, ndr, ndh;
-  float4 nst;
-  auto fetch = [&](int64_t row, int64_t end) {
-    nx = ny = ndr = ndh = make_uint4(0, 0, 0, 0);
-    nst = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (row < end && live) {
-      nx = load8(p.x, (row * p.ldx + t * 8) * 2);
-      if (p.y) ny = load8(p.y, (row * p.ldy + t * 8) * 2);
-      if (q.dr) ndr = load8(q.dr, (row * q.lddr + t * 8) * 2);
-      if (q.dh) ndh = load8(q.dh, (row * q.lddh + t * 8) * 2);
-      nst = p.stats[row];
-    }
-  };
-  auto rows = [&](int64_t row, int64_t step, int64_t end, int64_t mod) {
-    float A[8], B[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) A[i] = B[i] = 0.f;
-    if (live) {
-      if (p.y) post_factor<T>(p, mod, t, A);
-      if (q.dh) pre_factor<T>(p, mod, t, B);
-    }
-    fetch(row, end);
-    for (; row < end; row += step, g.par ^= 1) {
-      float yh[8], r[8], d[8], dh[8];
-      unpack8<T>(nx, r);
-      unpack8<T>(ny, yh);
-      unpack8<T>(ndr, d);
-      unpack8<T>(ndh, dh);
-      const float4 st = nst;
-      fetch(row + step, end);
-      if (p.y) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          yh[i] = (LAYER ? yh[i] - st.x : yh[i]) * st.y;
-          r[i] = fmaf(A[i], yh[i], r[i]);
-        }
-      }
-      if (q.dh) {
-        float2 s = make_float2(0.f, 0.f);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          r[i] = (LAYER ? r[i] - st.z : r[i]) * st.w;
-          acc.q[i] = fmaf(dh[i], r[i], acc.q[i]);
-          acc.s[i] += dh[i];
-          dh[i] *= B[i];
-          s.x = fmaf(dh[i], r[i], s.x);
-          if (LAYER) s.y += dh[i];
-        }
-        if (LAYER) s = g.sum(s, 0);
-        else s.x = g.sum(s.x, 0);
-        s.x *= inv_c;
-        s.y *= inv_c;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) d[i] = fmaf(st.w, dh[i] - r[i] * s.x - (LAYER ? s.y : 0.f), d[i]);
-      }
-      if (q.dx && live) *reinterpret_cast<uint4*>(static_cast<T*>(q.dx) + row * p.C + t * 8) = pack8<T>(d);
-      if (p.y) {
-        float2 s = make_float2(0.f, 0.f);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          acc.p[i] = fmaf(d[i], yh[i], acc.p[i]);
-          d[i] *= A[i];
-          s.x = fmaf(d[i], yh[i], s.x);
-          if (LAYER) s.y += d[i];
-        }
-        if (q.dy) {
-          if (LAYER) s = g.sum(s, 1);
-          else s.x = g.sum(s.x, 1);
-          s.x *= inv_c;
-          s.y *= inv_c;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) d[i] = st.y * (d[i] - yh[i] * s.x - (LAYER ? s.y : 0.f));
-          if (live) *reinterpret_cast<uint4*>(static_cast<T*>(q.dy) + row * p.C + t * 8) = pack8<T>(d);
-        }
-      }
-    }
-  };
-  // the groups' sums of one kind, added up in the order of the groups
-  auto add_up = [&](float* to, const float (&v)[8]) {
-    if (!live) return;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) to[t * 8 + i] = threadIdx.y == 0 ? v[i] : to[t * 8 + i] + v[i];
-  };
-  auto write_sums = [&](float* to, const float (&v)[8]) {
-    *reinterpret_cast<float4*>(to + t * 8) = make_float4(v[0], v[1], v[2], v[3]);
-    *reinterpret_cast<float4*>(to + t * 8 + 4) = make_float4(v[4], v[5], v[6], v[7]);
-  };
-
-  if constexpr (WHOLE) {
-    for (int64_t b = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y; b < q.samples; b += static_cast<int64_t>(gridDim.x) * blockDim.y) {
-      acc.clear();
-      rows(b * p.rows_per_mod, 1, (b + 1) * p.rows_per_mod, b);
-      if (!live) continue;
-      float f[8], o[8];
-      auto out = [&](void* to) { *reinterpret_cast<uint4*>(static_cast<T*>(to) + b * p.C + t * 8) = pack8<T>(o); };
-      if (p.y) {
-        if (q.dpost_w) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] = 1.f;
-          if (p.gate) unpack8<T>(load8(p.gate, (b * p.gate_stride + t * 8) * 2), f);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) wp[i] = fmaf(p.a * f[i], acc.p[i], wp[i]);
-        }
-        if (q.dgate) {
-          weight8(p.post_w, t, f);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) o[i] = p.a * f[i] * acc.p[i];
-          out(q.dgate);
-        }
-      }
-      if (q.dh) {
-        if (q.dpre_w) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] = 0.f;
-          if (p.scale) unpack8<T>(load8(p.scale, (b * p.scale_stride + t * 8) * 2), f);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) wn[i] = fmaf(1.f + f[i], acc.q[i], wn[i]);
-        }
-        if (q.dscale) {
-          weight8(p.pre_w, t, f);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) o[i] = f[i] * acc.q[i];
-          out(q.dscale);
-        }
-        if (q.dshift) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) o[i] = acc.s[i];
-          out(q.dshift);
-        }
-      }
-    }
-    if (!q.dpost_w && !q.dpre_w) return;
-    float* to = q.parts + static_cast<int64_t>(blockIdx.x) * 2 * p.C;
-    if (blockDim.y == 1) {
-      if (live) {
-        write_sums(to, wp);
-        write_sums(to + p.C, wn);
-      }
-      return;
-    }
-    for (int k = 0; k < (int)blockDim.y; ++k) {
-      __syncthreads();
-      if (k == (int)threadIdx.y) {
-        add_up(shared_sums, wp);
-        add_up(shared_sums + p.C, wn);
-      }
-    }
-    __syncthreads();
-    for (int i = threadIdx.y * nt + t; i < 2 * p.C; i += nt * blockDim.y) to[i] = shared_sums[i];
-  } else {
-    const int64_t b = blockIdx.x / q.chunks, first = b * p.rows_per_mod, from = first + (blockIdx.x - b * q.chunks) * q.chunk_rows;
-    const int64_t last = first + p.rows_per_mod, end = from + q.chunk_rows < last ? from + q.chunk_rows : last;
-    rows(from + threadIdx.y, blockDim.y, end, b);
-    float* to = q.parts + static_cast<int64_t>(blockIdx.x) * 3 * p.C;
-    if (blockDim.y == 1) {
-      if (live) {
-        write_sums(to, acc.p);
-        write_sums(to + p.C, acc.q);
-        write_sums(to + 2 * p.C, acc.s);
-      }
-      return;
-    }
-    for (int k = 0; k < (int)blockDim.y; ++k) {
-      __syncthreads();
-      if (k == (int)threadIdx.y) {
-        add_up(shared_sums, acc.p);
-        add_up(shared_sums + p.C, acc.q);
-        add_up(shared_sums + 2 * p.C, acc.s);
-      }
-    }
-    __syncthreads();
-    for (int i = threadIdx.y * nt + t; i < 3 * p.C; i += nt * blockDim.y) to[i] = shared_sums[i];
+  for (int c = 0; c < NC; ++c) {
+    live[c] = t + c * nt < p.C / 8;
+    acc[c].p = acc[c].q = acc[c].s = wp[c] = wn[c] = fill8(0.f);
   }
+
+  // the group's rows: row, row + step, .. below end
+  int row, step, end;
+  if (WHOLE) {
+    const int64_t groups = static_cast<int64_t>(gridDim.x) * blockDim.y, id = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+    row = static_cast<int>(q.samples * id / groups) * p.rows_per_mod;
+    end = static_cast<int>(q.samples * (id + 1) / groups) * p.rows_per_mod;
+    step = 1;
+  } else {
+    const int b = blockIdx.x / q.chunks, of = b * p.rows_per_mod, from = of + (blockIdx.x - b * q.chunks) * q.chunk_rows;
+    end = min(from + q.chunk_rows, of + p.rows_per_mod);
+    row = from + threadIdx.y;
+    step = blockDim.y;
+  }
+  const uint32_t mine = smem_u32(ring_bytes) + (threadIdx.y * nt + t) * 16;
+  auto place = [&](int slot, int which, int c) { return mine + ((slot * 4 + which) * NC + c) * all * 16; };
+  int ahead = row;
+  auto fetch = [&](int slot) {
+    if (ahead < end) {
+      const int64_t at = ahead;
+      const uint8_t* px = static_cast<const uint8_t*>(p.x) + (at * p.ldx + t * 8) * 2;
+      const uint8_t* py = static_cast<const uint8_t*>(p.y) + (at * p.ldy + t * 8) * 2;
+      const uint8_t* pr = static_cast<const uint8_t*>(q.dr) + (at * q.lddr + t * 8) * 2;
+      const uint8_t* ph = static_cast<const uint8_t*>(q.dh) + (at * q.lddh + t * 8) * 2;
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+        if (live[c]) {
+          copy8(place(slot, 0, c), px, c * nt * 16);
+          if (p.y) copy8(place(slot, 1, c), py, c * nt * 16);
+          if (q.dr) copy8(place(slot, 2, c), pr, c * nt * 16);
+          if (q.dh) copy8(place(slot, 3, c), ph, c * nt * 16);
+        }
+    }
+    ahead += step;
+    copies_commit();
+  };
+#pragma unroll
+  for (int d = 0; d < DEPTH - 1; ++d) fetch(d);
+  float4 next_st = row < end ? p.stats[row] : make_float4(0.f, 0.f, 0.f, 0.f);
+  int mod = row / p.rows_per_mod, mod_end = 0;
+  // A and B wait in shared memory
+  auto factor_at = [&](int which, int c, int i) { return place(DEPTH, which * 2 + i, c); };
+  auto put_factor = [&](int which, int c, const V8& f) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      asm volatile("st.shared.v2.b64 [%0], {%1, %2};" ::"r"(factor_at(which, c, i)), "l"(f[2 * i]), "l"(f[2 * i + 1]) : "memory");
+  };
+  auto factor = [&](int which, int c) {
+    V8 f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(f[2 * i]), "=l"(f[2 * i + 1]) : "r"(factor_at(which, c, i)) : "memory");
+    return f;
+  };
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    put_factor(0, c, fill8(0.f));
+    put_factor(1, c, fill8(0.f));
+  }
+  // WHOLE: a modulation row's gradients, and its part of the weights'
+  auto flush = [&]() {
+    const F2 a = both(p.a);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      if (live[c]) {
+        const int ch = t + c * nt;
+        V8 f, o;
+        auto out = [&](void* to) { *reinterpret_cast<uint4*>(static_cast<T*>(to) + static_cast<int64_t>(mod) * p.C + ch * 8) = pack8<T>(o); };
+        if (p.y) {
+          if (q.dpost_w) {
+            f = p.gate ? unpack8<T>(load8(p.gate, (mod * p.gate_stride + ch * 8) * 2)) : fill8(1.f);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) wp[c][i] = fma2(mul(a, f[i]), acc[c].p[i], wp[c][i]);
+          }
+          if (q.dgate) {
+            f = weight8(p.post_w, ch);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = mul(mul(a, f[i]), acc[c].p[i]);
+            out(q.dgate);
+          }
+        }
+        if (q.dh) {
+          if (q.dpre_w) {
+            f = p.scale ? unpack8<T>(load8(p.scale, (mod * p.scale_stride + ch * 8) * 2)) : fill8(0.f);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) wn[c][i] = fma2(add(both(1.f), f[i]), acc[c].q[i], wn[c][i]);
+          }
+          if (q.dscale) {
+            f = weight8(p.pre_w, ch);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = mul(f[i], acc[c].q[i]);
+            out(q.dscale);
+          }
+          if (q.dshift) {
+            o = acc[c].s;
+            out(q.dshift);
+          }
+        }
+      }
+      acc[c].p = acc[c].q = acc[c].s = fill8(0.f);
+    }
+  };
+  int slot = 0;
+  for (; row < end; row += step, g.par ^= 1) {
+    if (row >= mod_end) {
+      if (WHOLE && mod_end != 0) {
+        flush();
+        ++mod;
+      }
+      mod_end = (mod + 1) * p.rows_per_mod;
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+        if (live[c]) {
+          if (p.y) put_factor(0, c, post_factor<T>(p, mod, t + c * nt));
+          if (q.dh) put_factor(1, c, pre_factor<T>(p, mod, t + c * nt));
+        }
+    }
+    const float4 st = next_st;
+    if (row + step < end) next_st = p.stats[row + step];
+    copies_wait<DEPTH - 2>();
+    const uint4 none = make_uint4(0, 0, 0, 0);
+    const F2 y_minus = both(-st.x), y_rstd = both(st.y), r_minus = both(-st.z), r_rstd = both(st.w);
+    V8 yh[NC], w[NC], rh[NC];
+    constexpr int N = LAYER ? 8 : 3;
+    float m[N];  // the sums of t rh, w z, rh z, (t, z, w A, rh A, A)
+    F2 tr = both(0.f), wz = tr, rz = tr, ts = tr, zs = tr, wa = tr, ra = tr, as = tr;
+    const uint32_t src = mine + slot * 4 * NC * all * 16;
+    auto from = [&](int which, int c, bool there) { return unpack8<T>(live[c] && there ? ld_shared_v4(src + (which * NC + c) * all * 16) : none); };
+    // the factors are read where they are used: held, they would push others out of the registers (903 -> 1110 us)
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      yh[c] = from(1, c, p.y != nullptr);
+      w[c] = from(2, c, q.dr != nullptr);
+      rh[c] = fill8(0.f);
+      if (p.y) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) yh[c][i] = mul(LAYER ? add(yh[c][i], y_minus) : yh[c][i], y_rstd);
+      }
+      if (q.dh) {
+        rh[c] = from(0, c, true);
+        const V8 dh = from(3, c, true);
+        V8 f = factor(0, c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          rh[c][i] = fma2(f[i], yh[c][i], rh[c][i]);
+          rh[c][i] = mul(LAYER ? add(rh[c][i], r_minus) : rh[c][i], r_rstd);
+          acc[c].q[i] = fma2(dh[i], rh[c][i], acc[c].q[i]);
+          acc[c].s[i] = add(acc[c].s[i], dh[i]);
+        }
+        f = factor(1, c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const F2 tv = mul(dh[i], f[i]);
+          tr = fma2(tv, rh[c][i], tr);
+          if (LAYER) ts = add(ts, tv);
+          w[c][i] = fma2(r_rstd, tv, w[c][i]);
+        }
+      }
+    }
+    fetch(slot == 0 ? DEPTH - 1 : slot - 1);  // the slot that was read one row ago
+    if (++slot == DEPTH) slot = 0;
+    if (p.y) {
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const V8 f = factor(0, c);  // zeros where there is no column
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const F2 z = mul(f[i], yh[c][i]);
+          wz = fma2(w[c][i], z, wz);
+          rz = fma2(rh[c][i], z, rz);
+          if (LAYER) {
+            zs = add(zs, z);
+            wa = fma2(w[c][i], f[i], wa);
+            ra = fma2(rh[c][i], f[i], ra);
+            as = add(as, f[i]);
+          }
+        }
+      }
+    }
+    m[0] = total(tr);
+    m[1] = total(wz);
+    m[2] = total(rz);
+    if (LAYER) {
+      m[N - 5] = total(ts);
+      m[N - 4] = total(zs);
+      m[N - 3] = total(wa);
+      m[N - 2] = total(ra);
+      m[N - 1] = total(as);
+    }
+    g.sums<N>(m);
+    const float a1 = m[0] * inv_c * st.w, a0 = LAYER ? m[N - 5] * inv_c * st.w : 0.f;
+    const float e1 = m[1] - a1 * m[2] - (LAYER ? a0 * m[N - 4] : 0.f), e0 = LAYER ? m[N - 3] - a1 * m[N - 2] - a0 * m[N - 1] : 0.f;
+    const F2 xa1 = both(-a1), xa0 = both(-a0), xe1 = both(-e1 * inv_c), xe0 = both(-e0 * inv_c);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[c][i] = fma2(rh[c][i], xa1, LAYER ? add(w[c][i], xa0) : w[c][i]);  // D
+      const int64_t at = static_cast<int64_t>(row) * p.C + (t + c * nt) * 8;
+      if (q.dx && live[c]) *reinterpret_cast<uint4*>(static_cast<T*>(q.dx) + at) = pack8<T>(w[c]);
+      if (p.y) {
+        const V8 A = factor(0, c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          acc[c].p[i] = fma2(w[c][i], yh[c][i], acc[c].p[i]);
+          w[c][i] = fma2(yh[c][i], xe1, mul(w[c][i], A[i]));
+          w[c][i] = mul(y_rstd, LAYER ? add(w[c][i], xe0) : w[c][i]);
+        }
+        if (q.dy && live[c]) *reinterpret_cast<uint4*>(static_cast<T*>(q.dy) + at) = pack8<T>(w[c]);
+      }
+    }
+  }
+  if (WHOLE && mod_end != 0) flush();
+  copies_wait<0>();
+
+  // What is left to the second kernel: the groups' sums, added up in the order of the groups where there are several.
+  constexpr int KINDS = WHOLE ? 2 : 3;
+  if (WHOLE && !q.dpost_w && !q.dpre_w) return;
+  float* to = q.parts + static_cast<int64_t>(blockIdx.x) * KINDS * p.C;
+  float* sums = blockDim.y == 1 ? to : reinterpret_cast<float*>(ring_bytes);
+  for (int y = 0; y < (int)blockDim.y; ++y) {
+    if (blockDim.y > 1) __syncthreads();
+    if (y != (int)threadIdx.y) continue;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+      if (live[c]) {
+#pragma unroll
+        for (int k = 0; k < KINDS; ++k) {
+          const V8& v = WHOLE ? (k == 0 ? wp[c] : wn[c]) : (k == 0 ? acc[c].p : k == 1 ? acc[c].q : acc[c].s);
+          F2* at = reinterpret_cast<F2*>(sums + k * p.C + (t + c * nt) * 8);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) at[i] = y == 0 ? v[i] : add(at[i], v[i]);
+        }
+      }
+  }
+  if (blockDim.y == 1) return;
+  __syncthreads();
+  for (int i = threadIdx.y * nt + t; i < KINDS * p.C; i += all) to[i] = sums[i];
 }
 
 // Adds up the stretches' sums, in order: 32 columns per CTA, 16 threads per column, which take turns over the stretches of a
@@ -531,21 +737,19 @@ __global__ void __launch_bounds__(32 * FINISH) finish_weights_kernel(const __gri
   if (q.dpre_w) q.dpre_w[col] = b;
 }
 
-// How the backward pass shares out the rows.
+// How the backward pass shares out the rows: a CTA per SM, of as many groups as its threads hold.
 struct Plan {
-  int threads, groups, ctas, chunks;
+  int each, threads, groups, ctas, chunks;  // each: chunks per thread
   int64_t chunk_rows;
   bool whole;
   int64_t floats(int C) const { return static_cast<int64_t>(ctas) * (whole ? 2 : 3) * C; }
 };
 static Plan plan_backward(int64_t M, int64_t C, int64_t rows_per_mod) {
   Plan s{};
-  const int chunks = static_cast<int>(C / 8);
-  s.threads = (chunks + 31) / 32 * 32;
-  s.groups = std::min(MAX_GROUPS, std::max(1, 512 / s.threads));
-  const int64_t samples = M / rows_per_mod;
-  const int per_sm = s.threads * s.groups <= 512 ? 2 : 1;
-  const int64_t room = static_cast<int64_t>(sm_count()) * per_sm;
+  s.each = C <= 5120 ? 1 : 4;
+  s.threads = static_cast<int>((C / 8 + 32 * s.each - 1) / (32 * s.each) * 32);
+  s.groups = s.each == 4 ? 1 : std::min(15, backward_threads<1> / s.threads);  // a named barrier each
+  const int64_t samples = M / rows_per_mod, room = sm_count();
   s.whole = samples >= room;
   if (s.whole) {
     s.ctas = static_cast<int>(std::min<int64_t>(room, (samples + s.groups - 1) / s.groups));
@@ -561,31 +765,33 @@ static Plan plan_backward(int64_t M, int64_t C, int64_t rows_per_mod) {
 }
 
 template <typename T, int NC, bool LAYER, int THREADS, int CTAS> static int forward_as(const Params& p, int threads, int groups, cudaStream_t st) {
-  const int64_t need = (p.M + groups - 1) / groups, room = static_cast<int64_t>(sm_count()) * CTAS;
-  return launch_kernel("sandwich norm", reinterpret_cast<const void*>(forward_kernel<T, NC, LAYER, THREADS, CTAS>), dim3((unsigned)std::min(need, room)),
-                       dim3(threads, groups), 0, st, 1, false, p);
+  auto kernel = forward_kernel<T, NC, LAYER, THREADS, CTAS>;
+  static DeviceOnce limit;
+  if (int rc = limit.raise_smem(reinterpret_cast<const void*>(kernel), FORWARD_DEPTH * 2 * NC * THREADS * 16)) return rc;
+  const int need = (p.M + groups - 1) / groups, room = sm_count() * CTAS;
+  return launch_kernel("sandwich norm", reinterpret_cast<const void*>(kernel), dim3((unsigned)std::min(need, room)), dim3(threads, groups),
+                       FORWARD_DEPTH * 2 * NC * threads * groups * 16, st, 1, false, p);
 }
 template <typename T, bool LAYER> static int forward(const Params& p, cudaStream_t st) {
   const int chunks = p.C / 8;
   if (chunks <= 64) {
     const int threads = (chunks + 31) / 32 * 32;
-    return forward_as<T, 1, LAYER, 256, 4>(p, threads, std::min(MAX_GROUPS, 256 / threads), st);
+    return forward_as<T, 1, LAYER, 256, 4>(p, threads, 256 / threads, st);
   }
   const int threads = (chunks + 63) / 64 * 32;
-  if (threads <= 384) return forward_as<T, 2, LAYER, 384, 2>(p, threads, std::min(MAX_GROUPS, 384 / threads), st);
-  return forward_as<T, 2, LAYER, 1024, 1>(p, threads, 1, st);
+  if (threads <= 320) return forward_as<T, 2, LAYER, 320, 2>(p, threads, 320 / threads, st);
+  return forward_as<T, 2, LAYER, 512, 1>(p, threads, 1, st);
 }
 
-template <typename T, bool LAYER, bool WHOLE, int THREADS> static int backward_as(const Params& p, const Grads& q, const Plan& s, cudaStream_t st) {
-  const size_t smem = s.groups > 1 ? (size_t)(WHOLE ? 2 : 3) * p.C * 4 : 0;
-  return launch_kernel("sandwich norm gradient", reinterpret_cast<const void*>(backward_kernel<T, LAYER, WHOLE, THREADS>), dim3((unsigned)s.ctas), dim3(s.threads, s.groups),
-                       smem, st, 1, false, p, q);
+template <typename T, int NC, bool LAYER, bool WHOLE> static int backward_as(const Params& p, const Grads& q, const Plan& s, cudaStream_t st) {
+  auto kernel = backward_kernel<T, NC, LAYER, WHOLE>;
+  constexpr int bytes = (backward_depth<NC> + 1) * 64 * NC;  // a thread: the ring, and the factors
+  static DeviceOnce limit;
+  if (int rc = limit.raise_smem(reinterpret_cast<const void*>(kernel), bytes * backward_threads<NC>)) return rc;
+  return launch_kernel("sandwich norm gradient", reinterpret_cast<const void*>(kernel), dim3((unsigned)s.ctas), dim3(s.threads, s.groups), bytes * s.threads * s.groups, st, 1, false, p, q);
 }
 template <typename T, bool LAYER, bool WHOLE> static int backward_of(const Params& p, const Grads& q, const Plan& s, cudaStream_t st) {
-  const int threads = s.threads * s.groups;
-  if (threads <= 512) return backward_as<T, LAYER, WHOLE, 512>(p, q, s, st);
-  if (threads <= 640) return backward_as<T, LAYER, WHOLE, 640>(p, q, s, st);
-  return backward_as<T, LAYER, WHOLE, 1024>(p, q, s, st);
+  return s.each == 1 ? backward_as<T, 1, LAYER, WHOLE>(p, q, s, st) : backward_as<T, 4, LAYER, WHOLE>(p, q, s, st);
 }
 template <typename T> static int backward(const Params& p, const Grads& q, const Plan& s, bool layer, cudaStream_t st) {
   int rc;
@@ -603,7 +809,7 @@ template <typename T> static int backward(const Params& p, const Grads& q, const
 
 static int check(const Params& p, int dtype, int64_t C, int64_t mod_rows) {
   if (dtype != KSB_BF16 && dtype != KSB_FP16) return fail(KSB_ERR_INVALID, "dtype must be KSB_BF16 or KSB_FP16");
-  if (p.M < 0 || C <= 0 || C % 8 != 0 || p.M > INT32_MAX) return fail(KSB_ERR_INVALID, "bad shape M=%lld C=%lld (C %% 8 == 0)", (long long)p.M, (long long)C);
+  if (C <= 0 || C % 8 != 0) return fail(KSB_ERR_INVALID, "bad shape M=%d C=%lld (C %% 8 == 0)", p.M, (long long)C);
   if (C > KSB_NORM_MAX_C) return fail(KSB_ERR_UNSUPPORTED, "C=%lld is above %d", (long long)C, KSB_NORM_MAX_C);
   if (mod_rows < 1 || (p.M > 0 && p.M % mod_rows != 0)) return fail(KSB_ERR_INVALID, "mod_rows must divide M");
   const bool strides = (p.M <= 1 || (p.ldx >= C && (!p.y || p.ldy >= C))) && p.ldx % 8 == 0 && p.ldy % 8 == 0 && p.gate_stride % 8 == 0 && p.scale_stride % 8 == 0 && p.shift_stride % 8 == 0;
@@ -620,12 +826,14 @@ using namespace ksb;
 
 static int norm_params(norms::Params& p, const ksb_sandwich_norm_args* a) {
   if (!a) return fail(KSB_ERR_INVALID, "null pointer");
-  p.x = a->x; p.y = a->y; p.ldx = a->ldx; p.ldy = a->y ? a->ldy : 0; p.M = a->M; p.C = (int)a->C; p.eps = a->eps; p.a = a->residual_scale;
+  p.x = a->x; p.y = a->y; p.ldx = a->ldx; p.ldy = a->y ? a->ldy : 0; p.C = (int)a->C; p.eps = a->eps; p.a = a->residual_scale;
   p.gate = a->gate; p.scale = a->scale; p.shift = a->shift;
   p.gate_stride = a->gate_stride; p.scale_stride = a->scale_stride; p.shift_stride = a->shift_stride;
   p.post_w = a->post_w; p.pre_w = a->pre_w; p.stats = reinterpret_cast<float4*>(a->stats);
+  if (a->M < 0 || a->M > KSB_NORM_MAX_M) return fail(KSB_ERR_INVALID, "bad shape M=%lld", (long long)a->M);
+  p.M = (int)a->M;
   if (int rc = norms::check(p, a->dtype, a->C, a->mod_rows)) return rc;
-  p.rows_per_mod = p.M > 0 ? p.M / a->mod_rows : 1;
+  p.rows_per_mod = p.M > 0 ? (int)(p.M / a->mod_rows) : 1;
   return 0;
 }
 
@@ -671,7 +879,7 @@ extern "C" int ksb_sandwich_norm_backward(const ksb_sandwich_norm_args* a, const
   if (!p.y && (q.dy || q.dgate || q.dpost_w)) return fail(KSB_ERR_INVALID, "dy, dgate and dpost_w belong to y");
   if (!q.dh && (q.dscale || q.dshift || q.dpre_w)) return fail(KSB_ERR_INVALID, "dscale, dshift and dpre_w belong to dh");
   const norms::Plan s = norms::plan_backward(p.M, p.C, p.rows_per_mod);
-  q.chunk_rows = s.chunk_rows;
+  q.chunk_rows = (int)s.chunk_rows;
   q.chunks = s.chunks;
   q.samples = (int)a->mod_rows;
   const int before = launch_count();
