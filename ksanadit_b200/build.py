@@ -1,5 +1,5 @@
 """Builds the CUDA kernels and their C ABI into ``ksanadit_b200/lib/libksana_b200.so`` (sm_100a only), and the C++ side of the
-single calls (``host_call.cpp``, a CPython extension against torch's headers) into ``ksanadit_b200/lib/ksana_b200_host.<torch>.so``.
+single calls (``host_*.cpp``, a CPython extension against torch's headers) into ``ksanadit_b200/lib/ksana_b200_host.<torch>.so``.
 The latter is an accelerator: where it cannot be built, that is said and the library is built all the same.
 
 Usage: ``python -m ksanadit_b200.build [--force]``.  nvcc cross-compiles without a GPU present.
@@ -17,6 +17,7 @@ CSRC = os.path.join(PKG, "csrc")
 LIBDIR = os.path.join(PKG, "lib")
 LIB = os.path.join(LIBDIR, "libksana_b200.so")
 SOURCES = ["capi.cu", "rowwise_quant.cu", "fp8_gemm.cu", "fp8_gemm_split.cu", "sage_prepass.cu", "sage_attn.cu", "sage_attn_dual.cu", "elementwise.cu", "fused.cu", "w4_linear.cu", "block_norms.cu", "gated_linear.cu", "gated_rows.cu"]
+HOST_SOURCES = ["host_call.cpp", "host_ops.cpp"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC", "--use_fast_math=false",
@@ -40,7 +41,7 @@ def _stale(target, deps):
     return any(os.path.getmtime(d) > t for d in deps if os.path.exists(d))
 
 
-def _host_command(src, target):
+def _host_command(srcs, target):
     import sysconfig
 
     import torch
@@ -49,19 +50,19 @@ def _host_command(src, target):
     include = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"), sysconfig.get_paths()["include"],
                os.path.join(cuda, "include")]
     return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-            *("-I" + d for d in include), src, "-o", target, "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+            *("-I" + d for d in include), *srcs, "-o", target, "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
 
 
 def build_host(force: bool = False, verbose: bool = False) -> bool:
     """Builds the extension for the torch that is installed.  False, and why on stderr, where that cannot be done."""
-    src = os.path.join(CSRC, "host_call.cpp")
+    srcs = [os.path.join(CSRC, s) for s in HOST_SOURCES]
     try:
         from .native import host_path
         target = host_path()
-        if not (force or _stale(target, [src] + _deps())):
+        if not (force or _stale(target, srcs + _deps())):
             return True
         part = f"{target[:-3]}.{os.getpid()}.so"
-        cmd = _host_command(src, part)
+        cmd = _host_command(srcs, part)
         r = subprocess.run(cmd, capture_output=True, text=True)
         if verbose or r.returncode != 0:
             sys.stderr.write(" ".join(cmd) + "\n" + r.stdout + r.stderr)

@@ -20,22 +20,12 @@
 #include <vector>
 
 #include "../../include/ksana_b200.h"
+#include "host_call.h"
 
 namespace {
 
-// A strong reference.
-struct Ref {
-  PyObject* p = nullptr;
-  Ref() = default;
-  explicit Ref(PyObject* o) : p(o) { Py_XINCREF(p); }
-  Ref(Ref&& o) noexcept : p(o.p) { o.p = nullptr; }
-  Ref(const Ref& o) : p(o.p) { Py_XINCREF(p); }
-  Ref& operator=(Ref o) noexcept {
-    std::swap(p, o.p);
-    return *this;
-  }
-  ~Ref() { Py_XDECREF(p); }
-};
+using ksana_host::plain_tensor;
+using ksana_host::Ref;
 
 // A name in a dict, and what it held when the descriptor was built: an object, and of a tensor its place, type and layout.
 struct Entry {
@@ -45,15 +35,6 @@ struct Entry {
   at::ScalarType type = at::ScalarType::Undefined;
   std::vector<int64_t> sizes, strides;
 };
-
-// An exact tensor with memory of its own, not one that a transform wraps.
-bool plain_tensor(PyObject* o) {
-  if (!THPVariable_CheckExact(o)) return false;
-  const at::Tensor& t = THPVariable_Unpack(o);
-  const c10::DispatchKeySet wrapped({c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Functionalize,
-                                     c10::DispatchKey::Python, c10::DispatchKey::Batched});
-  return t.defined() && t.has_storage() && t.layout() == at::kStrided && !t.key_set().has_any(wrapped) && !t.is_conj() && !t.is_neg();
-}
 
 bool holds(const Entry& e) {
   PyObject* now = PyDict_GetItem(e.space.p, e.name.p);
@@ -233,7 +214,7 @@ PyObject* run(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
 
 PyMethodDef call_methods[] = {{"run", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(run)), METH_FASTCALL, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyTypeObject call_type = {PyVarObject_HEAD_INIT(nullptr, 0)};
-PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "ksana_b200_host", nullptr, -1, nullptr, nullptr, nullptr, nullptr, nullptr};
+PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "ksana_b200_host", nullptr, -1, ksana_host::op_methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
 

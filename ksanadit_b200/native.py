@@ -192,6 +192,23 @@ def host_module():
     return _host or None
 
 
+_host_ops = None  # False: tried, and there are none
+
+
+def host_ops():
+    """The extension, ready for the plain calls of the operators of a gated block half, or False."""
+    global _host_ops
+    if _host_ops is None:
+        _host_ops = host_module() or False
+        if _host_ops:
+            from . import ops
+            lib = _lib.load()
+            _host_ops.setup(vars(ops), _lib.KsanaB200Error, tuple(ctypes.cast(getattr(lib, n), c_void_p).value for n in (
+                "ksb_w4_linear", "ksb_gated_linear", "ksb_gated_linear_saved", "ksb_gated_linear_workspace", "ksb_gated_linear_backward", "ksb_sandwich_norm",
+                "ksb_sandwich_norm_workspace", "ksb_sandwich_norm_backward", "ksb_last_error")))
+    return _host_ops
+
+
 def linear_call(lin, call, dtype, device, quantize):
     """The C++ call of a Linear with descriptor ``call``; False where it has none, is not on a GPU, or was built from what a LinearCall
     cannot watch (a parameter of a tensor subclass, say): its calls go the general way."""

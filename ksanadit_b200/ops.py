@@ -656,6 +656,11 @@ def w4_linear(x, weight, weight_scale, weight_zero=None, bias=None, out_features
     out[m, n] = sum over groups of scale * sum (q - zero) x, plus bias; sums in fp32, one rounding.  N: ``out_features`` (default: 16
     per tile row, or the bias's length).  The group is K / weight_scale.shape[1]: 32, 64 or 128.  Up to 16 rows of x share one pass over
     the weight, more are taken 16 at a time: for many rows ``B200Fp8Linear`` is the faster class.  No gradients."""
+    host = native.host_ops()
+    if host:
+        out = host.w4_linear(x, weight, weight_scale, weight_zero, bias, out_features)
+        if out is not None:  # a plain call
+            return out
     dt, K = _dt(x), x.shape[-1]
     if weight.dim() != 3 or weight.dtype != torch.uint8 or weight.shape[2] != 512 or not weight.is_contiguous():
         raise _lib.KsanaB200Error("the packed weight must be a contiguous [ceil(N/16), ceil(K/64), 512] uint8 tensor")
@@ -792,6 +797,11 @@ def sandwich_norm(x, y=None, *, gate=None, scale=None, shift=None, post_weight=N
     [C], [1, C], or one row per leading index up to some axis ([B, 1, C], [B, C] or [B, L, C] for x [B, L, C]; any number that divides M
     for x [M, C]).  post_weight, pre_weight: fp32 [C].  All optional; without y, r is x itself; with ``pre=False``, h is None.  C % 8 == 0, at
     most 8192.  fp32 arithmetic, one rounding per result; h is the norm of the unrounded r.  Differentiable in all tensors."""
+    host = native.host_ops()
+    if host and kind in ("rms", "layer"):
+        rh = host.sandwich_norm(x, y, gate, scale, shift, post_weight, pre_weight, residual_scale, pre, kind == "layer", eps)
+        if rh is not None:  # a plain call
+            return rh if y is not None else (x, rh[1])
     tensors = (x, y, gate, scale, shift, post_weight, pre_weight)
     if kind not in ("rms", "layer"):
         raise _lib.KsanaB200Error(f"kind must be 'rms' or 'layer', got {kind!r}")
@@ -877,6 +887,11 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, act="silu"):
     x [..., K], w_gate and w_up [F, K], b_gate and b_up [F] or None, all of one half type -> h [..., F].  act: ``"silu"`` or ``"gelu_tanh"``.
     K and F must be multiples of 8.  fp32 sums, one rounding of h.  Differentiable in all tensors: for the backward pass the two projections are
     kept in 24 bits each; its products take their gradients in the half type."""
+    host = native.host_ops()
+    if host and act in ACTIVATIONS:
+        h = host.gated_linear(x, w_gate, w_up, b_gate, b_up, ACTIVATIONS[act])
+        if h is not None:  # a plain call
+            return h
     if act not in ACTIVATIONS:
         raise _lib.KsanaB200Error(f"act must be one of {sorted(ACTIVATIONS)}, got {act!r}")
     _dt(x)

@@ -7,6 +7,16 @@ from ksanadit_b200 import _lib, ops
 
 pytestmark = pytest.mark.gpu
 
+
+@pytest.fixture(params=["extension", "python"], autouse=True)
+def way(request, monkeypatch):
+    """Every test both ways: plain calls through the extension, and all calls through Python."""
+    from ksanadit_b200 import native
+    if request.param == "python":
+        monkeypatch.setattr(native, "host_ops", lambda: False)
+    else:
+        assert native.host_ops()
+
 NAMES = ("x", "y", "gate", "scale", "shift", "post_weight", "pre_weight")
 
 

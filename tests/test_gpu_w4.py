@@ -8,6 +8,16 @@ from ksanadit_b200 import _lib, ops, w4
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(params=["extension", "python"], autouse=True)
+def way(request, monkeypatch):
+    """Every test both ways: plain calls through the extension, and all calls through Python."""
+    from ksanadit_b200 import native
+    if request.param == "python":
+        monkeypatch.setattr(native, "host_ops", lambda: False)
+    else:
+        assert native.host_ops()
+
+
 def _case(M, N, K, group, zeros, dtype, seed=0):
     g = torch.Generator(device="cuda").manual_seed(seed)
     w = torch.randn(N, K, device="cuda", generator=g) * 0.02
