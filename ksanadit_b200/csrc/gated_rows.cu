@@ -18,7 +18,6 @@
 namespace ksb {
 namespace gated {
 
-constexpr int ROWS_KERNEL_ID = 7;
 constexpr int TILE_F = 8, STEP = 64;                 // rows of each weight in a row tile, columns of a step
 constexpr int WARPS = 16, ROWS_THREADS = WARPS * 32;
 constexpr int DEPTH = 4, SLOT_BYTES = 2048;          // of a warp's ring: [block of 32 columns][weight][lane] 16 bytes
@@ -31,7 +30,6 @@ struct RowsParams {
   int steps;                   // of a row tile
   int pitch;                   // bytes between rows of x in shared memory, 64 more than a multiple of 128: no two of a quarter warp's reads meet in a bank
   int x_at, sums_at;           // in shared memory, behind the rings
-  int* status;
 };
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
@@ -61,7 +59,6 @@ template <typename T, int NT> __global__ void __launch_bounds__(ROWS_THREADS, 1)
   // [0]: of the row tile that a warp comes into midway.  [1]: of the one it leaves midway, and on its way to memory any other's
   __shared__ __align__(16) float parts[2][WARPS][SUMS];
   __shared__ __align__(16) uint8_t nothing[256];  // x of the rows there are not
-  __shared__ __align__(8) uint64_t x_bar_word;
   const RowsCall& c = p.c;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
   const int split = p.split, rank = split > 1 ? (int)cluster_ctarank() : 0, cluster = blockIdx.x / split;
@@ -71,7 +68,7 @@ template <typename T, int NT> __global__ void __launch_bounds__(ROWS_THREADS, 1)
   const int begin = static_cast<int>(share * warp / WARPS), end = static_cast<int>(share * (warp + 1) / WARPS);
   uint8_t* xs = smem + p.x_at;
   float* sums = reinterpret_cast<float*>(smem + p.sums_at);  // split: [row tile][SUMS]
-  const uint32_t ring = smem_u32(smem) + warp * (DEPTH * SLOT_BYTES) + lane * 16, x_bar = smem_u32(&x_bar_word);
+  const uint32_t ring = smem_u32(smem) + warp * (DEPTH * SLOT_BYTES) + lane * 16;
   const int x0 = k0 * STEP, width = min(c.K - x0, steps * STEP);  // this CTA's columns of x
   int u = begin / steps, k = begin - u * steps;
   // the lane's place in both weights for the next step to ask for
@@ -98,24 +95,20 @@ template <typename T, int NT> __global__ void __launch_bounds__(ROWS_THREADS, 1)
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  if (threadIdx.x == 0) {
-    mbar_init(x_bar, 1);
-    fence_barrier_init();
-    mbar_arrive_expect_tx(x_bar, c.M * width * 2);
-    for (int m = 0; m < c.M; ++m)
-      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(xs) + m * p.pitch),
-                   "l"(static_cast<const T*>(c.x) + m * c.ldx + x0), "r"(width * 2), "r"(x_bar) : "memory");
+  {
+    const int units16 = steps * (STEP / 8), full = width / 8;  // 16-byte units of a row
+    const int each = WARPS / c.M, m = warp / each;  // warps per row (at most 16 rows); the last may have none
+    if (m < c.M) {
+      const T* row = static_cast<const T*>(c.x) + m * c.ldx + x0;
+      for (int i = (warp - m * each) * 32 + lane; i < units16; i += each * 32) copy16(smem_u32(xs) + m * p.pitch + i * 16, row + (i < full ? i * 8 : 0), i < full);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    if (threadIdx.x < 16) reinterpret_cast<uint4*>(nothing)[threadIdx.x] = make_uint4(0, 0, 0, 0);
   }
 #pragma unroll
   for (int d = 0; d < DEPTH - 1; ++d) fetch(d);
-  // zeros behind the last column of x (up to seven units of 16 bytes of its last step), and in place of its missing rows
-  if (threadIdx.x < 16) reinterpret_cast<uint4*>(nothing)[threadIdx.x] = make_uint4(0, 0, 0, 0);
-  if (width < steps * STEP && threadIdx.x < 8 * c.M) {
-    const int unit = width / 8 + (threadIdx.x & 7);
-    if (unit < steps * 8) *reinterpret_cast<uint4*>(xs + (threadIdx.x >> 3) * p.pitch + unit * 16) = make_uint4(0, 0, 0, 0);
-  }
+  asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory");  // x, asked for first
   __syncthreads();
-  const bool failed = !mbar_wait_warp(x_bar, 0, p.status, (ROWS_KERNEL_ID << 16) | 1);
 
   float acc[NT][4];
 #pragma unroll
@@ -159,7 +152,7 @@ template <typename T, int NT> __global__ void __launch_bounds__(ROWS_THREADS, 1)
   }
   bool entered = k != 0;  // the row tile was begun by an earlier warp
   int slot = 0;
-  for (int at = begin; at < end && !failed; ++at) {
+  for (int at = begin; at < end; ++at) {
     asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 2) : "memory");
     const uint32_t mine = ring + slot * SLOT_BYTES;
 #pragma unroll
@@ -187,24 +180,23 @@ template <typename T, int NT> __global__ void __launch_bounds__(ROWS_THREADS, 1)
     }
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
-  if (k != 0 && begin < end) put(entered ? 0 : 1);
+  if (begin == end || k != 0) put(begin == end || entered ? 0 : 1);  // without a share: zeros
   __syncthreads();
-  // The warp that has begun a row tile and left it to others adds up its pieces.
-  const int tail = end / steps, start = tail * steps;  // the row tile that the end falls into
-  if (end != start && begin < end && begin <= start) {
+  // Row tiles that several warps share, each known by the warp that has begun it and left it to others: 32 elements at a time, by all
+  // warps in turn.
+  const int batches = (live + 31) / 32;
 #pragma unroll 1
-    for (int j = lane; j < live; j += 32) {
-      float g = parts[1][warp][sum_at(j)], v = parts[1][warp][sum_at(j) + 8];
-      for (int w = warp + 1, from = end; w < WARPS && from < start + steps; ++w) {
-        const int to = static_cast<int>(share * (w + 1) / WARPS);
-        if (to > from) {
-          g += parts[0][w][sum_at(j)];
-          v += parts[0][w][sum_at(j) + 8];
-        }
-        from = to;
-      }
-      keep(tail, j, g, v);
+  for (int i = warp; i < WARPS * batches; i += WARPS) {
+    const int w0 = i / batches, j = (i - w0 * batches) * 32 + lane;
+    const int first = static_cast<int>(share * w0 / WARPS), left = static_cast<int>(share * (w0 + 1) / WARPS), tail = left / steps, start = tail * steps;
+    if (left == start || first == left || first > start || j >= live) continue;
+    float g = parts[1][w0][sum_at(j)], v = parts[1][w0][sum_at(j) + 8];
+#pragma unroll 4
+    for (int w = w0 + 1; w < WARPS && static_cast<int>(share * w / WARPS) < start + steps; ++w) {
+      g += parts[0][w][sum_at(j)];
+      v += parts[0][w][sum_at(j) + 8];
     }
+    keep(tail, j, g, v);
   }
   if (split > 1) {
     cluster_sync_all();  // every CTA's sums are there
@@ -223,7 +215,7 @@ template <typename T, int NT> __global__ void __launch_bounds__(ROWS_THREADS, 1)
   }
 }
 
-constexpr int rows_fixed_bytes(int nt) { return 2 * WARPS * 16 * 8 * nt * 4 + 256 + 8 + 128; }
+constexpr int rows_fixed_bytes(int nt) { return 2 * WARPS * 16 * 8 * nt * 4 + 256 + 128; }
 template <typename T, int NT> static int launch_rows(const RowsParams& p, int grid, size_t smem, cudaStream_t st) {
   auto kernel = rows_kernel<T, NT>;
   static DeviceOnce limit;
@@ -234,14 +226,12 @@ template <typename T, int NT> static int launch_rows(const RowsParams& p, int gr
 int run_rows(const RowsCall& call, int dtype, cudaStream_t st) {
   RowsParams p{};
   p.c = call;
-  p.status = status_words();
-  if (!p.status) return fail(KSB_ERR_CUDA, "status words unavailable");
   const int units = call.F / TILE_F, nt = call.M > 8 ? 2 : 1;
   p.steps = (call.K + STEP - 1) / STEP;
   p.x_at = WARPS * DEPTH * SLOT_BYTES;
   int clusters = 1;
   auto plan = [&](int split) -> int64_t {
-    clusters = std::min(units, std::max(1, sm_count() / split));
+    clusters = std::min(units, cluster_room(split));
     p.split = split;
     p.units_each = units / clusters;
     p.units_over = units % clusters;

@@ -47,31 +47,45 @@ struct Params {
   int* status;
 };
 
-// (w & 0x000f000f) | c as one instruction
-__device__ __forceinline__ uint32_t take(uint32_t w, uint32_t c) {
+// Eight weights of a word as four pairs, (q - z) times UNIT: an AND (or one lop3) and one fma each, and one shift for the word; shifting every
+// pair into place held up the integer pipe (1 x 30720 x 5120: 20.9 us against 19.4).
+__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t c) {
   uint32_t v;
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(v) : "r"(w), "r"(0x000f000fu), "r"(c));
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(v) : "r"(w), "r"(mask), "r"(c));
   return v;
 }
 template <typename T> struct Nibbles;
-// 128 + q is the bf16 number 0x4300 | q, 1024 + q the fp16 number 0x6400 | q; 128 + z and 1024 + z are exact as well.
+// The low eight bits of a bf16 count in steps of 2^-133, through the subnormal numbers and the first normal ones (bf16 arithmetic keeps
+// both): a nibble in bits 0 - 3 is q 2^-133, in bits 4 - 7 q 2^-129.  Brought to q / 64, since 2^127 is as far as a factor goes.
 template <> struct Nibbles<__nv_bfloat16> {
   typedef uint16_t IsHalf;
-  static __device__ __forceinline__ uint32_t offset(uint32_t z) { return (0x4300u | z) * 0x10001u; }
-  static __device__ __forceinline__ uint32_t pair(uint32_t w, int i, uint32_t off) {
-    const uint32_t v = take(w >> (4 * i), 0x43004300u);
-    const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&off));
-    return *reinterpret_cast<const uint32_t*>(&d);
+  static constexpr float UNIT = 1.f / 64;
+  uint32_t minus;  // -z / 64 twice
+  __device__ __forceinline__ explicit Nibbles(uint32_t z) {
+    const uint32_t n = (0x4300u | z) * 0x10001u;  // 128 + z
+    minus = fma(n, 0xbc80bc80u, 0x40004000u);     // (128 + z) (-1 / 64) + 2
   }
+  static __device__ __forceinline__ uint32_t fma(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t d;
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
+  }
+  __device__ __forceinline__ uint32_t low(uint32_t w) const { return fma(w & 0x000f000fu, 0x7f007f00u, minus); }
+  __device__ __forceinline__ uint32_t high(uint32_t w) const { return fma(w & 0x00f000f0u, 0x7d007d00u, minus); }
 };
+// 1024 + q and 1024 + 16 q are the fp16 numbers 0x6400 | q and 0x6400 | q << 4.
 template <> struct Nibbles<__half> {
   typedef uint8_t IsHalf;
-  static __device__ __forceinline__ uint32_t offset(uint32_t z) { return (0x6400u | z) * 0x10001u; }
-  static __device__ __forceinline__ uint32_t pair(uint32_t w, int i, uint32_t off) {
-    const uint32_t v = take(w >> (4 * i), 0x64006400u);
-    const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&off));
-    return *reinterpret_cast<const uint32_t*>(&d);
+  static constexpr float UNIT = 1.f;
+  uint32_t minus, minus16;  // -(1024 + z), -(64 + z)
+  __device__ __forceinline__ explicit Nibbles(uint32_t z) : minus((0xe400u | z) * 0x10001u), minus16((0xd400u | z << 4) * 0x10001u) {}
+  static __device__ __forceinline__ uint32_t fma(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t d;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
   }
+  __device__ __forceinline__ uint32_t low(uint32_t w) const { return fma(and_or(w, 0x000f000fu, 0x64006400u), 0x3c003c00u, minus); }
+  __device__ __forceinline__ uint32_t high(uint32_t w) const { return fma(and_or(w, 0x00f000f0u, 0x64006400u), 0x2c002c00u, minus16); }
 };
 
 // c = a * b + c; the first of a group's products starts from zeros
@@ -95,6 +109,11 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                : "memory");
 }
 
+// 16 bytes, or zeros
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
+  const int bytes = there ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ float load_cluster(uint32_t addr) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
@@ -111,9 +130,9 @@ __global__ void __launch_bounds__(THREADS, 1) w4_kernel(const __grid_constant__ 
   // [0]: of the row tile that a warp comes into midway.  [1]: of the one it leaves midway, and on its way to memory any other's
   __shared__ __align__(16) float parts[2][WARPS][SUMS];
   __shared__ __align__(16) uint8_t nothing[256];  // x of the rows there are not
-  __shared__ __align__(8) uint64_t bars[WARPS * MAX_SLOTS + 1];
+  __shared__ __align__(8) uint64_t bars[WARPS * MAX_SLOTS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
-  const int split = p.split, rank = split > 1 ? (int)cluster_ctarank() : 0, cluster = blockIdx.x / split;
+  const int split = p.split, rank = split > 1 ? (int)cluster_ctarank() : 0, cta = blockIdx.x, cluster = cta / split;
   const int k0 = p.steps * rank / split, steps = p.steps * (rank + 1) / split - k0;  // this CTA's steps of every row tile
   const int u0 = cluster * p.units_each + min(cluster, p.units_over), units = p.units_each + (cluster < p.units_over);
   const int64_t share = static_cast<int64_t>(units) * steps;
@@ -121,7 +140,7 @@ __global__ void __launch_bounds__(THREADS, 1) w4_kernel(const __grid_constant__ 
   uint8_t* ring = smem + warp * p.slots * p.slot_bytes;
   uint8_t* xs = smem + p.x_at;
   float* sums = reinterpret_cast<float*>(smem + p.sums_at);  // split: [row tile][SUMS]
-  const uint32_t ring_at = smem_u32(ring), bar0 = smem_u32(bars + warp * MAX_SLOTS), x_bar = smem_u32(bars + WARPS * MAX_SLOTS);
+  const uint32_t ring_at = smem_u32(ring), bar0 = smem_u32(bars + warp * MAX_SLOTS);
   int u = begin / steps, k = begin - u * steps;
   int ahead = begin, ahead_u = u, ahead_k = k;  // of the next slot to ask for
   const int x0 = k0 * GT * TILE_K, width = min(p.K - x0, steps * GT * TILE_K);  // this CTA's columns of x
@@ -142,23 +161,25 @@ __global__ void __launch_bounds__(THREADS, 1) w4_kernel(const __grid_constant__ 
       ++ahead_u;
     }
   };
+  // x, ahead of the weight, whose slots it would have to wait for; zeros behind its last column, and in place of its missing rows
+  {
+    const int units16 = steps * GT * 8, full = width / 8;  // 16-byte units of a row
+    const int each = WARPS / p.M, m = warp / each;  // warps per row (at most 16 rows); the last may have none
+    if (m < p.M) {
+      const T* row = static_cast<const T*>(p.x) + m * p.ldx + x0;
+      for (int i = (warp - m * each) * 32 + lane; i < units16; i += each * 32) copy16(smem_u32(xs) + m * p.pitch + i * 16, row + (i < full ? i * 8 : 0), i < full);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    if (threadIdx.x < 16) reinterpret_cast<uint4*>(nothing)[threadIdx.x] = make_uint4(0, 0, 0, 0);
+  }
   if (lane == 0) {
     for (int s = 0; s < p.slots; ++s) mbar_init(bar0 + 8 * s, 1);
-    if (warp == 0) mbar_init(x_bar, 1);
     fence_barrier_init();
-    if (warp == 0) {
-      // Ahead of the weight: behind its slots a row of x took a round trip of microseconds.
-      mbar_arrive_expect_tx(x_bar, p.M * width * 2);
-      for (int m = 0; m < p.M; ++m) bulk_load(smem_u32(xs) + m * p.pitch, static_cast<const T*>(p.x) + m * p.ldx + x0, width * 2, x_bar);
-    }
     for (int s = 0; s < p.slots && ahead < end; ++s) fetch(s);
   }
-  // zeros behind the last column of x, and in place of its missing rows
-  if (threadIdx.x < 16) reinterpret_cast<uint4*>(nothing)[threadIdx.x] = make_uint4(0, 0, 0, 0);
-  if (G == 32 && width < steps * TILE_K && threadIdx.x < 4 * p.M)
-    *reinterpret_cast<uint4*>(xs + (threadIdx.x >> 2) * p.pitch + width * 2 + (threadIdx.x & 3) * 16) = make_uint4(0, 0, 0, 0);
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();
-  bool failed = !mbar_wait_warp(x_bar, 0, p.status, (KERNEL_ID << 16) | 3);
+  bool failed = false;
 
   float acc[NT][4];
 #pragma unroll
@@ -171,7 +192,7 @@ __global__ void __launch_bounds__(THREADS, 1) w4_kernel(const __grid_constant__ 
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        parts[which][warp][(nt * 8 + 2 * t + (i & 1)) * TILE_N + r + (i >> 1) * 8] = acc[nt][i];
+        parts[which][warp][(nt * 8 + 2 * t + (i & 1)) * TILE_N + r + (i >> 1) * 8] = acc[nt][i] * (1.f / Nibbles<T>::UNIT);
         acc[nt][i] = 0.f;
       }
     __syncwarp();
@@ -210,7 +231,7 @@ __global__ void __launch_bounds__(THREADS, 1) w4_kernel(const __grid_constant__ 
     const uint8_t* zeros = ring + slot * p.slot_bytes + p.zero_at + r;
     // a row's last half tile may be behind K: it has no group of its own, and zeros in x
     const int lone = SCALES == 2 && (p.groups & 1) && k0 + k + n == p.steps ? n - 1 : -1;
-#pragma unroll(GT == 1 ? 2 : 1)
+#pragma unroll 2
     for (int j = 0; j < n; ++j) {
       float part[NT][4];
 #pragma unroll
@@ -224,19 +245,19 @@ __global__ void __launch_bounds__(THREADS, 1) w4_kernel(const __grid_constant__ 
           z0 = zeros[g] & 15u;
           z1 = zeros[g + 8] & 15u;
         }
-        z0 = Nibbles<T>::offset(z0);
-        z1 = Nibbles<T>::offset(z1);
+        const Nibbles<T> n0(z0), n1(z1);
         uint32_t a[2][4];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          a[c][0] = Nibbles<T>::pair(w0, 2 * c, z0);
-          a[c][1] = Nibbles<T>::pair(w1, 2 * c, z1);
-          a[c][2] = Nibbles<T>::pair(w0, 2 * c + 1, z0);
-          a[c][3] = Nibbles<T>::pair(w1, 2 * c + 1, z1);
+          const uint32_t v0 = w0 >> (8 * c), v1 = w1 >> (8 * c);
+          a[c][0] = n0.low(v0);
+          a[c][1] = n1.low(v1);
+          a[c][2] = n0.high(v0);
+          a[c][3] = n1.high(v1);
         }
         float s0 = 0.f, s1 = 0.f;
         if (done) {
-          s0 = HalfOps<T>::to_f(scales[g]);
+          s0 = HalfOps<T>::to_f(scales[g]);  // over UNIT: see put
           s1 = HalfOps<T>::to_f(scales[g + 8]);
         }
 #pragma unroll
@@ -279,21 +300,20 @@ __global__ void __launch_bounds__(THREADS, 1) w4_kernel(const __grid_constant__ 
   if (failed) {  // what is on its way lands before the block leaves
     for (int s = slot; s < slot + p.slots; ++s) mbar_wait(bar0 + 8 * (s % p.slots), phase ^ (s >= p.slots), p.status, (KERNEL_ID << 16) | 2);
   }
-  if (k != 0 && begin < end) put(entered ? 0 : 1);
+  if (begin == end || k != 0) put(begin == end || entered ? 0 : 1);  // without a share: zeros
   __syncthreads();
-  // The warp that has begun a row tile and left it to others adds up its pieces.
-  const int tail = end / steps, start = tail * steps;  // the row tile that the end falls into
-  if (end != start && begin < end && begin <= start) {
+  // Row tiles that several warps share, each known by the warp that has begun it and left it to others: 32 sums at a time, by all warps in
+  // turn (by one warp, a row tile of sixteen pieces and 16 rows took 5 us).
+  const int batches = (live + 31) / 32;
 #pragma unroll 1
-    for (int j = lane; j < live; j += 32) {
-      float v = parts[1][warp][j];
-      for (int w = warp + 1, from = end; w < WARPS && from < start + steps; ++w) {
-        const int to = static_cast<int>(share * (w + 1) / WARPS);
-        if (to > from) v += parts[0][w][j];
-        from = to;
-      }
-      keep(tail, j, v);
-    }
+  for (int i = warp; i < WARPS * batches; i += WARPS) {
+    const int w0 = i / batches, j = (i - w0 * batches) * 32 + lane;
+    const int first = static_cast<int>(share * w0 / WARPS), left = static_cast<int>(share * (w0 + 1) / WARPS), tail = left / steps, start = tail * steps;
+    if (left == start || first == left || first > start || j >= live) continue;
+    float v = parts[1][w0][j];
+#pragma unroll 4
+    for (int w = w0 + 1; w < WARPS && static_cast<int>(share * w / WARPS) < start + steps; ++w) v += parts[0][w][j];
+    keep(tail, j, v);
   }
   if (split > 1) {
     cluster_sync_all();  // every CTA's sums are there
@@ -362,7 +382,7 @@ extern "C" int ksb_w4_linear(const void* x, int dtype, int64_t M, int64_t K, int
   };
   // K is shared by a cluster where that fills the GPU, or makes room for the rows of x.
   auto plan = [&](int rows, int split) {
-    const int clusters = std::min(units, std::max(1, sm_count() / split)), sums = w4::TILE_N * (rows > 8 ? 16 : 8) * 4;
+    const int clusters = std::min(units, cluster_room(split)), sums = w4::TILE_N * (rows > 8 ? 16 : 8) * 4;
     p.split = split;
     p.units_each = units / clusters;
     p.units_over = units % clusters;
@@ -388,7 +408,7 @@ extern "C" int ksb_w4_linear(const void* x, int dtype, int64_t M, int64_t K, int
     p.M = rows;
     p.x = static_cast<const uint8_t*>(x) + m0 * ldx * 2;
     p.out = static_cast<uint8_t*>(out) + m0 * ldo * 2;
-    const int grid = std::min(units, std::max(1, sm_count() / split)) * split;
+    const int grid = std::min(units, cluster_room(split)) * split;
     if (int rc = dtype == KSB_BF16 ? w4::dispatch<__nv_bfloat16>(p, group, grid, smem, st) : w4::dispatch<__half>(p, group, grid, smem, st)) return rc;
     m0 += rows;
   }
