@@ -671,6 +671,7 @@ template <typename T> __global__ void __launch_bounds__(32 * FINISH) finish_kern
     const float* from = q.parts + (static_cast<int64_t>(b) * q.chunks + first) * 3 * p.C + col;
     s[0] = s[1] = s[2] = 0.f;
     if (!live) return;
+#pragma unroll 4
     for (int c = first; c < q.chunks; c += step, from += static_cast<int64_t>(step) * 3 * p.C) {
       s[0] += from[0];
       s[1] += from[p.C];
@@ -720,6 +721,7 @@ __global__ void __launch_bounds__(32 * FINISH) finish_weights_kernel(const __gri
   pdl_wait();
   float a = 0.f, b = 0.f;
   if (col < p.C)
+#pragma unroll 4
     for (int c = j; c < count; c += FINISH) {
       a += q.parts[static_cast<int64_t>(c) * 2 * p.C + col];
       b += q.parts[static_cast<int64_t>(c) * 2 * p.C + p.C + col];

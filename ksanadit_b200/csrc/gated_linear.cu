@@ -32,7 +32,9 @@ enum Kind : int { PROJECT = 0, DX = 1, DW = 2 };
 // CTAs): at most TN columns, how many is the launch's choice.
 template <int KIND, int CTAS, int TN, bool FLEX> struct Cfg {
   static constexpr int OUT_N = KIND == PROJECT ? TN / 2 : TN;  // columns of the output
-  static constexpr int PIECE_COLS = 64, PIECE_BYTES = 32 * PIECE_COLS * (KIND == PROJECT ? 3 : 2);  // PROJECT: a half's piece, and a byte's
+  // PROJECT: pieces of 32 columns, since a warp's way through a piece (two accumulators, the activation, with `save` three stores one after the
+  // other) is as long as a main loop of K = 1536; a half's piece, and a byte's
+  static constexpr int PIECE_COLS = KIND == PROJECT ? 32 : 64, PIECE_BYTES = 32 * PIECE_COLS * (KIND == PROJECT ? 3 : 2);
   static constexpr int EW = FLEX ? 4 : 4 * (OUT_N / PIECE_COLS);  // output warps
   static constexpr int LOADS = KIND == PROJECT ? (CTAS == 2 ? 2 : 3) : KIND == DX ? 1 + TN / CTAS / 64 : 2 + TN / CTAS / 64;  // TMA boxes per stage
   static constexpr int THREADS = 32 * (LOADS + 1 + EW);
@@ -263,6 +265,8 @@ __global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, FLEX>::THREADS, 1) gemm_ke
     pdl_release();
     const int q = warp & 3, ew = warp - C::LOADS - 1, col0 = (ew >> 2) * C::PIECE_COLS;  // lanes of tensor memory; the warp's columns of a tile
     const uint32_t piece = pieces + ew * C::PIECE_BYTES;
+    constexpr int UNITS = C::PIECE_COLS / 8;  // of 16 bytes in a row of a piece, swizzled as the tensor map has it
+    const int swizzle = UNITS == 8 ? lane & 7 : (lane >> 1) & 3;
     const uint32_t piece_row = piece + lane * (C::PIECE_COLS * 2);
     const uint32_t tempty_even = CTAS == 2 ? mapa_shared(tempty0, 0) : 0u;
     uint32_t count = 0;
@@ -283,7 +287,7 @@ __global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, FLEX>::THREADS, 1) gemm_ke
           for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(w[i]);
         };
         auto put = [&](int c, const float (&y)[8]) {
-          st_shared_v4(piece_row + (((c >> 3) ^ (lane & 7)) << 4), make_uint4(HalfOps<T>::pack2(make_float2(y[0], y[1])), HalfOps<T>::pack2(make_float2(y[2], y[3])),
+          st_shared_v4(piece_row + (((c >> 3) ^ swizzle) << 4), make_uint4(HalfOps<T>::pack2(make_float2(y[0], y[1])), HalfOps<T>::pack2(make_float2(y[2], y[3])),
                                                                           HalfOps<T>::pack2(make_float2(y[4], y[5])), HalfOps<T>::pack2(make_float2(y[6], y[7]))));
         };
         auto open = [&]() {  // the piece's last store has read it
@@ -337,7 +341,7 @@ __global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, FLEX>::THREADS, 1) gemm_ke
           } else {
           if (p.save) {
             // the upper 24 bits of each fp32 value, as two planes
-            const uint32_t low_row = piece + 32 * C::PIECE_COLS * 2 + lane * 64;
+            const uint32_t low_row = piece + 32 * C::PIECE_COLS * 2 + lane * C::PIECE_COLS;
 #pragma unroll 1
             for (int up = 0; up < 2; ++up) {
               open();
@@ -352,9 +356,9 @@ __global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, FLEX>::THREADS, 1) gemm_ke
                   with_bias(v + e, up ? p.b_up : p.b_gate, c + e, y);
 #pragma unroll
                   for (int i = 0; i < 8; ++i) r[e + i] = round24(y[i]);
-                  st_shared_v4(piece_row + ((((c + e) >> 3) ^ (lane & 7)) << 4), make_uint4(high2(r + e), high2(r + e + 2), high2(r + e + 4), high2(r + e + 6)));
+                  st_shared_v4(piece_row + ((((c + e) >> 3) ^ swizzle) << 4), make_uint4(high2(r + e), high2(r + e + 2), high2(r + e + 4), high2(r + e + 6)));
                 }
-                st_shared_v4(low_row + (((c >> 4) ^ ((lane >> 1) & 3)) << 4), make_uint4(low4(r), low4(r + 4), low4(r + 8), low4(r + 12)));
+                st_shared_v4(low_row + c, make_uint4(low4(r), low4(r + 4), low4(r + 8), low4(r + 12)));
               }
               close(&p.out[1 + 2 * up]);
               if (lane == 0) tma_store_2d(&p.out[2 + 2 * up], piece + 32 * C::PIECE_COLS * 2, n0, row0);
@@ -476,6 +480,7 @@ template <typename T> __global__ void __launch_bounds__(256) bias_grad_kernel(co
   pdl_release();
   float s = 0.f;
   if (col < 2 * F)
+#pragma unroll 8
     for (int i = j; i < stretches; i += 8) s += parts[static_cast<int64_t>(i) * 2 * F + col];
   sums[j][lane] = s;
   __syncthreads();
@@ -554,7 +559,7 @@ static double waves(int64_t M, int64_t N, int tm, int tn, int workers, int probl
 // The form of a projection: by estimated time, waves x stages of a tile x time of a stage (us).
 static int project(Job& j, int dtype, cudaStream_t st) {
   const int sms = sm_count();
-  const double pair = sms < 2 ? 1e30 : waves(j.M, j.N, 256, 128, sms / 2, 1) * 0.285, wide = waves(j.M, j.N, 128, 128, sms, 1) * 0.30;
+  const double pair = sms < 2 ? 1e30 : waves(j.M, j.N, 256, 128, sms / 2, 1) * 0.285, wide = waves(j.M, j.N, 128, 128, sms, 1) * 0.40;
   double flex = 1e30;
   int cols = 0;
   if (!j.p.save && j.M <= BM)
@@ -567,7 +572,7 @@ static int project(Job& j, int dtype, cudaStream_t st) {
 }
 template <int KIND> static int gradient(Job& j, int dtype, cudaStream_t st) {
   const int sms = sm_count();
-  const double pair = sms < 2 ? 1e30 : waves(j.M, j.N, 256, 256, sms / 2, j.problems) * 0.285, wide = waves(j.M, j.N, 128, 256, sms, j.problems) * 0.30;
+  const double pair = sms < 2 ? 1e30 : waves(j.M, j.N, 256, 256, sms / 2, j.problems) * 0.285, wide = waves(j.M, j.N, 128, 256, sms, j.problems) * 0.40;
   const double narrow = waves(j.M, j.N, 128, 128, sms, j.problems) * 0.25;
   if (narrow < wide && narrow < pair) return launch_form<KIND, 1, 128>(j, dtype, true, st);
   return wide < pair ? launch_form<KIND, 1, 256>(j, dtype, true, st) : launch_form<KIND, 2, 256>(j, dtype, true, st);

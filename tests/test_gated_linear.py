@@ -52,3 +52,38 @@ def test_c_entries_refuse_before_any_launch():
         assert backward(**kw) == -1, kw
     assert lib.ksb_gated_linear_backward(None, P, None) == -1
     assert lib.ksb_gated_linear_workspace(0, 8) == 0 and lib.ksb_gated_linear_workspace(4, 12) == 0 and lib.ksb_gated_linear_workspace(4, 8) > 0
+
+
+def test_registered_operators_have_shape_inference():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    import ksanadit_b200.torch_ops  # noqa: F401
+    t = torch.ops.ksana_b200
+    with FakeTensorMode():
+        x, w = torch.empty(2, 7, 64, dtype=torch.bfloat16, device="cuda"), torch.empty(48, 64, dtype=torch.bfloat16, device="cuda")
+        h = t.gated_linear(x, w, w)
+        assert h.shape == (2, 7, 48) and h.dtype == torch.bfloat16
+        r, h = t.sandwich_norm(x, x)
+        assert r.shape == h.shape == x.shape and r.dtype == h.dtype == x.dtype
+        o = t.w4_linear(x, torch.empty(3, 1, 512, dtype=torch.uint8, device="cuda"), torch.empty(3, 1, 16, dtype=torch.bfloat16, device="cuda"), None, None, 40)
+        assert o.shape == (2, 7, 40) and o.dtype == torch.bfloat16
+    with pytest.raises(Exception):
+        t.gated_linear(_t(2, 16), _t(8, 16), _t(8, 16))
+
+
+def test_module_refuses_what_it_does_not_have():
+    from ksanadit_b200.gated_block import B200GatedFeedForward, gated_stack
+    m = B200GatedFeedForward(128, 264, bias=True)
+    assert set(dict(m.named_parameters())) == {"w_gate", "w_up", "b_gate", "b_up", "down.weight", "down.bias", "pre_norm", "post_norm", "modulation.weight",
+                                               "modulation.weight_scale", "modulation.bias"}
+    assert [n for n, p in m.named_parameters() if not p.requires_grad] == ["modulation.weight", "modulation.weight_scale", "modulation.bias"]
+    x = _t(1, 2, 128)
+    assert gated_stack([], x) is x
+    with pytest.raises(_lib.KsanaB200Error):
+        gated_stack([m], x, vectors=[])
+    with pytest.raises(_lib.KsanaB200Error):
+        B200GatedFeedForward(128, 264, act="relu")
+    with pytest.raises(_lib.KsanaB200Error):
+        B200GatedFeedForward(100, 264)  # its modulation's groups
+    with pytest.raises(_lib.KsanaB200Error):
+        B200GatedFeedForward(128, 264, modulation=False)(x, x[:, 0])
