@@ -106,11 +106,17 @@ Tensor dense(const Tensor& d) {
   Tensor c = d.contiguous();
   return aligned(c) ? c : c.clone();
 }
+// Which of a function's tensor arguments (some of them absent) this backward pass asks gradients of.
+int64_t asked(AutogradContext* ctx, int64_t there) {
+  int64_t need = 0;
+  for (int64_t i = 0, edge = 0; there >> i; ++i)
+    if (there >> i & 1) need |= static_cast<int64_t>(ctx->needs_input_grad(edge++)) << i;
+  return need;
+}
 void not_twice(const variable_list& grads) {
   if (!at::GradMode::is_enabled()) return;
   for (const Tensor& g : grads) TORCH_CHECK(!g.defined() || !g.requires_grad(), "trying to differentiate twice a function that was marked with @once_differentiable");
 }
-// a saved tensor with rows on 16-byte boundaries, as it was when it came in
 PyObject* none() { Py_RETURN_NONE; }
 
 // ---------------------------------------------------------------------------------------------- 4-bit Linear
@@ -174,10 +180,7 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
     const Tensor h = gated_run(x, wg, wu, b0, b1, static_cast<int>(act), s, saved);
     ctx->save_for_backward({x, wg, wu, saved});
     ctx->saved_data["act"] = act;
-    const bool need[5] = {x.requires_grad(), wg.requires_grad(), wu.requires_grad(), b0.defined() && b0.requires_grad(), b1.defined() && b1.requires_grad()};
-    int64_t mask = 0;
-    for (int i = 0; i < 5; ++i) mask |= static_cast<int64_t>(need[i]) << i;
-    ctx->saved_data["need"] = mask;
+    ctx->saved_data["there"] = static_cast<int64_t>(7 | b0.defined() << 3 | b1.defined() << 4);
     return h;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -190,7 +193,7 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
     GatedShape s;
     const Tensor no;
     TORCH_CHECK(gated_shape(x, wg, wu, no, no, s), "gated_linear: the saved tensors are not those of the call");
-    const int64_t need = ctx->saved_data["need"].toInt();
+    const int64_t need = asked(ctx, ctx->saved_data["there"].toInt());
     const std::array<std::vector<int64_t>, 5> shapes{x.sizes().vec(), {s.F, s.K}, {s.F, s.K}, {s.F}, {s.F}};
     for (int i = 0; i < 5; ++i)
       if (need >> i & 1) out[i] = at::empty(shapes[i], x.options());
@@ -322,9 +325,9 @@ struct SandwichNorm : torch::autograd::Function<SandwichNorm> {
     variable_list save(t.begin(), t.end());
     save.push_back(stats);
     ctx->save_for_backward(save);
-    int64_t need = 0;
-    for (int i = 0; i < NORM_TENSORS; ++i) need |= static_cast<int64_t>(t[i].defined() && t[i].requires_grad()) << i;
-    ctx->saved_data["need"] = need;
+    int64_t there = 0;
+    for (int i = 0; i < NORM_TENSORS; ++i) there |= static_cast<int64_t>(t[i].defined()) << i;
+    ctx->saved_data["there"] = there;
     ctx->saved_data["residual_scale"] = residual_scale;
     ctx->saved_data["pre"] = pre;
     ctx->saved_data["layer"] = layer;
@@ -348,7 +351,7 @@ struct SandwichNorm : torch::autograd::Function<SandwichNorm> {
     TORCH_CHECK(norm_call(t, ctx->saved_data["residual_scale"].toDouble(), pre, ctx->saved_data["layer"].toBool(), ctx->saved_data["eps"].toDouble(), c),
                 "sandwich_norm: the saved tensors are not those of the call");
     c.a.stats = static_cast<float*>(saved[NORM_TENSORS].data_ptr());
-    const int64_t need = ctx->saved_data["need"].toInt();
+    const int64_t need = asked(ctx, ctx->saved_data["there"].toInt());
     const Tensor& x = t[X];
     for (int i = 0; i < NORM_TENSORS; ++i) {
       // without dh, what belongs to the norm behind the sum has no gradient

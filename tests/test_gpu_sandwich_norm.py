@@ -16,6 +16,7 @@ def way(request, monkeypatch):
         monkeypatch.setattr(native, "host_ops", lambda: False)
     else:
         assert native.host_ops()
+    return request.param
 
 NAMES = ("x", "y", "gate", "scale", "shift", "post_weight", "pre_weight")
 
@@ -173,6 +174,28 @@ def test_optional_parts(without, use_r, use_h):
             _compare(name, g, ref[name], size[name], 100 if name not in ("x", "y") else 0)
         else:
             assert g is None, name
+
+
+def test_each_gradient_alone(way):
+    t = _inputs((2, 40, 264), (2, 1), True, torch.bfloat16, 19)
+    leaves = {k: t[k].requires_grad_(True) for k in NAMES}
+
+    def call():
+        return ops.sandwich_norm(t["x"], t["y"], **{k: t[k] for k in NAMES[2:]})
+
+    whole = dict(zip(leaves, torch.autograd.grad(call(), list(leaves.values()), (t["dr"], t["dh"]))))
+    for n in NAMES:
+        out = call()
+        before = ops.STATS.kernels
+        (g,) = torch.autograd.grad(out, [t[n]], (t["dr"], t["dh"]))
+        assert torch.equal(g, whole[n]), n
+        # sums over rows only where they are asked for (from Python a function does not hear which are)
+        assert way == "python" or ops.STATS.kernels - before == (1 if n in ("x", "y") else 2), n
+    for n in NAMES:
+        for k in NAMES:
+            t[k].requires_grad_(k == n)
+        (g,) = torch.autograd.grad(call(), [t[n]], (t["dr"], t["dh"]))
+        assert torch.equal(g, whole[n]), n
 
 
 @pytest.mark.parametrize("kind", ["rms", "layer"])

@@ -16,6 +16,7 @@ def way(request, monkeypatch):
         monkeypatch.setattr(native, "host_ops", lambda: False)
     else:
         assert native.host_ops()
+    return request.param
 
 
 def _case(M, N, K, group, zeros, dtype, seed=0):
