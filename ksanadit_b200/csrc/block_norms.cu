@@ -302,6 +302,8 @@ __global__ void __launch_bounds__(THREADS, CTAS) forward_kernel(const __grid_con
     copies_commit();
   };
   int row = ahead;
+  pdl_wait();  // whatever ran ahead, the caller's kernels too
+  pdl_release();
 #pragma unroll
   for (int d = 0; d < DEPTH - 1; ++d) fetch(d);
   V8 A[NC], B[NC];
@@ -442,6 +444,8 @@ __global__ void __launch_bounds__(backward_threads<NC>, 1) backward_kernel(const
     ahead += step;
     copies_commit();
   };
+  pdl_wait();
+  pdl_release();
 #pragma unroll
   for (int d = 0; d < DEPTH - 1; ++d) fetch(d);
   float4 next_st = row < end ? p.stats[row] : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -653,6 +657,7 @@ template <typename T> __global__ void __launch_bounds__(32 * FINISH) finish_kern
   const int lane = threadIdx.x, j = threadIdx.y, col = blockIdx.x * 32 + lane;
   const bool live = col < p.C;
   pdl_wait();
+  pdl_release();
   const bool by_sample = q.samples >= FINISH;
   const float wp = p.post_w && live ? p.post_w[col] : 1.f, wn = p.pre_w && live ? p.pre_w[col] : 1.f;
   float dwp = 0.f, dwn = 0.f;
@@ -719,6 +724,7 @@ __global__ void __launch_bounds__(32 * FINISH) finish_weights_kernel(const __gri
   __shared__ float part[2][FINISH][33];
   const int lane = threadIdx.x, j = threadIdx.y, col = blockIdx.x * 32 + lane;
   pdl_wait();
+  pdl_release();
   float a = 0.f, b = 0.f;
   if (col < p.C)
 #pragma unroll 4
@@ -772,7 +778,7 @@ template <typename T, int NC, bool LAYER, int THREADS, int CTAS> static int forw
   if (int rc = limit.raise_smem(reinterpret_cast<const void*>(kernel), FORWARD_DEPTH * 2 * NC * THREADS * 16)) return rc;
   const int need = (p.M + groups - 1) / groups, room = sm_count() * CTAS;
   return launch_kernel("sandwich norm", reinterpret_cast<const void*>(kernel), dim3((unsigned)std::min(need, room)), dim3(threads, groups),
-                       FORWARD_DEPTH * 2 * NC * threads * groups * 16, st, 1, false, p);
+                       FORWARD_DEPTH * 2 * NC * threads * groups * 16, st, 1, true, p);
 }
 template <typename T, bool LAYER> static int forward(const Params& p, cudaStream_t st) {
   const int chunks = p.C / 8;
@@ -790,7 +796,7 @@ template <typename T, int NC, bool LAYER, bool WHOLE> static int backward_as(con
   constexpr int bytes = (backward_depth<NC> + 1) * 64 * NC;  // a thread: the ring, and the factors
   static DeviceOnce limit;
   if (int rc = limit.raise_smem(reinterpret_cast<const void*>(kernel), bytes * backward_threads<NC>)) return rc;
-  return launch_kernel("sandwich norm gradient", reinterpret_cast<const void*>(kernel), dim3((unsigned)s.ctas), dim3(s.threads, s.groups), bytes * s.threads * s.groups, st, 1, false, p, q);
+  return launch_kernel("sandwich norm gradient", reinterpret_cast<const void*>(kernel), dim3((unsigned)s.ctas), dim3(s.threads, s.groups), bytes * s.threads * s.groups, st, 1, true, p, q);
 }
 template <typename T, bool LAYER, bool WHOLE> static int backward_of(const Params& p, const Grads& q, const Plan& s, cudaStream_t st) {
   return s.each == 1 ? backward_as<T, 1, LAYER, WHOLE>(p, q, s, st) : backward_as<T, 4, LAYER, WHOLE>(p, q, s, st);

@@ -40,12 +40,14 @@ template <int KIND, int CTAS, int TN, bool FLEX> struct Cfg {
   static constexpr int THREADS = 32 * (LOADS + 1 + EW);
   static constexpr int A_BYTES = BM * ROW_BYTES, B_ROWS = TN / CTAS, B_BYTES = B_ROWS * ROW_BYTES, STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int OUT_BYTES = FLEX ? 0 : EW * PIECE_BYTES;
+  static constexpr int BIAS_COLS = FLEX ? TN / 2 : PIECE_COLS;                          // of an output warp
+  static constexpr int BIAS_BYTES = KIND == PROJECT ? EW * 2 * BIAS_COLS * 4 : 0;
   static constexpr int MOST = FLEX ? 10 : 6;  // stages
-  static constexpr int ROOM = 232448 - OUT_BYTES - (2 * MOST + 4) * 8 - 16;
+  static constexpr int ROOM = 232448 - OUT_BYTES - BIAS_BYTES - (2 * MOST + 4) * 8 - 16;
   static constexpr int STAGES = ROOM / STAGE_BYTES > MOST ? MOST : ROOM / STAGE_BYTES;
   static constexpr int TMEM_COLS = 2 * TN;
-  // [stages x (A | B)][output pieces][barriers]
-  static constexpr int SMEM_BYTES = FLEX ? 232448 : STAGES * STAGE_BYTES + OUT_BYTES + (2 * STAGES + 4) * 8 + 16;
+  // [stages x (A | B)][output pieces][biases][barriers]
+  static constexpr int SMEM_BYTES = FLEX ? 232448 : STAGES * STAGE_BYTES + OUT_BYTES + BIAS_BYTES + (2 * STAGES + 4) * 8 + 16;
   static_assert(SMEM_BYTES <= 232448 && STAGES >= 3, "shared memory");
 };
 
@@ -143,7 +145,7 @@ __global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, FLEX>::THREADS, 1) gemm_ke
   const uint32_t STAGES = FLEX ? p.stages : C::STAGES, B_BYTES = FLEX ? p.flex_cols * 2 * ROW_BYTES : C::B_BYTES, STAGE_BYTES = C::A_BYTES + B_BYTES;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t base = smem_u32(smem);
-  const uint32_t pieces = base + STAGES * STAGE_BYTES, bars = pieces + C::OUT_BYTES;
+  const uint32_t pieces = base + STAGES * STAGE_BYTES, biases = pieces + C::OUT_BYTES, bars = biases + C::BIAS_BYTES;
   const uint32_t full0 = bars, empty0 = full0 + 8 * STAGES, tfull0 = empty0 + 8 * STAGES, tempty0 = tfull0 + 16, tmem_slot = tempty0 + 16;
   volatile uint32_t* tmem_slot_gen = reinterpret_cast<volatile uint32_t*>(smem + (tmem_slot - base));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -274,9 +276,22 @@ __global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, FLEX>::THREADS, 1) gemm_ke
       int problem, tm, tn;
       tile_coords(p, tile, problem, tm, tn);
       const uint32_t acc = count & 1, aph = (count >> 1) & 1;
+      const int row0 = (tm * CTAS + (int)crank) * BM + q * 32, n0 = tn * OUT_N + col0;
+      // The biases of the warp's columns, as fp32, ahead of the accumulator: read behind it, column by column, they took 5 us of
+      // 77 x 4096 x 10240.
+      const uint32_t bias_at = biases + ew * (2 * C::BIAS_COLS * 4);
+      if (KIND == PROJECT) {
+#pragma unroll
+        for (int c = lane; c < 2 * C::BIAS_COLS; c += 32) {
+          const int which = c / C::BIAS_COLS, col = n0 + c % C::BIAS_COLS;
+          const void* bias = which ? p.b_up : p.b_gate;
+          const float f = bias && col < p.N ? HalfOps<T>::to_f(static_cast<const T*>(bias)[col]) : 0.f;
+          asm volatile("st.shared.f32 [%0], %1;" ::"r"(bias_at + c * 4), "f"(f) : "memory");
+        }
+        __syncwarp();
+      }
       if (!mbar_wait_warp(tfull0 + 8 * acc, aph, p.status, (KERNEL_ID << 16) | 4)) break;
       tc_fence_after();
-      const int row0 = (tm * CTAS + (int)crank) * BM + q * 32, n0 = tn * OUT_N + col0;
       if (row0 < p.M && n0 < p.N) {  // uniform over the warp
         const uint32_t t_row = tmem_base + acc * TN + (static_cast<uint32_t>(q * 32) << 16) + col0;
         auto take16 = [&](uint32_t at, float (&v)[16]) {
@@ -300,20 +315,11 @@ __global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, FLEX>::THREADS, 1) gemm_ke
           if (lane == 0) tma_store_2d(map, piece, n0, row0);
         };
         if (KIND == PROJECT) {
-          // eight columns with their bias; the same for all lanes
-          auto with_bias = [&](const float* v, const void* bias, int c, float (&y)[8]) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = v[i];
-            if (bias && n0 + c < p.N) {
-              const uint4 b = *reinterpret_cast<const uint4*>(static_cast<const T*>(bias) + n0 + c);
-              const uint32_t w[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float2 f = HalfOps<T>::unpack2(w[i]);
-                y[2 * i] += f.x;
-                y[2 * i + 1] += f.y;
-              }
-            }
+          // eight columns with their bias
+          auto with_bias = [&](const float* v, int up, int c, float (&y)[8]) {
+            const uint4 a = ld_shared_v4(bias_at + (up * C::BIAS_COLS + c) * 4), b = ld_shared_v4(bias_at + (up * C::BIAS_COLS + c) * 4 + 16);
+            y[0] = v[0] + __uint_as_float(a.x); y[1] = v[1] + __uint_as_float(a.y); y[2] = v[2] + __uint_as_float(a.z); y[3] = v[3] + __uint_as_float(a.w);
+            y[4] = v[4] + __uint_as_float(b.x); y[5] = v[5] + __uint_as_float(b.y); y[6] = v[6] + __uint_as_float(b.z); y[7] = v[7] + __uint_as_float(b.w);
           };
           if constexpr (FLEX) {
             // few rows: straight to memory
@@ -330,8 +336,8 @@ __global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, FLEX>::THREADS, 1) gemm_ke
                 fv[i] = __uint_as_float(v[i]);
                 fw[i] = __uint_as_float(w[i]);
               }
-              with_bias(fv, p.b_gate, c, g);
-              with_bias(fw, p.b_up, c, u);
+              with_bias(fv, 0, c, g);
+              with_bias(fw, 1, c, u);
 #pragma unroll
               for (int i = 0; i < 8; ++i) g[i] = g[i] * act_sigmoid(g[i], p.act) * u[i];
               *reinterpret_cast<uint4*>(static_cast<T*>(p.h) + static_cast<int64_t>(row) * p.N + n0 + c) =
@@ -353,7 +359,7 @@ __global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, FLEX>::THREADS, 1) gemm_ke
 #pragma unroll
                 for (int e = 0; e < 16; e += 8) {
                   float y[8];
-                  with_bias(v + e, up ? p.b_up : p.b_gate, c + e, y);
+                  with_bias(v + e, up, c + e, y);
 #pragma unroll
                   for (int i = 0; i < 8; ++i) r[e + i] = round24(y[i]);
                   st_shared_v4(piece_row + ((((c + e) >> 3) ^ swizzle) << 4), make_uint4(high2(r + e), high2(r + e + 2), high2(r + e + 4), high2(r + e + 6)));
@@ -373,8 +379,8 @@ __global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, FLEX>::THREADS, 1) gemm_ke
 #pragma unroll
             for (int e = 0; e < 16; e += 8) {
               float g[8], u[8];
-              with_bias(v + e, p.b_gate, c + e, g);
-              with_bias(w + e, p.b_up, c + e, u);
+              with_bias(v + e, 0, c + e, g);
+              with_bias(w + e, 1, c + e, u);
 #pragma unroll
               for (int i = 0; i < 8; ++i) g[i] = g[i] * act_sigmoid(g[i], p.act) * u[i];
               put(c + e, g);
@@ -432,6 +438,8 @@ struct ActParams {
 template <typename T> __global__ void __launch_bounds__(256) act_grad_kernel(const __grid_constant__ ActParams p) {
   const int c = blockIdx.x * 256 + threadIdx.x;
   if (c * 8 >= p.F) return;
+  pdl_wait();
+  pdl_release();
   const int64_t first = blockIdx.y * p.stretch, last = first + p.stretch < p.M ? first + p.stretch : p.M;
   float sg[8], su[8];
 #pragma unroll
@@ -567,8 +575,8 @@ static int project(Job& j, int dtype, cudaStream_t st) {
       const double t = waves(j.M, j.N, 128, c, sms, 1) * std::max(0.25, 0.285 * c / 128);
       if (t <= flex) flex = t, cols = c;
     }
-  if (flex < wide && flex < pair) return launch_form<PROJECT, 1, 256, true>(j, dtype, false, st, cols);
-  return wide < pair ? launch_form<PROJECT, 1, 256>(j, dtype, false, st) : launch_form<PROJECT, 2, 256>(j, dtype, false, st);
+  if (flex < wide && flex < pair) return launch_form<PROJECT, 1, 256, true>(j, dtype, true, st, cols);
+  return wide < pair ? launch_form<PROJECT, 1, 256>(j, dtype, true, st) : launch_form<PROJECT, 2, 256>(j, dtype, true, st);
 }
 template <int KIND> static int gradient(Job& j, int dtype, cudaStream_t st) {
   const int sms = sm_count();
@@ -672,7 +680,7 @@ extern "C" int ksb_gated_linear_backward(const ksb_gated_linear_grads* a, void* 
   const bool bf16 = a->dtype == KSB_BF16;
   const dim3 grid((unsigned)((F / 8 + 255) / 256), (unsigned)stretches);
   if (int rc = launch_kernel("gated linear", bf16 ? reinterpret_cast<const void*>(gated::act_grad_kernel<__nv_bfloat16>) : reinterpret_cast<const void*>(gated::act_grad_kernel<__half>),
-                             grid, dim3(256), 0, st, 1, false, e))
+                             grid, dim3(256), 0, st, 1, true, e))
     return rc;
   if (biases) {
     const float* parts = e.parts;

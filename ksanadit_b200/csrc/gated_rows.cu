@@ -95,6 +95,8 @@ template <typename T, int NT> __global__ void __launch_bounds__(ROWS_THREADS, 1)
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
+  pdl_wait();  // whatever ran ahead, the caller's kernels too
+  pdl_release();
   {
     const int units16 = steps * (STEP / 8), full = width / 8;  // 16-byte units of a row
     const int each = WARPS / c.M, m = warp / each;  // warps per row (at most 16 rows); the last may have none
@@ -220,7 +222,7 @@ template <typename T, int NT> static int launch_rows(const RowsParams& p, int gr
   auto kernel = rows_kernel<T, NT>;
   static DeviceOnce limit;
   if (int rc = limit.raise_smem(reinterpret_cast<const void*>(kernel), SMEM_LIMIT - rows_fixed_bytes(NT))) return rc;
-  return launch_kernel("gated linear", reinterpret_cast<const void*>(kernel), dim3((unsigned)grid), dim3(ROWS_THREADS), smem, st, p.split, false, p);
+  return launch_kernel("gated linear", reinterpret_cast<const void*>(kernel), dim3((unsigned)grid), dim3(ROWS_THREADS), smem, st, p.split, true, p);
 }
 
 int run_rows(const RowsCall& call, int dtype, cudaStream_t st) {

@@ -161,6 +161,12 @@ __global__ void __launch_bounds__(THREADS, 1) w4_kernel(const __grid_constant__ 
       ++ahead_u;
     }
   };
+  if (lane == 0) {
+    for (int s = 0; s < p.slots; ++s) mbar_init(bar0 + 8 * s, 1);
+    fence_barrier_init();
+  }
+  pdl_wait();  // whatever ran ahead, the caller's kernels too
+  pdl_release();
   // x, ahead of the weight, whose slots it would have to wait for; zeros behind its last column, and in place of its missing rows
   {
     const int units16 = steps * GT * 8, full = width / 8;  // 16-byte units of a row
@@ -172,11 +178,8 @@ __global__ void __launch_bounds__(THREADS, 1) w4_kernel(const __grid_constant__ 
     asm volatile("cp.async.commit_group;" ::: "memory");
     if (threadIdx.x < 16) reinterpret_cast<uint4*>(nothing)[threadIdx.x] = make_uint4(0, 0, 0, 0);
   }
-  if (lane == 0) {
-    for (int s = 0; s < p.slots; ++s) mbar_init(bar0 + 8 * s, 1);
-    fence_barrier_init();
+  if (lane == 0)
     for (int s = 0; s < p.slots && ahead < end; ++s) fetch(s);
-  }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();
   bool failed = false;
@@ -226,6 +229,7 @@ __global__ void __launch_bounds__(THREADS, 1) w4_kernel(const __grid_constant__ 
       break;
     }
     const int n = min(min(p.slot_steps, end - at), steps - k);
+    if (p.bias && k + n == steps && lane == 0) asm volatile("prefetch.global.L1 [%0];" ::"l"(static_cast<const T*>(p.bias) + min((u0 + u) * TILE_N, p.N - 1)));
     const uint8_t* tiles = ring + slot * p.slot_bytes + lane * 16;
     const T* scales = reinterpret_cast<const T*>(ring + slot * p.slot_bytes + p.scale_at) + r;
     const uint8_t* zeros = ring + slot * p.slot_bytes + p.zero_at + r;
@@ -333,7 +337,7 @@ template <typename T, int NT, bool ZEROS, int G> static int launch(const Params&
   auto kernel = w4_kernel<T, NT, ZEROS, G>;
   static DeviceOnce limit;
   if (int rc = limit.raise_smem(reinterpret_cast<const void*>(kernel), SMEM_LIMIT - fixed_bytes(NT))) return rc;
-  return launch_kernel("w4 linear", reinterpret_cast<const void*>(kernel), dim3((unsigned)grid), dim3(THREADS), smem, st, p.split, false, p);
+  return launch_kernel("w4 linear", reinterpret_cast<const void*>(kernel), dim3((unsigned)grid), dim3(THREADS), smem, st, p.split, true, p);
 }
 template <typename T, int NT, bool ZEROS> static int with_group(const Params& p, int group, int grid, size_t smem, cudaStream_t st) {
   return group == 32 ? launch<T, NT, ZEROS, 32>(p, grid, smem, st) : group == 64 ? launch<T, NT, ZEROS, 64>(p, grid, smem, st) : launch<T, NT, ZEROS, 128>(p, grid, smem, st);
