@@ -471,7 +471,7 @@ typedef struct ksb_gated_linear_grads {
   int64_t M, F, K, ldx, ldg, ldu, lddh;
   int dtype, act;
 } ksb_gated_linear_grads;
-int64_t ksb_gated_linear_workspace(int64_t M, int64_t F);
+int64_t ksb_gated_linear_workspace(int64_t M, int64_t F, int64_t K);
 int ksb_gated_linear_backward(const ksb_gated_linear_grads* args, void* workspace, ksb_stream_t stream);
 
 #ifdef __cplusplus

@@ -80,7 +80,7 @@ SIGNATURES = {
     "ksb_gated_linear": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int,
                                  c_void_p, c_void_p, c_void_p]),
     "ksb_gated_linear_saved": (c_int64, [c_int64, c_int64]),
-    "ksb_gated_linear_workspace": (c_int64, [c_int64, c_int64]),
+    "ksb_gated_linear_workspace": (c_int64, [c_int64, c_int64, c_int64]),
     "ksb_gated_linear_backward": (c_int, [c_void_p, c_void_p, c_void_p]),
 }
 

@@ -14,6 +14,8 @@
 //            In a CTA pair (cta_group::2, 256 x 256 tiles) the even CTA brings the rows of Wg, the odd one those of Wu.
 //   DX       two runs over F into one accumulator: A = dg, du as they lie, B = Wg, Wu read column by column (MN-major)
 //   DW       two problems of one launch: A = dg, du and B = x, all read column by column
+// The gradients of few output tiles with a long sum are split over it: each part leaves its fp32 accumulators in the workspace, and join_kernel
+// adds them up in the order of the sum.
 // A column-wise operand needs no transposed copy: a box of 64 columns x 64 rows lands in the layout that the tensor core reads as
 // MN-major with 128-byte swizzle.
 #include <algorithm>
@@ -55,7 +57,9 @@ struct Params {
   CUtensorMap a[2], b[2], out[5];  // PROJECT with `save`: h, upper and lower part of g, of u
   int M, N;                       // of the output
   int tiles_m, tiles_n, num_tiles, problem_tiles;
-  int steps, num_k;               // stages per run over the sum, and per tile
+  int steps, num_k;               // stages per run over the sum, and over all of it
+  int splits;                     // parts of the sum (gradients)
+  float* parts;                   // with several: [problem][part][tile][CTA of a pair][four columns][128 rows] float4
   int group_m;                    // row tiles that go through all columns together
   const void* b_gate;             // PROJECT: halves or null
   const void* b_up;
@@ -129,13 +133,23 @@ static Saved saved_layout(int64_t M, int64_t F) {
   return s;
 }
 
-__device__ __forceinline__ void tile_coords(const Params& p, int tile, int& problem, int& tm, int& tn) {
-  problem = tile / p.problem_tiles;
-  tile -= problem * p.problem_tiles;
+// A piece of work: an output tile, and the part [k0, k1) of the sum.
+struct Work {
+  int problem, tm, tn, k0, k1;
+};
+__device__ __forceinline__ Work work_of(const Params& p, int tile) {
+  Work w;
+  const int part = tile / p.problem_tiles;
+  w.problem = part / p.splits;
+  const int split = part - w.problem * p.splits;
+  w.k0 = static_cast<int>(static_cast<int64_t>(p.num_k) * split / p.splits);
+  w.k1 = static_cast<int>(static_cast<int64_t>(p.num_k) * (split + 1) / p.splits);
+  tile -= part * p.problem_tiles;
   const int per_group = p.group_m * p.tiles_n, rg = tile / per_group, first = rg * p.group_m;
   const int rows = min(p.group_m, p.tiles_m - first), r = tile - rg * per_group;
-  tm = first + r % rows;
-  tn = r / rows;
+  w.tm = first + r % rows;
+  w.tn = r / rows;
+  return w;
 }
 
 template <typename T, int KIND, int CTAS, int TN, bool FLEX>
@@ -193,10 +207,9 @@ __global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, FLEX>::THREADS, 1) gemm_ke
       uint32_t it = 0, s = 0, ph = 1;
       bool ok = true;
       for (int tile = worker; tile < p.num_tiles && ok; tile += workers) {
-        int problem, tm, tn;
-        tile_coords(p, tile, problem, tm, tn);
-        const int row = (tm * CTAS + (int)crank) * BM, col = tn * TN + (int)crank * C::B_ROWS;
-        for (int k = 0; k < p.num_k; ++k, ++it) {
+        const Work w = work_of(p, tile);
+        const int row = (w.tm * CTAS + (int)crank) * BM, col = w.tn * TN + (int)crank * C::B_ROWS;
+        for (int k = w.k0; k < w.k1; ++k, ++it) {
           if (!mbar_wait(empty0 + 8 * s, ph, p.status, (KERNEL_ID << 16) | 1)) { ok = false; break; }
           if (CTAS == 1) mbar_arrive_expect_tx(full0 + 8 * s, bytes);
           else if (crank == 0) mbar_arrive_expect_tx(full0 + 8 * s, 2 * bytes);
@@ -205,13 +218,13 @@ __global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, FLEX>::THREADS, 1) gemm_ke
           const CUtensorMap* map;
           int x, y;
           if (of_a) {
-            map = &p.a[KIND == DW ? problem : run];
+            map = &p.a[KIND == DW ? w.problem : run];
             x = KIND == DW ? row + 64 * box : kk;
             y = KIND == DW ? kk : row;
           } else {
             map = &p.b[KIND == PROJECT ? (CTAS == 2 ? (int)crank : box) : run];
             x = KIND == PROJECT ? kk : col + 64 * box;
-            y = KIND == PROJECT ? tn * OUT_N : kk;
+            y = KIND == PROJECT ? w.tn * OUT_N : kk;
           }
           const uint32_t dst = base + s * STAGE_BYTES + offset;
           if (CTAS == 2) tma_load_2d_pair(dst, map, mapa_shared(full0 + 8 * s, 0), x, y);
@@ -239,7 +252,8 @@ __global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, FLEX>::THREADS, 1) gemm_ke
         if (!mbar_wait(tempty0 + 8 * acc, aph ^ 1, p.status, (KERNEL_ID << 16) | 2)) break;
         tc_fence_after();
         const uint32_t d = tmem_base + acc * TN;
-        for (int k = 0; k < p.num_k; ++k) {
+        const Work w = work_of(p, tile);
+        for (int k = w.k0; k < w.k1; ++k) {
           if (!mbar_wait(full0 + 8 * s, ph, p.status, (KERNEL_ID << 16) | 3)) { ok = false; break; }
           tc_fence_after();
           const uint32_t sa = base + s * STAGE_BYTES, sb = sa + C::A_BYTES;
@@ -247,8 +261,8 @@ __global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, FLEX>::THREADS, 1) gemm_ke
 #pragma unroll
           for (int kk = 0; kk < BK / 16; ++kk) {  // 16 columns of the sum: 32 bytes of a row, or 16 rows of 128 bytes
             const uint64_t ak = da + kk * (a_mn ? 128 : 2), bk = db + kk * (b_mn ? 128 : 2);
-            if (CTAS == 2) mma_f16_pair(d, ak, bk, idesc, (k | kk) != 0);
-            else mma_bf16_ss(d, ak, bk, idesc, (k | kk) != 0);
+            if (CTAS == 2) mma_f16_pair(d, ak, bk, idesc, k != w.k0 || kk != 0);
+            else mma_bf16_ss(d, ak, bk, idesc, k != w.k0 || kk != 0);
           }
           if (CTAS == 2) mma_commit_pair(empty0 + 8 * s); else mma_commit(empty0 + 8 * s);
           if (++s == STAGES) {
@@ -273,10 +287,9 @@ __global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, FLEX>::THREADS, 1) gemm_ke
     const uint32_t tempty_even = CTAS == 2 ? mapa_shared(tempty0, 0) : 0u;
     uint32_t count = 0;
     for (int tile = worker; tile < p.num_tiles; tile += workers, ++count) {
-      int problem, tm, tn;
-      tile_coords(p, tile, problem, tm, tn);
+      const Work w = work_of(p, tile);
       const uint32_t acc = count & 1, aph = (count >> 1) & 1;
-      const int row0 = (tm * CTAS + (int)crank) * BM + q * 32, n0 = tn * OUT_N + col0;
+      const int row0 = (w.tm * CTAS + (int)crank) * BM + q * 32, n0 = w.tn * OUT_N + col0;
       // The biases of the warp's columns, as fp32, ahead of the accumulator: read behind it, column by column, they took 5 us of
       // 77 x 4096 x 10240.
       const uint32_t bias_at = biases + ew * (2 * C::BIAS_COLS * 4);
@@ -388,6 +401,15 @@ __global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, FLEX>::THREADS, 1) gemm_ke
           }
           close(&p.out[0]);
           }
+        } else if (p.splits > 1) {
+          float4* to = reinterpret_cast<float4*>(p.parts) + (static_cast<int64_t>(tile) * CTAS + crank) * (BM * TN / 4) + q * 32 + lane;
+#pragma unroll
+          for (int c = 0; c < C::PIECE_COLS; c += 16) {
+            float v[16];
+            take16(t_row + c, v);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) to[((col0 + c) / 4 + i) * BM] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+          }
         } else {
           open();
 #pragma unroll
@@ -402,7 +424,7 @@ __global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, FLEX>::THREADS, 1) gemm_ke
               put(c + e, y);
             }
           }
-          close(&p.out[problem]);
+          close(&p.out[w.problem]);
         }
       }
       tc_fence_before();
@@ -421,6 +443,51 @@ __global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, FLEX>::THREADS, 1) gemm_ke
   if (warp == C::LOADS) {
     tc_fence_after();
     if (CTAS == 2) tmem_dealloc_pair(tmem_base, C::TMEM_COLS); else tmem_dealloc(tmem_base, C::TMEM_COLS);
+  }
+}
+
+// The outputs of a split launch: a warp adds up 32 rows x 16 columns of the parts, in their order, a row per lane.
+struct JoinParams {
+  Params p;
+  void* out[2];
+  int problems, ctas, tile_cols;  // as the products' launch had them
+};
+template <typename T> __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ JoinParams j) {
+  const Params& p = j.p;
+  pdl_wait();
+  pdl_release();
+  const int lane = threadIdx.x & 31, groups = j.tile_cols / 16, per_tile = j.ctas * 4 * groups;  // of 16 columns
+  const int64_t total = static_cast<int64_t>(j.problems) * p.problem_tiles * per_tile, tile_floats = static_cast<int64_t>(j.ctas) * BM * j.tile_cols;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); i < total; i += static_cast<int64_t>(gridDim.x) * 8) {
+    const int64_t t = i / per_tile;
+    const int r = static_cast<int>(i - t * per_tile), crank = r / (4 * groups), q = r / groups % 4, g = r % groups;
+    const int problem = static_cast<int>(t / p.problem_tiles);
+    const int64_t first = static_cast<int64_t>(problem) * p.splits * p.problem_tiles + (t - static_cast<int64_t>(problem) * p.problem_tiles);  // its first part
+    const Work w = work_of(p, static_cast<int>(first));
+    const int row = (w.tm * j.ctas + crank) * BM + q * 32 + lane, col = w.tn * j.tile_cols + g * 16;
+    if (col >= p.N) continue;
+    const float4* from = reinterpret_cast<const float4*>(p.parts + first * tile_floats) + crank * (BM * j.tile_cols / 4) + g * 4 * BM + q * 32 + lane;
+    float4 v[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (row < p.M) {
+#pragma unroll 2
+      for (int s = 0; s < p.splits; ++s, from += static_cast<int64_t>(p.problem_tiles) * tile_floats / 4)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float4 f = from[c * BM];
+          v[c].x += f.x;
+          v[c].y += f.y;
+          v[c].z += f.z;
+          v[c].w += f.w;
+        }
+      T* to = static_cast<T*>(j.out[problem]) + static_cast<int64_t>(row) * p.N + col;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (col + 8 * h < p.N)
+          *reinterpret_cast<uint4*>(to + 8 * h) = make_uint4(HalfOps<T>::pack2(make_float2(v[2 * h].x, v[2 * h].y)), HalfOps<T>::pack2(make_float2(v[2 * h].z, v[2 * h].w)),
+                                                              HalfOps<T>::pack2(make_float2(v[2 * h + 1].x, v[2 * h + 1].y)), HalfOps<T>::pack2(make_float2(v[2 * h + 1].z, v[2 * h + 1].w)));
+    }
   }
 }
 
@@ -529,7 +596,7 @@ struct Job {
   Params p;
 };
 
-template <int KIND, int CTAS, int TN, bool FLEX = false> static int launch_form(Job& j, int dtype, bool chained, cudaStream_t st, int flex_cols = 0) {
+template <int KIND, int CTAS, int TN, bool FLEX = false> static int launch_form(Job& j, int dtype, bool chained, cudaStream_t st, int flex_cols = 0, int splits = 1) {
   using C = Cfg<KIND, CTAS, TN, FLEX>;
   Params& p = j.p;
   p.status = status_words();
@@ -546,12 +613,13 @@ template <int KIND, int CTAS, int TN, bool FLEX = false> static int launch_form(
   p.N = (int)j.N;
   p.tiles_m = (int)((j.M + CTAS * BM - 1) / (CTAS * BM));
   p.tiles_n = (int)((j.N + out_n - 1) / out_n);
-  const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n * j.problems;
+  const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n * j.problems * splits;
   if (tiles > INT32_MAX) return fail(KSB_ERR_UNSUPPORTED, "too many tiles");
   p.problem_tiles = p.tiles_m * p.tiles_n;
   p.num_tiles = (int)tiles;
   p.steps = (int)((j.sum + BK - 1) / BK);
   p.num_k = p.steps * (KIND == DX ? 2 : 1);
+  p.splits = splits;
   p.flex_cols = out_n;
   p.stages = std::min<int>(C::MOST, C::ROOM / (C::A_BYTES + 2 * out_n * ROW_BYTES));  // FLEX
   // Row tiles that share each column tile's operand while it is in L2; their own operand's rows are to take about 32 MB of it.
@@ -578,12 +646,53 @@ static int project(Job& j, int dtype, cudaStream_t st) {
   if (flex < wide && flex < pair) return launch_form<PROJECT, 1, 256, true>(j, dtype, true, st, cols);
   return wide < pair ? launch_form<PROJECT, 1, 256>(j, dtype, true, st) : launch_form<PROJECT, 2, 256>(j, dtype, true, st);
 }
-template <int KIND> static int gradient(Job& j, int dtype, cudaStream_t st) {
+
+// The form of a gradient's products, and into how many parts the sum is split.
+struct GradPlan {
+  int form, splits;  // 0: CTA pairs, 256 x 256; 1: 128 x 256; 2: 128 x 128
+  double us;
+  int64_t floats;    // of the parts
+};
+static GradPlan plan_gradient(int64_t M, int64_t N, int64_t num_k, int problems) {
   const int sms = sm_count();
-  const double pair = sms < 2 ? 1e30 : waves(j.M, j.N, 256, 256, sms / 2, j.problems) * 0.285, wide = waves(j.M, j.N, 128, 256, sms, j.problems) * 0.40;
-  const double narrow = waves(j.M, j.N, 128, 128, sms, j.problems) * 0.25;
-  if (narrow < wide && narrow < pair) return launch_form<KIND, 1, 128>(j, dtype, true, st);
-  return wide < pair ? launch_form<KIND, 1, 256>(j, dtype, true, st) : launch_form<KIND, 2, 256>(j, dtype, true, st);
+  const struct { int tm, tn, workers; double step; } forms[3] = {{256, 256, sms / 2, 0.285}, {128, 256, sms, 0.40}, {128, 128, sms, 0.25}};
+  GradPlan best{0, 1, 1e30, 0};
+  for (int f = 0; f < 3; ++f) {
+    if (forms[f].workers < 1) continue;
+    const int64_t tiles = ((M + forms[f].tm - 1) / forms[f].tm) * ((N + forms[f].tn - 1) / forms[f].tn) * problems, tile_floats = (int64_t)forms[f].tm * forms[f].tn;
+    for (int s = 1; s <= 64 && (s == 1 || num_k / s >= 8); ++s) {
+      // Estimated: waves x (stages of a part x time of a stage + output), and for a split the parts written and read at some 4 TB/s and
+      // the second launch.  With one part and with this rule, the elements' gradients included: dx of 300 x 1536 x 8960 83 and 45 us, of
+      // 1101 x 1536 x 4616 63 and 55.5; the weights' of 75600 x 256 x 512 396 and 147 us, of 32760 x 64 x 128 162 and 44.
+      const double waves = (double)((tiles * s + forms[f].workers - 1) / forms[f].workers);
+      const double us = waves * ((double)((num_k + s - 1) / s) * forms[f].step + 1.5) + (s > 1 ? 3.0 + (double)(tiles * s * tile_floats) * 8 / 4e6 : 0.0);
+      if (us < 0.97 * best.us) best = {f, s, us, s > 1 ? tiles * s * tile_floats : 0};
+      if (tiles * (s + 1) > 4 * (int64_t)forms[f].workers) break;
+    }
+  }
+  return best;
+}
+static int64_t num_k_of(int64_t sum, int runs) { return (sum + BK - 1) / BK * runs; }
+
+template <int KIND> static int gradient(Job& j, int dtype, float* parts, cudaStream_t st) {
+  // One weight gradient alone is planned as both are: the same bits whatever is asked for.
+  const GradPlan plan = plan_gradient(j.M, j.N, num_k_of(j.sum, KIND == DX ? 2 : 1), KIND == DX ? 1 : 2);
+  j.p.parts = parts;
+  int rc;
+  if (plan.form == 0) rc = launch_form<KIND, 2, 256>(j, dtype, true, st, 0, plan.splits);
+  else if (plan.form == 1) rc = launch_form<KIND, 1, 256>(j, dtype, true, st, 0, plan.splits);
+  else rc = launch_form<KIND, 1, 128>(j, dtype, true, st, 0, plan.splits);
+  if (rc || plan.splits == 1) return rc;
+  JoinParams join{};
+  join.p = j.p;
+  for (int i = 0; i < j.problems; ++i) join.out[i] = const_cast<void*>(j.out[i].ptr);
+  join.problems = j.problems;
+  join.ctas = plan.form == 0 ? 2 : 1;
+  join.tile_cols = plan.form == 2 ? 128 : 256;
+  const int64_t items = (int64_t)j.problems * j.p.problem_tiles * join.ctas * 4 * (join.tile_cols / 16);
+  const unsigned grid = (unsigned)std::min<int64_t>((items + 7) / 8, (int64_t)sm_count() * 8);
+  return launch_kernel("gated linear", dtype == KSB_BF16 ? reinterpret_cast<const void*>(join_kernel<__nv_bfloat16>) : reinterpret_cast<const void*>(join_kernel<__half>), dim3(grid),
+                       dim3(256), 0, st, 1, true, join);
 }
 
 static int64_t row_stretch(int64_t M, int64_t F) {
@@ -639,12 +748,16 @@ extern "C" int ksb_gated_linear(const void* x, int64_t ldx, const void* w_gate, 
 
 extern "C" int64_t ksb_gated_linear_saved(int64_t M, int64_t F) { return M <= 0 || F <= 0 || F % 8 != 0 ? 0 : gated::saved_layout(M, F).bytes; }
 
-// [dg][du][sums of the bias gradients]
+// [dg][du][sums of the bias gradients][parts of the products' sums: of dx, then of the weights']
 static int64_t gated_bytes(int64_t M, int64_t F) { return (M * F * 2 + 255) / 256 * 256; }
-extern "C" int64_t ksb_gated_linear_workspace(int64_t M, int64_t F) {
-  if (M <= 0 || F <= 0 || F % 8 != 0) return 0;
+static int64_t bias_bytes(int64_t M, int64_t F) {
   const int64_t stretch = gated::row_stretch(M, F);
-  return 2 * gated_bytes(M, F) + (M + stretch - 1) / stretch * 2 * F * 4;
+  return ((M + stretch - 1) / stretch * 2 * F * 4 + 255) / 256 * 256;
+}
+extern "C" int64_t ksb_gated_linear_workspace(int64_t M, int64_t F, int64_t K) {
+  if (M <= 0 || F <= 0 || F % 8 != 0 || K <= 0 || K % 8 != 0) return 0;
+  const int64_t floats = std::max(gated::plan_gradient(M, K, gated::num_k_of(F, 2), 1).floats, gated::plan_gradient(F, K, gated::num_k_of(M, 1), 2).floats);
+  return 2 * gated_bytes(M, F) + bias_bytes(M, F) + floats * 4;
 }
 
 extern "C" int ksb_gated_linear_backward(const ksb_gated_linear_grads* a, void* workspace, ksb_stream_t stream) {
@@ -667,6 +780,7 @@ extern "C" int ksb_gated_linear_backward(const ksb_gated_linear_grads* a, void* 
     if (!aligned16(t)) return fail(KSB_ERR_INVALID, "unaligned pointer");
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   void *dg = ws, *du = ws + gated_bytes(M, F);
+  float* parts = reinterpret_cast<float*>(ws + 2 * gated_bytes(M, F) + bias_bytes(M, F));
   const bool biases = a->db_gate || a->db_up;
   const int before = launch_count();
   gated::ActParams e{};
@@ -699,7 +813,7 @@ extern "C" int ksb_gated_linear_backward(const ksb_gated_linear_grads* a, void* 
     j.out[0] = {a->dx, M, K, K};
     j.outs = 1;
     j.M = M; j.N = K; j.sum = F; j.problems = 1;
-    if (int rc = gated::gradient<gated::DX>(j, a->dtype, st)) return rc;
+    if (int rc = gated::gradient<gated::DX>(j, a->dtype, parts, st)) return rc;
   }
   if (weights) {
     gated::Job j{};
@@ -715,7 +829,7 @@ extern "C" int ksb_gated_linear_backward(const ksb_gated_linear_grads* a, void* 
     j.outs = j.problems;
     j.b[0] = {a->x, M, K, M > 1 ? a->ldx : K};
     j.M = F; j.N = K; j.sum = M;
-    if (int rc = gated::gradient<gated::DW>(j, a->dtype, st)) return rc;
+    if (int rc = gated::gradient<gated::DW>(j, a->dtype, parts, st)) return rc;
   }
   return launch_count() - before;
 }

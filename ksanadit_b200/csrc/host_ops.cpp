@@ -197,7 +197,7 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
     const std::array<std::vector<int64_t>, 5> shapes{x.sizes().vec(), {s.F, s.K}, {s.F, s.K}, {s.F}, {s.F}};
     for (int i = 0; i < 5; ++i)
       if (need >> i & 1) out[i] = at::empty(shapes[i], x.options());
-    const Tensor ws = bytes(lib.gated_workspace(s.M, s.F), x);
+    const Tensor ws = bytes(lib.gated_workspace(s.M, s.F, s.K), x);
     ksb_gated_linear_grads a{};
     a.x = x.data_ptr(); a.w_gate = wg.data_ptr(); a.w_up = wu.data_ptr(); a.saved = saved[3].data_ptr(); a.dh = dh.data_ptr();
     a.dx = ptr(out[0]); a.dw_gate = ptr(out[1]); a.dw_up = ptr(out[2]); a.db_gate = ptr(out[3]); a.db_up = ptr(out[4]);

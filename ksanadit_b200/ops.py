@@ -876,7 +876,7 @@ class _GatedLinear(torch.autograd.Function):
             lib = _lib.load()
             args = native.GatedGrads(x2.data_ptr(), wg.data_ptr(), wu.data_ptr(), saved.data_ptr(), dh2.data_ptr(), *(_p(t) for t in out), M, F, K,
                                      x2.stride(0), wg.stride(0), wu.stride(0), dh2.stride(0), _dt(x), ctx.act)
-            ws = native.workspace(lib.ksb_gated_linear_workspace(M, F), x.device)
+            ws = native.workspace(lib.ksb_gated_linear_workspace(M, F, K), x.device)
             STATS.count(native.queued(lib.ksb_gated_linear_backward(ctypes.addressof(args), ws.data_ptr(), _stream()), "ksb_gated_linear_backward"))
         return (*out, None)
 

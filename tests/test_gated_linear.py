@@ -51,7 +51,11 @@ def test_c_entries_refuse_before_any_launch():
                dict(lddh=4), dict(ldx=12), dict(ldg=8), dict(ldu=17), dict(M=-1), dict(F=4), dict(K=4), dict(dtype=3), dict(act=-1)):
         assert backward(**kw) == -1, kw
     assert lib.ksb_gated_linear_backward(None, P, None) == -1
-    assert lib.ksb_gated_linear_workspace(0, 8) == 0 and lib.ksb_gated_linear_workspace(4, 12) == 0 and lib.ksb_gated_linear_workspace(4, 8) > 0
+    assert lib.ksb_gated_linear_workspace(0, 8, 8) == 0 and lib.ksb_gated_linear_workspace(4, 12, 8) == 0 and lib.ksb_gated_linear_workspace(4, 8, 12) == 0
+    assert lib.ksb_gated_linear_workspace(4, 8, 8) > 0
+    # few tiles and a long sum: room for its parts besides dg, du and the bias sums
+    assert lib.ksb_gated_linear_workspace(75600, 128, 256) > 4 * 75600 * 128 + 4 * 128 * 256 * 8
+    assert lib.ksb_gated_linear_saved(4, 8) > 0 and lib.ksb_gated_linear_saved(0, 8) == 0 and lib.ksb_gated_linear_saved(4, 9) == 0
 
 
 def test_registered_operators_have_shape_inference():

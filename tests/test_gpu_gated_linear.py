@@ -120,7 +120,8 @@ def test_forward(M, K, F, act, bias, dtype):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("act,bias", [("silu", True), ("gelu_tanh", False)])
 @pytest.mark.parametrize("M,K,F", [(1, 8, 8), (2, 72, 24), (33, 64, 128), (64, 128, 64), (65, 200, 72), (130, 520, 264), (257, 136, 1000), (300, 1536, 392), (1101, 264, 520),
-                                   (2500, 1160, 1288), (40, 8200, 16), (9000, 24, 40), (100, 72, 13832), (100, 20008, 64), (300, 72, 20008)])
+                                   (2500, 1160, 1288), (40, 8200, 16), (9000, 24, 40), (100, 72, 13832), (100, 20008, 64), (300, 72, 20008), (20000, 136, 72),
+                                   (6001, 264, 520), (513, 72, 9000), (7000, 8, 8)])
 def test_gradients(M, K, F, act, bias, dtype):
     t = _inputs(M, K, F, dtype, bias, M + K + F + 1)
     leaves = {k: t[k].requires_grad_(True) for k in ("x", "w_gate", "w_up", "b_gate", "b_up") if t[k] is not None}
