@@ -17,6 +17,9 @@
 // two, always the same columns, so that what the modulation and the weights make of them stays in registers as long as the modulation
 // row does.  A thread copies what it will read itself (cp.async) some rows ahead into a ring in shared memory: HBM is kept busy
 // through the exchanges of a row's sums, of which there are two to four, one after the other.
+//
+// Measured (bf16, RMS): forward 2 x 32760 x 1536 141 us (5.7 TB/s), 75600 x 5120 485 us (6.4 TB/s); backward 243 us (5.0) and 889 us (5.2 TB/s;
+// bound by issue slots: two exchanges or other numbers of warps and chunks were slower, below).  One row 6 us, all of it launch.
 #include <algorithm>
 
 #include "../../include/ksana_b200.h"
@@ -67,8 +70,7 @@ struct Grads {
 
 __device__ __forceinline__ uint4 load8(const void* base, int64_t offset_bytes) { return *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(base) + offset_bytes); }
 
-// Two fp32 numbers in one register pair; one instruction works on both (bound by issue slots, the backward pass took a third longer
-// without: 75600 x 5120 921 us against PLACE).
+// Two fp32 numbers in one register pair; one instruction works on both (backward pass of 75600 x 5120: 914 us, one by one 921).
 typedef unsigned long long F2;
 __device__ __forceinline__ F2 pair(float x, float y) {
   F2 r;

