@@ -12,6 +12,8 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
 #include <array>
@@ -113,9 +115,30 @@ int64_t asked(AutogradContext* ctx, int64_t there) {
     if (there >> i & 1) need |= static_cast<int64_t>(ctx->needs_input_grad(edge++)) << i;
   return need;
 }
-void not_twice(const variable_list& grads) {
-  if (!at::GradMode::is_enabled()) return;
-  for (const Tensor& g : grads) TORCH_CHECK(!g.defined() || !g.requires_grad(), "trying to differentiate twice a function that was marked with @once_differentiable");
+// Gradients that raise when they are differentiated again: with create_graph they would count as constants.
+constexpr const char* AGAIN = "the operators of a gated half have no second derivatives";
+variable_list last_derivatives(variable_list&& out, bool again) {
+  const auto node = again ? torch::autograd::get_current_node() : nullptr;
+  for (Tensor& g : out) {
+    if (!node || !g.defined()) continue;
+    torch::autograd::edge_list inputs = node->next_edges();
+    torch::autograd::create_gradient_edge(g, std::shared_ptr<torch::autograd::Node>(new torch::autograd::Error(AGAIN, std::move(inputs)), torch::autograd::deleteNode));
+  }
+  return std::move(out);
+}
+// A leaf's accumulation node keeps the stream that it was made on for as long as any graph of the leaf lives.  One of the default stream cannot take
+// part in a capture, and its failure inside the engine can end the process; here it is an error of this call, ahead of any launch.
+void leaves_can_be_captured() {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(c10::cuda::getCurrentCUDAStream().stream(), &status) != cudaSuccess || status == cudaStreamCaptureStatusNone) return;
+  const auto node = torch::autograd::get_current_node();
+  if (!node) return;
+  for (const auto& edge : node->next_edges()) {
+    if (!edge.function || !dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get())) continue;
+    const auto stream = edge.function->stream();
+    TORCH_CHECK(!stream || !stream->device().is_cuda() || c10::cuda::CUDAStream(*stream) != c10::cuda::getDefaultCUDAStream(stream->device_index()),
+                "a backward pass is captured while a graph of the same leaves that was made on the default stream is alive: release its outputs first");
+  }
 }
 PyObject* none() { Py_RETURN_NONE; }
 
@@ -184,7 +207,8 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
     return h;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    not_twice(grads);
+    leaves_can_be_captured();
+    const bool again = at::GradMode::is_enabled();
     at::NoGradGuard no_grad;
     variable_list out(6);
     if (!grads[0].defined()) return out;
@@ -204,7 +228,7 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
     a.M = s.M; a.F = s.F; a.K = s.K; a.ldx = s.ldx; a.ldg = s.ldg; a.ldu = s.ldu; a.lddh = s.F;
     a.dtype = dtype_of(x); a.act = static_cast<int>(ctx->saved_data["act"].toInt());
     count(lib.gated_backward(&a, ws.data_ptr(), stream_of(x)), "ksb_gated_linear_backward");
-    return out;
+    return last_derivatives(std::move(out), again);
   }
 };
 
@@ -338,7 +362,8 @@ struct SandwichNorm : torch::autograd::Function<SandwichNorm> {
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    not_twice(grads);
+    leaves_can_be_captured();
+    const bool again = at::GradMode::is_enabled();
     at::NoGradGuard no_grad;
     variable_list out(NORM_TENSORS + 4);
     const auto saved = ctx->get_saved_variables();
@@ -372,7 +397,7 @@ struct SandwichNorm : torch::autograd::Function<SandwichNorm> {
       if (out[i].numel() != t[i].numel()) out[i] = out[i].to(at::kFloat).sum(0).to(x.scalar_type());
       out[i] = out[i].view(t[i].sizes());
     }
-    return out;
+    return last_derivatives(std::move(out), again);
   }
 };
 
@@ -404,6 +429,14 @@ PyObject* sandwich_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// For a backward pass that runs in Python.
+PyObject* check_captured_leaves(PyObject*, PyObject*) {
+  HANDLE_TH_ERRORS
+  leaves_can_be_captured();
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
 // setup(dict with STATS, the library's exception, addresses of the nine entries above in their order)
 PyObject* setup(PyObject*, PyObject* args) {
   PyObject *ops, *error;
@@ -430,6 +463,7 @@ PyCFunction fast(PyObject* (*f)(PyObject*, PyObject* const*, Py_ssize_t)) { retu
 }  // namespace
 
 PyMethodDef op_methods[] = {{"setup", setup, METH_VARARGS, nullptr},
+                            {"check_captured_leaves", check_captured_leaves, METH_NOARGS, nullptr},
                             {"w4_linear", fast(w4_linear), METH_FASTCALL, nullptr},
                             {"gated_linear", fast(gated_linear), METH_FASTCALL, nullptr},
                             {"sandwich_norm", fast(sandwich_norm), METH_FASTCALL, nullptr},

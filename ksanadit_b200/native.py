@@ -209,6 +209,13 @@ def host_ops():
     return _host_ops
 
 
+def check_captured_leaves():
+    """Raises where a captured backward pass would reach leaves whose accumulation nodes belong to the default stream (the extension's check)."""
+    host = host_module()
+    if host:
+        host.check_captured_leaves()
+
+
 def linear_call(lin, call, dtype, device, quantize):
     """The C++ call of a Linear with descriptor ``call``; False where it has none, is not on a GPU, or was built from what a LinearCall
     cannot watch (a parameter of a tensor subclass, say): its calls go the general way."""

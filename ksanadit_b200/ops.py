@@ -739,6 +739,30 @@ def _norm_launch(x, y, gate, scale, shift, post_weight, pre_weight, residual_sca
     return r, h, stats, (x2, y2, g2, s2, h2)
 
 
+class _NoSecond(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, n_inputs, *inputs_and_grads):
+        return inputs_and_grads[n_inputs:]
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise _lib.KsanaB200Error("the operators of a gated half have no second derivatives")
+
+
+def _once(backward):
+    """Gradients that raise when they are differentiated again: with create_graph they would count as constants."""
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        again = torch.is_grad_enabled()
+        native.check_captured_leaves()
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        inputs = [t for t in ctx.saved_tensors if t is not None and t.requires_grad]
+        return _NoSecond.apply(len(inputs), *inputs, *out) if again else out
+
+    return run
+
+
 class _SandwichNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, y, gate, scale, shift, post_weight, pre_weight, residual_scale, pre, layer, eps, mod_rows):
@@ -749,7 +773,7 @@ class _SandwichNorm(torch.autograd.Function):
         return (None if y is None else r), h
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dr, dh):
         x, y, gate, scale, shift, post_weight, pre_weight, stats = ctx.saved_tensors
         residual_scale, pre, layer, eps, mod_rows = ctx.plain
@@ -858,14 +882,14 @@ class _GatedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, b_gate, b_up, act):
         h, saved = _gated_launch(x, w_gate, w_up, b_gate, b_up, act, True)
-        ctx.save_for_backward(x, w_gate, w_up, saved)
+        ctx.save_for_backward(x, w_gate, w_up, saved, b_gate, b_up)
         ctx.act = act
         return h
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dh):
-        x, w_gate, w_up, saved = ctx.saved_tensors
+        x, w_gate, w_up, saved = ctx.saved_tensors[:4]
         need = ctx.needs_input_grad
         F, K = w_gate.shape
         with torch.cuda.device(x.device):

@@ -325,3 +325,37 @@ def test_repeats_streams_and_graph():
     torch.cuda.synchronize()
     for a, b in zip(out, step()):
         assert torch.equal(a, b)
+
+
+def test_no_second_derivatives():
+    """With create_graph the gradients are the same ones; to differentiate them again is an error, not a constant."""
+    t = _inputs((2, 20, 72), (2, 1), True, torch.bfloat16, 21)
+    leaves = [t[n].requires_grad_(True) for n in NAMES]
+    step = lambda: torch.cat(ops.sandwich_norm(t["x"], **{n: t[n] for n in NAMES[1:]}))  # noqa: E731
+    whole = torch.autograd.grad(step().float().sum(), leaves)
+    again = torch.autograd.grad(step().float().sum(), leaves, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(whole, again))
+    for g in again:
+        with pytest.raises(RuntimeError, match="no second derivatives"):
+            torch.autograd.grad(g.float().square().sum(), leaves[0], allow_unused=True)
+
+
+def test_capture_with_eager_leaves_alive():
+    """A leaf's accumulation node of the default stream cannot take part in a capture: an error of the call, and nothing is lost."""
+    t = _inputs((2, 20, 72), (2, 1), True, torch.bfloat16, 21)
+    leaves = [t[n].requires_grad_(True) for n in NAMES]
+    step = lambda: torch.cat(ops.sandwich_norm(t["x"], **{n: t[n] for n in NAMES[1:]}))  # noqa: E731
+    eager = step()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="release its outputs"):
+        with torch.cuda.graph(graph):
+            torch.autograd.grad(step().sum(), leaves)
+    whole = torch.autograd.grad(eager.sum(), leaves)
+    del eager
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = torch.autograd.grad(step().sum(), leaves)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(out, whole))
+    _lib.assert_device_ok()
