@@ -141,3 +141,98 @@ def test_launches_are_counted_and_registered_operators_agree():
         assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
         w = m.modulation
         assert torch.equal(t.w4_linear(temb, w.weight, w.weight_scale, None, w.bias, 384), w(temb))
+
+
+def test_the_same_tensor_twice():
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x, w = (torch.randn(*s, device="cuda", generator=g).bfloat16() for s in ((70, 72), (136, 72)))
+    x2, w2 = x.clone(), w.clone()
+    for t in (x, w, x2, w2):
+        t.requires_grad_(True)
+    dh = torch.randn(70, 136, device="cuda", generator=g).bfloat16()
+    h = ops.gated_linear(x, w, w)
+    assert torch.equal(h, ops.gated_linear(x, w, w2))
+    both = torch.autograd.grad(ops.gated_linear(x, w, w2), [x, w, w2], dh)
+    one = torch.autograd.grad(h, [x, w], dh)
+    assert torch.equal(one[0], both[0]) and torch.equal(one[1], both[1] + both[2])
+    d = torch.randn(70, 72, device="cuda", generator=g).bfloat16()
+    r, n = ops.sandwich_norm(x, x, gate=x[0], scale=x[0])
+    r2, n2 = ops.sandwich_norm(x, x2, gate=x2[0], scale=x2[0])
+    assert torch.equal(r, r2) and torch.equal(n, n2)
+    one, two = torch.autograd.grad((r, n), [x], (d, d)), torch.autograd.grad((r2, n2), [x, x2], (d, d))
+    # the parts are rounded sums in either order: a few half steps of the largest
+    assert torch.allclose(one[0].float(), two[0].float() + two[1].float(), rtol=0, atol=4 * 2.0 ** -8 * float(two[1].abs().max() + two[0].abs().max()))
+
+
+def test_threads_and_streams_at_once():
+    """Calls of all three operators from several threads, each on its own stream, at the same time: nothing is shared between them."""
+    import threading
+    g = torch.Generator(device="cuda").manual_seed(6)
+    w = [(torch.randn(520, 264, device="cuda", generator=g) * 0.1).bfloat16() for _ in range(2)]
+    lin = B200W4Linear.from_float(torch.nn.Linear(264 - 264 % 32, 777, device="cuda"), 32)
+    xs = [torch.randn(m, 264, device="cuda", generator=g).bfloat16() for m in (3, 33, 300, 900)]
+
+    def run(x):
+        x = x.detach().requires_grad_(True)
+        h = ops.gated_linear(x, *w)
+        r, n = ops.sandwich_norm(x, x * 0.5)
+        with torch.no_grad():
+            small = lin(x[:9, :256].contiguous())
+        return [h.detach(), small, *torch.autograd.grad((h, r, n), [x], (h.detach(), r.detach(), n.detach()))]
+
+    want = [run(x) for x in xs]
+    torch.cuda.synchronize()
+    got, failed = [None] * len(xs), []
+
+    def worker(i):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(20):
+                    got[i] = run(xs[i])
+            stream.synchronize()
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=worker, args=(i,)) for i in range(len(xs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+    assert all(torch.equal(a, b) for p, q in zip(want, got) for a, b in zip(p, q))
+    _lib.assert_device_ok()
+
+
+def test_checkpoint_hooks_and_transforms():
+    from torch.utils.checkpoint import checkpoint
+    g = torch.Generator(device="cuda").manual_seed(7)
+    x = torch.randn(50, 72, device="cuda", generator=g).bfloat16().requires_grad_(True)
+    w = [(torch.randn(136, 72, device="cuda", generator=g) * 0.1).bfloat16().requires_grad_(True) for _ in range(2)]
+
+    def half(x, a, b):
+        return ops.sandwich_norm(ops.gated_linear(x, a, b), kind="layer")[1]
+
+    dh = torch.randn(50, 136, device="cuda", generator=g).bfloat16()
+    want = torch.autograd.grad(half(x, *w), [x, *w], dh)
+    got = torch.autograd.grad(checkpoint(half, x, *w, use_reentrant=False), [x, *w], dh)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    with torch.autograd.graph.save_on_cpu(pin_memory=False):
+        h = half(x, *w)
+    got = torch.autograd.grad(h, [x, *w], dh)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    # transforms see no kernel they could follow: refused, in either pass
+    h = half(x, *w)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(h, [x], torch.stack([dh, dh]), is_grads_batched=True)
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda v: half(v, *w))(torch.stack([x, x]))
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda v: half(v, *w).float().sum())(x)
+    h = half(x, *w)
+    with torch.no_grad():
+        w[0].mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(h, [x], dh)
+    with torch.inference_mode():
+        assert half(x, *w).shape == (50, 136)
