@@ -8,14 +8,17 @@
 // at most 15 in magnitude, exact in bf16 and fp16, so the products are exact and their sums are fp32 per group; the scale
 // multiplies a group's fp32 sum, it is never rounded into the weight.
 //
-// One CTA of sixteen warps per SM takes an even share of the row tiles, each warp an even share of that share's tiles: it copies
-// them, their scales and zero points into a ring of its own in shared memory, a few slots ahead (bulk copies; no warp waits for
-// another), and only at the end the sums of row tiles that several warps share are added up, in the order of the warps.  x
-// waits in shared memory.  Where it leaves no room for a ring, or there are few row tiles, the CTAs of a cluster share K: each
+// One CTA of sixteen warps per SM takes an even share of the row tiles, each warp an even share of that share's tiles.  A lane copies the
+// tiles' bytes that it will read itself (cp.async), and lanes of the warp the scales and zero points, into a ring of the warp's own, so no
+// warp waits for another until the end, when the sums of row tiles that several warps share are added up, in the order of the warps.  x
+// waits in shared memory.  Where it leaves no room for the rings, or there are few row tiles, the CTAs of a cluster share K: each
 // keeps its row tiles' sums, and in the end they are added up in the order of K through distributed shared memory.
 //
-// Measured: 1 x 5120 -> 30720 (81 MB) 18.6 us, of which the stream alone takes 15.8 and HBM's rate 12.5; 5 x 1536 -> 9216 in groups of 32
-// 6.3 us and 16 x 8960 -> 1533 9.8 us, where launch, x's way into shared memory and the last sums come one after the other.
+// Close to bound by issue slots, so a slot of the ring is four tiles, whose copies and products are unrolled, and what a warp keeps of its
+// place is one count.  1 x 5120 -> 30720 (81 MB): 16.3 us, without half the products 15.1, HBM's rate 12.5; with a step to a
+// slot (89 instructions a tile) 18.7, with bulk copies and mbarriers 18.4, and there deeper rings gained nothing.  8 rows 19.0 us, 16 rows 28.3; 4 x 13824
+// -> 30720 (222 MB) 40.2 us, 5.5 TB/s.  5 x 1536 -> 9216 in groups of 32 6.2 us and 16 x 8960 -> 1533 9.3 us, where launch, x's way into
+// shared memory and the last sums come one after the other.
 #include <algorithm>
 
 #include "../../include/ksana_b200.h"
@@ -25,11 +28,15 @@
 namespace ksb {
 namespace w4 {
 
-constexpr int KERNEL_ID = 6;
 constexpr int TILE_N = 16, TILE_K = 64, TILE_BYTES = 512;
 constexpr int WARPS = 16, THREADS = WARPS * 32;
-constexpr int MAX_SLOTS = 4;  // of a warp's ring
 constexpr int SMEM_LIMIT = 232448;
+// A step: the tiles of a group of 128 columns, or one tile.  A slot of a warp's ring: up to four tiles, their scales and zero points.
+constexpr int SLOT_TILES = 4;
+// Slots of a ring: a third one gains 4 % (1 x 5120 -> 30720 17.1 -> 16.3 us), and costs more where sixteen rows of x then need a cluster (28.3 -> 37.3 us).
+__host__ __device__ constexpr int depth(int nt) { return nt == 1 ? 3 : 2; }
+__host__ __device__ constexpr int step_tiles(int group) { return group == 128 ? 2 : 1; }
+__host__ __device__ constexpr int slot_bytes(int group, bool zeros) { return SLOT_TILES * TILE_BYTES + SLOT_TILES * TILE_K / group * (zeros ? 48 : 32); }
 
 struct Params {
   const void* x;
@@ -45,9 +52,7 @@ struct Params {
   int steps, groups;     // of a row tile (a step: GT tiles)
   int pitch;             // bytes between rows of x in shared memory: 64 more than a multiple of 128, so that the eight 16-byte
                          // reads of a quarter warp (two rows, four neighbours each) are in different banks
-  int slots, slot_steps, slot_bytes, scale_at, zero_at;  // a warp's ring
   int x_at, sums_at;     // in shared memory, behind the rings
-  int* status;
 };
 
 // Eight weights of a word as four pairs, (q - z) times UNIT: an AND (or one lop3) and one fma each, and one shift for the word; shifting every
@@ -107,11 +112,6 @@ template <typename T> __device__ __forceinline__ void mma16(float (&c)[4], const
   else mma_bf16(c, a, b0, b1, c0, c1, c2, c3);
 }
 
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
-               : "memory");
-}
-
 // 16 bytes, or zeros
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
   const int bytes = there ? 16 : 0;
@@ -127,47 +127,66 @@ __device__ __forceinline__ float load_cluster(uint32_t addr) {
 template <typename T, int NT, bool ZEROS, int G>
 __global__ void __launch_bounds__(THREADS, 1) w4_kernel(const __grid_constant__ Params p) {
   extern __shared__ __align__(128) uint8_t smem[];
-  constexpr int GT = G == 128 ? 2 : 1;        // tiles per step
-  constexpr int SCALES = G == 32 ? 2 : 1;     // groups per step
+  constexpr int GT = step_tiles(G), SCALES = G == 32 ? 2 : 1;  // tiles and groups per step
+  constexpr int SLOT = slot_bytes(G, ZEROS), SLOT_STEPS = SLOT_TILES / GT, GROUPS = SLOT_STEPS * SCALES, DEPTH = depth(NT);
+  constexpr int SLOT_BYTES = SLOT_TILES * TILE_BYTES, SCALE_AT = SLOT_BYTES, ZERO_AT = SCALE_AT + GROUPS * 32;
   constexpr int SUMS = TILE_N * 8 * NT;       // of a row tile: [row of x][row of the weight]
   // [0]: of the row tile that a warp comes into midway.  [1]: of the one it leaves midway, and on its way to memory any other's
   __shared__ __align__(16) float parts[2][WARPS][SUMS];
   __shared__ __align__(16) uint8_t nothing[256];  // x of the rows there are not
-  __shared__ __align__(8) uint64_t bars[WARPS * MAX_SLOTS];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
   const int split = p.split, rank = split > 1 ? (int)cluster_ctarank() : 0, cta = blockIdx.x, cluster = cta / split;
   const int k0 = p.steps * rank / split, steps = p.steps * (rank + 1) / split - k0;  // this CTA's steps of every row tile
   const int u0 = cluster * p.units_each + min(cluster, p.units_over), units = p.units_each + (cluster < p.units_over);
   const int64_t share = static_cast<int64_t>(units) * steps;
   const int begin = static_cast<int>(share * warp / WARPS), end = static_cast<int>(share * (warp + 1) / WARPS);
-  uint8_t* ring = smem + warp * p.slots * p.slot_bytes;
+  const uint8_t* ring = smem + warp * (DEPTH * SLOT);
   uint8_t* xs = smem + p.x_at;
   float* sums = reinterpret_cast<float*>(smem + p.sums_at);  // split: [row tile][SUMS]
-  const uint32_t ring_at = smem_u32(ring), bar0 = smem_u32(bars + warp * MAX_SLOTS);
+  const uint32_t ring_at = smem_u32(ring);
   int u = begin / steps, k = begin - u * steps;
-  int ahead = begin, ahead_u = u, ahead_k = k;  // of the next slot to ask for
-  const int x0 = k0 * GT * TILE_K, width = min(p.K - x0, steps * GT * TILE_K);  // this CTA's columns of x
-  // Up to a slot of steps, not past a row tile's end.
-  auto fetch = [&](int s) {
-    const int n = min(min(p.slot_steps, end - ahead), steps - ahead_k);
-    const int64_t row = u0 + ahead_u, kk = k0 + ahead_k, g0 = row * p.groups + kk * SCALES;
-    const uint32_t groups = SCALES == 1 ? n : min(2 * n, p.groups - 2 * (int)kk), bytes = n * GT * TILE_BYTES;
-    const uint32_t dst = ring_at + s * p.slot_bytes, bar = bar0 + 8 * s;
-    mbar_arrive_expect_tx(bar, bytes + groups * (ZEROS ? 48 : 32));
-    bulk_load(dst, p.weight + (row * p.steps + kk) * (GT * TILE_BYTES), bytes, bar);
-    bulk_load(dst + p.scale_at, p.scale + g0 * 32, groups * 32, bar);
-    if (ZEROS) bulk_load(dst + p.zero_at, p.zero + g0 * 16, groups * 16, bar);
-    ahead += n;
-    ahead_k += n;
-    if (ahead_k == steps) {
-      ahead_k = 0;
-      ++ahead_u;
-    }
+  // Of the next steps to ask for: row tile, how many the warp has of it from there on, and the lane's place in them.  Lanes bring the scales and
+  // zero points too, 16 bytes each.
+  int ahead_u = u, ahead_left = min(steps - k, end - begin);
+  const uint8_t* weight = p.weight + (static_cast<int64_t>(u0 + u) * p.steps + k0 + k) * (GT * TILE_BYTES) + lane * 16;
+  const bool is_zero = ZEROS && lane >= 2 * GROUPS, has_scale = lane < (ZEROS ? 3 : 2) * GROUPS;
+  const int group = is_zero ? lane - 2 * GROUPS : lane >> 1;  // in the slot
+  auto scale_place = [&](int at_k) {
+    const int64_t g = static_cast<int64_t>(u0 + ahead_u) * p.groups + static_cast<int64_t>(k0 + at_k) * SCALES + group;
+    return is_zero ? p.zero + g * 16 : p.scale + g * 32 + (lane & 1) * 16;
   };
-  if (lane == 0) {
-    for (int s = 0; s < p.slots; ++s) mbar_init(bar0 + 8 * s, 1);
-    fence_barrier_init();
-  }
+  const uint8_t* scale = scale_place(k);
+  const int last_u = (end - 1) / steps, last_steps = end - last_u * steps;
+  // a row's last half tile may be behind K: it has no group of its own (zeros here), and zeros in x
+  const bool lone = SCALES == 2 && (p.groups & 1) && k0 + steps == p.steps;
+  const int x0 = k0 * GT * TILE_K, width = min(p.K - x0, steps * GT * TILE_K);  // this CTA's columns of x
+  const uint32_t scale_to = ring_at + (is_zero ? ZERO_AT + group * 16 : SCALE_AT + lane * 16), tiles_to = ring_at + lane * 16;
+  // Up to a slot of steps, not past a row tile's end.
+  auto fetch = [&](int slot) {  // its place in bytes
+    if (ahead_left > SLOT_STEPS - (lone ? 0 : 1)) {
+#pragma unroll
+      for (int g = 0; g < SLOT_TILES; ++g) copy16(tiles_to + slot + g * TILE_BYTES, weight + g * TILE_BYTES, true);
+      if (has_scale) copy16(scale_to + slot, scale, true);
+      ahead_left -= SLOT_STEPS;
+      weight += SLOT_BYTES;
+      scale += is_zero ? GROUPS * 16 : GROUPS * 32;
+    } else if (ahead_left > 0) {
+      const int n = min(SLOT_STEPS, ahead_left), groups = n * SCALES - (lone && n == ahead_left && (ahead_u < last_u || last_steps == steps) ? 1 : 0);
+#pragma unroll 1
+      for (int g = 0; g < n * GT; ++g) copy16(tiles_to + slot + g * TILE_BYTES, weight + g * TILE_BYTES, true);
+      if (has_scale) copy16(scale_to + slot, group < groups ? scale : p.scale, group < groups);
+      ahead_left -= n;
+      weight += n * (GT * TILE_BYTES);
+      scale += n * SCALES * (is_zero ? 16 : 32);
+    }
+    if (ahead_left == 0 && ahead_u < last_u) {
+      ++ahead_u;
+      ahead_left = ahead_u == last_u ? last_steps : steps;
+      weight += static_cast<int64_t>(p.steps - steps) * (GT * TILE_BYTES);
+      scale = scale_place(0);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
   pdl_wait();  // whatever ran ahead, the caller's kernels too
   pdl_release();
   // x, ahead of the weight, whose slots it would have to wait for; zeros behind its last column, and in place of its missing rows
@@ -181,11 +200,10 @@ __global__ void __launch_bounds__(THREADS, 1) w4_kernel(const __grid_constant__ 
     asm volatile("cp.async.commit_group;" ::: "memory");
     if (threadIdx.x < 16) reinterpret_cast<uint4*>(nothing)[threadIdx.x] = make_uint4(0, 0, 0, 0);
   }
-  if (lane == 0)
-    for (int s = 0; s < p.slots && ahead < end; ++s) fetch(s);
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+  for (int d = 0; d < DEPTH - 1; ++d) fetch(d * SLOT);
+  asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory");  // x, asked for first
   __syncthreads();
-  bool failed = false;
 
   float acc[NT][4];
 #pragma unroll
@@ -215,38 +233,35 @@ __global__ void __launch_bounds__(THREADS, 1) w4_kernel(const __grid_constant__ 
   };
   const int live = p.M * TILE_N;  // sums that there are
   // a lane's x: of a row that there is not, the same zeros at every step
-  const uint8_t* x_at[NT];
+  const uint8_t *x_row[NT], *xk[NT];
   int x_step[NT];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const bool there = nt * 8 + r < p.M;
-    x_at[nt] = (there ? xs + (nt * 8 + r) * p.pitch : nothing) + t * 16;
     x_step[nt] = there ? GT * 128 : 0;
+    x_row[nt] = (there ? xs + (nt * 8 + r) * p.pitch : nothing) + t * 16;
+    xk[nt] = x_row[nt] + k * x_step[nt];
   }
   bool entered = k != 0;  // the row tile was begun by an earlier warp
-  int slot = 0;
-  uint32_t phase = 0;
-  for (int at = begin; at < end;) {
-    if (failed || !mbar_wait_warp(bar0 + 8 * slot, phase, p.status, (KERNEL_ID << 16) | 1)) {
-      failed = true;
-      break;
-    }
-    const int n = min(min(p.slot_steps, end - at), steps - k);
-    if (p.bias && k + n == steps && lane == 0) asm volatile("prefetch.global.L1 [%0];" ::"l"(static_cast<const T*>(p.bias) + min((u0 + u) * TILE_N, p.N - 1)));
-    const uint8_t* tiles = ring + slot * p.slot_bytes + lane * 16;
-    const T* scales = reinterpret_cast<const T*>(ring + slot * p.slot_bytes + p.scale_at) + r;
-    const uint8_t* zeros = ring + slot * p.slot_bytes + p.zero_at + r;
-    // a row's last half tile may be behind K: it has no group of its own, and zeros in x
-    const int lone = SCALES == 2 && (p.groups & 1) && k0 + k + n == p.steps ? n - 1 : -1;
-#pragma unroll 2
-    for (int j = 0; j < n; ++j) {
+  int slot = 0, free_slot = (DEPTH - 1) * SLOT;
+  int left = min(steps - k, end - begin);  // of the row tile
+  while (left > 0) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 2) : "memory");
+    __syncwarp();  // every lane's part of the slot is there, and the slot before has been read
+    fetch(free_slot);
+    free_slot = slot;
+    const uint8_t* tiles = ring + slot + lane * 16;
+    const T* scales = reinterpret_cast<const T*>(ring + slot + SCALE_AT) + r;
+    const uint8_t* zeros = ring + slot + ZERO_AT + r;
+    slot = slot == (DEPTH - 1) * SLOT ? 0 : slot + SLOT;
+    auto step = [&](int j) {
       float part[NT][4];
 #pragma unroll
       for (int half = 0; half < 2 * GT; ++half) {
-        const uint4 a4 = *reinterpret_cast<const uint4*>(tiles + (half >> 1) * TILE_BYTES);
+        const uint4 a4 = *reinterpret_cast<const uint4*>(tiles + (j * GT + (half >> 1)) * TILE_BYTES);
         const uint32_t w0 = half & 1 ? a4.z : a4.x, w1 = half & 1 ? a4.w : a4.y;
         const bool first = SCALES == 2 || half == 0, done = SCALES == 2 || half == 2 * GT - 1;
-        const int g = SCALES == 2 && half == 1 && j != lone ? TILE_N : 0;
+        const int g = (j * SCALES + (SCALES == 2 ? half : 0)) * TILE_N;
         uint32_t z0 = 8, z1 = 8;
         if (ZEROS) {
           z0 = zeros[g] & 15u;
@@ -269,7 +284,7 @@ __global__ void __launch_bounds__(THREADS, 1) w4_kernel(const __grid_constant__ 
         }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          const uint4 b = *reinterpret_cast<const uint4*>(x_at[nt] + (k + j) * x_step[nt] + half * 64);
+          const uint4 b = *reinterpret_cast<const uint4*>(xk[nt] + j * x_step[nt] + half * 64);
           mma16<T>(part[nt], a[0], b.x, b.y, first);
           mma16<T>(part[nt], a[1], b.z, b.w, false);
           if (done) {
@@ -280,32 +295,36 @@ __global__ void __launch_bounds__(THREADS, 1) w4_kernel(const __grid_constant__ 
           }
         }
       }
-      tiles += GT * TILE_BYTES;
-      scales += SCALES * TILE_N;
-      zeros += SCALES * TILE_N;
-    }
-    __syncwarp();
-    if (lane == 0 && ahead < end) fetch(slot);
-    if (++slot == p.slots) {
-      slot = 0;
-      phase ^= 1;
-    }
-    at += n;
-    k += n;
-    if (k == steps) {  // the end of a row tile
-      put(entered ? 0 : 1);
-      if (!entered) {
+    };
+    if (left >= SLOT_STEPS) {
+#pragma unroll
+      for (int j = 0; j < SLOT_STEPS; ++j) step(j);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) xk[nt] += SLOT_STEPS * x_step[nt];
+      left -= SLOT_STEPS;
+    } else {
 #pragma unroll 1
-        for (int j = lane; j < live; j += 32) keep(u, j, parts[1][warp][j]);
-        __syncwarp();
-      }
-      entered = false;
-      k = 0;
-      ++u;
+      for (int j = 0; j < left; ++j) step(j);
+      left = 0;
     }
-  }
-  if (failed) {  // what is on its way lands before the block leaves
-    for (int s = slot; s < slot + p.slots; ++s) mbar_wait(bar0 + 8 * (s % p.slots), phase ^ (s >= p.slots), p.status, (KERNEL_ID << 16) | 2);
+    if (left > 0) continue;
+    if (u == last_u && last_steps != steps) {  // left midway
+      k = last_steps;
+      break;
+    }
+    put(entered ? 0 : 1);
+    if (!entered) {
+#pragma unroll 1
+      for (int j = lane; j < live; j += 32) keep(u, j, parts[1][warp][j]);
+      __syncwarp();
+    }
+    entered = false;
+    k = 0;
+    if (++u > last_u) break;
+    left = u == last_u ? last_steps : steps;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) xk[nt] = x_row[nt];
+    if (p.bias && lane == 0) asm volatile("prefetch.global.L1 [%0];" ::"l"(static_cast<const T*>(p.bias) + min((u0 + u) * TILE_N, p.N - 1)));
   }
   if (begin == end || k != 0) put(begin == end || entered ? 0 : 1);  // without a share: zeros
   __syncthreads();
@@ -335,7 +354,7 @@ __global__ void __launch_bounds__(THREADS, 1) w4_kernel(const __grid_constant__ 
   }
 }
 
-constexpr int fixed_bytes(int nt) { return 2 * WARPS * TILE_N * 8 * nt * 4 + 256 + WARPS * MAX_SLOTS * 8 + 128; }
+constexpr int fixed_bytes(int nt) { return 2 * WARPS * TILE_N * 8 * nt * 4 + 256 + 128; }
 template <typename T, int NT, bool ZEROS, int G> static int launch(const Params& p, int grid, size_t smem, cudaStream_t st) {
   auto kernel = w4_kernel<T, NT, ZEROS, G>;
   static DeviceOnce limit;
@@ -367,8 +386,6 @@ extern "C" int ksb_w4_linear(const void* x, int dtype, int64_t M, int64_t K, int
   if (!aligned16(x) || !aligned16(weight) || !aligned16(scale) || (zero && !aligned16(zero)) || (M > 1 && (ldx < K || ldx % 8 != 0)) || (M > 1 && ldo < N))
     return fail(KSB_ERR_INVALID, "x, the packed weight, its scales and zero points must be 16-byte aligned, ldx %% 8 == 0");
   w4::Params p{};
-  p.status = status_words();
-  if (!p.status) return fail(KSB_ERR_CUDA, "status words unavailable");
   p.weight = static_cast<const uint8_t*>(weight);
   p.scale = static_cast<const uint8_t*>(scale);
   p.zero = static_cast<const uint8_t*>(zero);
@@ -376,32 +393,20 @@ extern "C" int ksb_w4_linear(const void* x, int dtype, int64_t M, int64_t K, int
   p.ldx = ldx; p.ldo = ldo;
   p.N = (int)N; p.K = (int)K;
   const int units = (int)((N + w4::TILE_N - 1) / w4::TILE_N);
-  const int tiles = (int)((K + w4::TILE_K - 1) / w4::TILE_K), step_tiles = group == 128 ? 2 : 1;
+  const int tiles = (int)((K + w4::TILE_K - 1) / w4::TILE_K), step_tiles = w4::step_tiles(group);
   p.steps = tiles / step_tiles;
   p.groups = (int)(K / group);
-  // A slot: eight tiles and their scales, or four where x leaves less room.
-  auto slot = [&](int slot_tiles) {
-    const int groups = slot_tiles / step_tiles * (group == 32 ? 2 : 1);
-    p.slot_steps = slot_tiles / step_tiles;
-    p.scale_at = slot_tiles * w4::TILE_BYTES;
-    p.zero_at = p.scale_at + groups * 32;
-    p.slot_bytes = (p.zero_at + (zero ? groups * 16 : 0) + 127) / 128 * 128;
-  };
   // K is shared by a cluster where that fills the GPU, or makes room for the rows of x.
   auto plan = [&](int rows, int split) {
     const int clusters = std::min(units, cluster_room(split)), sums = w4::TILE_N * (rows > 8 ? 16 : 8) * 4;
+    p.x_at = w4::WARPS * w4::depth(rows > 8 ? 2 : 1) * w4::slot_bytes(group, zero != nullptr);
     p.split = split;
     p.units_each = units / clusters;
     p.units_over = units % clusters;
     p.pitch = ((p.steps + split - 1) / split) * step_tiles * 128 + 64;
     const int64_t kept = split > 1 ? (int64_t)(p.units_each + 1) * sums : 0;
-    const int64_t room = (w4::SMEM_LIMIT - w4::fixed_bytes(rows > 8 ? 2 : 1) - (int64_t)rows * p.pitch - kept) / w4::WARPS;
-    slot(8);
-    if (room < 2 * p.slot_bytes) slot(4);
-    p.slots = (int)std::max<int64_t>(0, std::min<int64_t>(w4::MAX_SLOTS, room / p.slot_bytes));
-    p.x_at = w4::WARPS * p.slots * p.slot_bytes;
     p.sums_at = p.x_at + rows * p.pitch;
-    return p.slots >= 2 ? p.sums_at + (int)kept : 0;
+    return p.sums_at + kept <= w4::SMEM_LIMIT - w4::fixed_bytes(rows > 8 ? 2 : 1) ? (int)(p.sums_at + kept) : 0;
   };
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   int launches = 0;
