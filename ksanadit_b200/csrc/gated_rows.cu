@@ -11,7 +11,8 @@
 // for that, or there are few row tiles, the CTAs of a cluster share K: each keeps its row tiles' sums, and in the end they are added
 // up in the order of K through distributed shared memory.
 //
-// Measured: 1 x 1536 -> 8960 11.6 us (55 MB: 4.7 TB/s with launch and the last sums, 8.5 us at HBM's rate), 1 x 5120 -> 13824 48 us (5.9 TB/s).
+// Measured: 1 x 1536 -> 8960 11.3 us (55 MB: 4.9 TB/s with launch and the last sums, 8.5 us at HBM's rate), 1 x 5120 -> 13824 46.7 us (6.1 TB/s; 48.1
+// where the L2 does not ask for 256 bytes at once, 49.6 with a fourth slot, 49.2 with half of the products).
 #include <algorithm>
 
 #include "gated.h"
@@ -22,7 +23,7 @@ namespace gated {
 
 constexpr int TILE_F = 8, STEP = 64;                 // rows of each weight in a row tile, columns of a step
 constexpr int WARPS = 16, ROWS_THREADS = WARPS * 32;
-constexpr int DEPTH = 4, SLOT_BYTES = 2048;          // of a warp's ring: [block of 32 columns][weight][lane] 16 bytes
+constexpr int DEPTH = 3, SLOT_BYTES = 2048;          // of a warp's ring: [block of 32 columns][weight][lane] 16 bytes
 constexpr int SMEM_LIMIT = 232448;
 
 struct RowsParams {
@@ -34,9 +35,10 @@ struct RowsParams {
   int x_at, sums_at;           // in shared memory, behind the rings
 };
 
+// A step takes 128 bytes of a weight's row: the L2 asks for the next 128 with them.
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
   const int bytes = there ? 16 : 0;  // the rest is filled with zeros
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+  asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
 template <typename T> __device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1);
@@ -62,7 +64,7 @@ template <typename T, int NT> __global__ void __launch_bounds__(ROWS_THREADS, 1)
   __shared__ __align__(16) float parts[2][WARPS][SUMS];
   __shared__ __align__(16) uint8_t nothing[256];  // x of the rows there are not
   const RowsCall& c = p.c;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
   const int split = p.split, rank = split > 1 ? (int)cluster_ctarank() : 0, cluster = blockIdx.x / split;
   const int k0 = p.steps * rank / split, steps = p.steps * (rank + 1) / split - k0;  // this CTA's steps of every row tile
   const int u0 = cluster * p.units_each + min(cluster, p.units_over), units = p.units_each + (cluster < p.units_over);
