@@ -29,7 +29,8 @@
 namespace ksb {
 namespace norms {
 
-template <int NC> constexpr int backward_depth = NC == 4 ? 2 : 4;       // rows of the backward pass's ring
+// Rows of the backward pass's ring.  Of 5120 columns, three and four: 30000 rows 401 and 369 us, layer norm 380 and 396.
+template <int NC, bool LAYER> constexpr int backward_depth = NC == 4 ? 2 : LAYER ? 3 : 4;
 template <int NC> constexpr int backward_threads = NC == 4 ? 256 : 640;  // of a CTA, one per SM
 
 struct Params {
@@ -163,12 +164,19 @@ template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("c
 // sets of places, so that one barrier per exchange is enough.  The places behind the last warp's hold zeros.
 constexpr int PLACES = 8;
 constexpr int RED_FLOATS = 2 * PLACES * 64;  // groups x warps, in fours, are at most 64
-struct Group {
+// Every lane's v, all the same, for the compiler to know it: counts and addresses then leave the vector registers, and branches take one
+// instruction.  It is asked for (of the rows' counts, of the warps') where it gained.  us without and with: forward 30000 x 1536 70.9 and 65.0, x 4096
+// 169 and 155, 5000 x 5120 40.9 and 37.7, layer norm 2 x 32760 x 5120 646 and 582; but CTAs of all 320 threads with many rows, which
+// come to the copy's rate without it, lose: 75600 x 5120 485 and 531, 30000 x 2560 102 and 114.  Backward: four chunks, 20000 x 8192 442 and 365,
+// 75600 x 1 x 1536 877 and 744, layer norm 2 x 32760 x 5120 875 and (of the warps alone) 832; but 75600 x 5120 889 and 1081, 30000 x 1536 123 and 134.
+template <bool ASKED> __device__ __forceinline__ int uniform(int v) { return ASKED ? __shfl_sync(0xffffffffu, v, 0) : v; }
+
+template <bool UNIFORM> struct Group {
   float* red;  // [2][PLACES][warps, in fours]
   int id, warps, warp, lane, par;
   __device__ __forceinline__ Group(float* all, int group, int threads, int t)
-      : id(group), warps(threads / 32), warp(t >> 5), lane(t & 31), par(0) {
-    red = all + group * 2 * PLACES * four();
+      : id(uniform<UNIFORM>(group)), warps(threads / 32), warp(uniform<UNIFORM>(t >> 5)), lane(t & 31), par(0) {
+    red = all + id * 2 * PLACES * four();
     if (warps > 1)
       for (int i = t; i < 2 * PLACES * four(); i += threads) red[i] = 0.f;
     barrier();
@@ -248,8 +256,8 @@ struct Group {
 };
 
 // 1 / std of a row of which this thread holds NC chunks, and the row's mean; `chunk`(c) gives chunk c (zeros where there is none)
-template <int NC, bool LAYER, typename Chunk>
-__device__ __forceinline__ float2 row_stats(Group& g, const Chunk& chunk, const bool (&live)[NC], float inv_c, float eps, int place) {
+template <int NC, bool LAYER, typename Of, typename Chunk>
+__device__ __forceinline__ float2 row_stats(Of& g, const Chunk& chunk, const bool (&live)[NC], float inv_c, float eps, int place) {
   float mean = 0.f;
   if (LAYER) {
     F2 s = both(0.f);
@@ -277,20 +285,21 @@ __device__ __forceinline__ float2 row_stats(Group& g, const Chunk& chunk, const 
 }
 
 constexpr int FORWARD_DEPTH = 4;
-template <typename T, int NC, bool LAYER, int THREADS, int CTAS>
+template <typename T, int NC, bool LAYER, int THREADS, int CTAS, bool UNIFORM>
 __global__ void __launch_bounds__(THREADS, CTAS) forward_kernel(const __grid_constant__ Params p) {
   extern __shared__ __align__(16) uint8_t ring_bytes[];  // [FORWARD_DEPTH][x, y][NC][threads] 16 bytes
   __shared__ __align__(16) float red[RED_FLOATS];
   constexpr int DEPTH = FORWARD_DEPTH;
   const int t = threadIdx.x, nt = blockDim.x, chunks = p.C / 8, all = nt * blockDim.y;
-  Group g(red, threadIdx.y, nt, t);
+  const int y = uniform<UNIFORM>(threadIdx.y);
+  Group<UNIFORM> g(red, y, nt, t);
   const float inv_c = 1.f / static_cast<float>(p.C);
   bool live[NC];
 #pragma unroll
   for (int c = 0; c < NC; ++c) live[c] = t + c * nt < chunks;
   const int step = gridDim.x * blockDim.y;  // rows are below 2^31, and so is a row and DEPTH steps: see the launch
-  const uint32_t mine = smem_u32(ring_bytes) + (threadIdx.y * nt + t) * 16;
-  int ahead = blockIdx.x * blockDim.y + threadIdx.y;
+  const uint32_t mine = smem_u32(ring_bytes) + (y * nt + t) * 16;
+  int ahead = blockIdx.x * blockDim.y + y;
   auto fetch = [&](int slot) {
     if (ahead < p.M) {
 #pragma unroll
@@ -398,9 +407,11 @@ template <typename T, int NC, bool LAYER, bool WHOLE>
 __global__ void __launch_bounds__(backward_threads<NC>, 1) backward_kernel(const __grid_constant__ Params p, const __grid_constant__ Grads q) {
   extern __shared__ __align__(16) uint8_t ring_bytes[];  // [DEPTH][x, y, dr, dh][NC][threads] 16 bytes and the factors; in the end the groups' sums
   __shared__ __align__(16) float red[RED_FLOATS];
-  constexpr int DEPTH = backward_depth<NC>;
+  constexpr int DEPTH = backward_depth<NC, LAYER>;
   const int t = threadIdx.x, nt = blockDim.x, all = nt * blockDim.y;
-  Group g(red, threadIdx.y, nt, t);
+  constexpr bool ROWS = NC == 4 || WHOLE, WARPS = LAYER && !ROWS;
+  const int y = uniform<WARPS>(threadIdx.y), group_row = uniform<ROWS>(threadIdx.y);
+  Group<WARPS> g(red, y, nt, t);
   const float inv_c = 1.f / static_cast<float>(p.C);
   bool live[NC];
   Sums acc[NC];
@@ -414,17 +425,17 @@ __global__ void __launch_bounds__(backward_threads<NC>, 1) backward_kernel(const
   // the group's rows: row, row + step, .. below end
   int row, step, end;
   if (WHOLE) {
-    const int64_t groups = static_cast<int64_t>(gridDim.x) * blockDim.y, id = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+    const int64_t groups = static_cast<int64_t>(gridDim.x) * blockDim.y, id = static_cast<int64_t>(blockIdx.x) * blockDim.y + group_row;
     row = static_cast<int>(q.samples * id / groups) * p.rows_per_mod;
     end = static_cast<int>(q.samples * (id + 1) / groups) * p.rows_per_mod;
     step = 1;
   } else {
     const int b = blockIdx.x / q.chunks, of = b * p.rows_per_mod, from = of + (blockIdx.x - b * q.chunks) * q.chunk_rows;
     end = min(from + q.chunk_rows, of + p.rows_per_mod);
-    row = from + threadIdx.y;
+    row = from + group_row;
     step = blockDim.y;
   }
-  const uint32_t mine = smem_u32(ring_bytes) + (threadIdx.y * nt + t) * 16;
+  const uint32_t mine = smem_u32(ring_bytes) + (y * nt + t) * 16;
   auto place = [&](int slot, int which, int c) { return mine + ((slot * 4 + which) * NC + c) * all * 16; };
   int ahead = row;
   auto fetch = [&](int slot) {
@@ -774,8 +785,8 @@ static Plan plan_backward(int64_t M, int64_t C, int64_t rows_per_mod) {
   return s;
 }
 
-template <typename T, int NC, bool LAYER, int THREADS, int CTAS> static int forward_as(const Params& p, int threads, int groups, cudaStream_t st) {
-  auto kernel = forward_kernel<T, NC, LAYER, THREADS, CTAS>;
+template <typename T, int NC, bool LAYER, int THREADS, int CTAS, bool UNIFORM = true> static int forward_as(const Params& p, int threads, int groups, cudaStream_t st) {
+  auto kernel = forward_kernel<T, NC, LAYER, THREADS, CTAS, UNIFORM>;
   static DeviceOnce limit;
   if (int rc = limit.raise_smem(reinterpret_cast<const void*>(kernel), FORWARD_DEPTH * 2 * NC * THREADS * 16)) return rc;
   const int need = (p.M + groups - 1) / groups, room = sm_count() * CTAS;
@@ -789,13 +800,14 @@ template <typename T, bool LAYER> static int forward(const Params& p, cudaStream
     return forward_as<T, 1, LAYER, 256, 4>(p, threads, 256 / threads, st);
   }
   const int threads = (chunks + 63) / 64 * 32;
+  if (!LAYER && threads <= 320 && 320 / threads * threads == 320 && p.M > 16384) return forward_as<T, 2, false, 320, 2, false>(p, threads, 320 / threads, st);  // see uniform
   if (threads <= 320) return forward_as<T, 2, LAYER, 320, 2>(p, threads, 320 / threads, st);
   return forward_as<T, 2, LAYER, 512, 1>(p, threads, 1, st);
 }
 
 template <typename T, int NC, bool LAYER, bool WHOLE> static int backward_as(const Params& p, const Grads& q, const Plan& s, cudaStream_t st) {
   auto kernel = backward_kernel<T, NC, LAYER, WHOLE>;
-  constexpr int bytes = (backward_depth<NC> + 1) * 64 * NC;  // a thread: the ring, and the factors
+  constexpr int bytes = (backward_depth<NC, LAYER> + 1) * 64 * NC;  // a thread: the ring, and the factors
   static DeviceOnce limit;
   if (int rc = limit.raise_smem(reinterpret_cast<const void*>(kernel), bytes * backward_threads<NC>)) return rc;
   return launch_kernel("sandwich norm gradient", reinterpret_cast<const void*>(kernel), dim3((unsigned)s.ctas), dim3(s.threads, s.groups), bytes * s.threads * s.groups, st, 1, true, p, q);
