@@ -507,17 +507,21 @@ struct ActParams {
   int64_t low_ld, low, u;  // planes of what is saved
   int F, act;
 };
-template <typename T> __global__ void __launch_bounds__(256) act_grad_kernel(const __grid_constant__ ActParams p) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c * 8 >= p.F) return;
+// A CTA's threads: chunks of eight columns, and takers of turns over the rows of its stretch.  One row at a time and 64 registers, for four CTAs per
+// SM: 16380 x 13824 419 us (6.5 TB/s), with two rows at a time and two CTAs 597; 64 x 4 threads 423.
+constexpr int ACT_COLS = 32, ACT_ROWS = 8;
+template <typename T> __global__ void __launch_bounds__(ACT_COLS * ACT_ROWS, 4) act_grad_kernel(const __grid_constant__ ActParams p) {
+  __shared__ __align__(16) float sums[2][ACT_ROWS][ACT_COLS * 8];
+  const int c = blockIdx.x * ACT_COLS + threadIdx.x;
+  const bool live = c * 8 < p.F;
   pdl_wait();
   pdl_release();
-  const int64_t first = blockIdx.y * p.stretch, last = first + p.stretch < p.M ? first + p.stretch : p.M;
+  const int64_t first = blockIdx.y * p.stretch, last = !live ? 0 : first + p.stretch < p.M ? first + p.stretch : p.M;
   float sg[8], su[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) sg[i] = su[i] = 0.f;
-#pragma unroll 2
-  for (int64_t row = first; row < last; ++row) {
+#pragma unroll 1
+  for (int64_t row = first + threadIdx.y; row < last; row += ACT_ROWS) {
     const int64_t at = row * p.F + c * 8;
     const uint4 dv = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.dh) + row * p.lddh + c * 8);
     const uint8_t *hp = p.saved + at * 2, *lp = p.saved + p.low + row * p.low_ld + c * 8;
@@ -542,32 +546,43 @@ template <typename T> __global__ void __launch_bounds__(256) act_grad_kernel(con
     *reinterpret_cast<uint4*>(static_cast<T*>(p.dg) + at) = make_uint4(og[0], og[1], og[2], og[3]);
     *reinterpret_cast<uint4*>(static_cast<T*>(p.du) + at) = make_uint4(ou[0], ou[1], ou[2], ou[3]);
   }
-  if (p.parts) {
-    float* to = p.parts + static_cast<int64_t>(blockIdx.y) * 2 * p.F + c * 8;
+  if (p.parts) {  // the CTA's sums of its stretch, in the order of the turns
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const float* s = h ? su : sg;
-      *reinterpret_cast<float4*>(to + h * p.F) = make_float4(s[0], s[1], s[2], s[3]);
-      *reinterpret_cast<float4*>(to + h * p.F + 4) = make_float4(s[4], s[5], s[6], s[7]);
+      const float* v = h ? su : sg;
+      float4* at = reinterpret_cast<float4*>(&sums[h][threadIdx.y][threadIdx.x * 8]);
+      at[0] = make_float4(v[0], v[1], v[2], v[3]);
+      at[1] = make_float4(v[4], v[5], v[6], v[7]);
+    }
+    __syncthreads();
+    float* to = p.parts + static_cast<int64_t>(blockIdx.y) * 2 * p.F;
+    for (int i = threadIdx.y * ACT_COLS + threadIdx.x; i < 2 * ACT_COLS * 8; i += ACT_COLS * ACT_ROWS) {
+      const int h = i / (ACT_COLS * 8), j = i - h * (ACT_COLS * 8), col = blockIdx.x * (ACT_COLS * 8) + j;
+      float v = 0.f;
+#pragma unroll
+      for (int y = 0; y < ACT_ROWS; ++y) v += sums[h][y][j];
+      if (col < p.F) to[static_cast<int64_t>(h) * p.F + col] = v;
     }
   }
 }
-// The bias gradients from the stretches' sums, in their order: 32 columns and 8 takers of turns per CTA.
-template <typename T> __global__ void __launch_bounds__(256) bias_grad_kernel(const float* parts, int stretches, int F, void* dbg, void* dbu) {
-  __shared__ float sums[8][33];
-  const int lane = threadIdx.x & 31, j = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
+// The bias gradients from the stretches' sums, in their order: 32 columns and 32 takers of turns per CTA.
+constexpr int TAKERS = 32;
+template <typename T> __global__ void __launch_bounds__(32 * TAKERS) bias_grad_kernel(const float* parts, int stretches, int F, void* dbg, void* dbu) {
+  __shared__ float sums[TAKERS][33];
+  const int lane = threadIdx.x & 31, j = threadIdx.x >> 5;
+  const int64_t cols = 2 * static_cast<int64_t>(F), col = static_cast<int64_t>(blockIdx.x) * 32 + lane;
   pdl_wait();
   pdl_release();
   float s = 0.f;
-  if (col < 2 * F)
-#pragma unroll 8
-    for (int i = j; i < stretches; i += 8) s += parts[static_cast<int64_t>(i) * 2 * F + col];
+  if (col < cols)
+#pragma unroll 4
+    for (int i = j; i < stretches; i += TAKERS) s += parts[i * cols + col];
   sums[j][lane] = s;
   __syncthreads();
-  if (j != 0 || col >= 2 * F) return;
+  if (j != 0 || col >= cols) return;
   s = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) s += sums[i][lane];
+  for (int i = 0; i < TAKERS; ++i) s += sums[i][lane];
   void* to = col < F ? dbg : dbu;
   if (to) static_cast<T*>(to)[col < F ? col : col - F] = HalfOps<T>::from_f(s);
 }
@@ -706,9 +721,10 @@ template <int KIND> static int gradient(Job& j, int dtype, float* parts, cudaStr
 }
 
 static int64_t row_stretch(int64_t M, int64_t F) {
-  // rows per CTA: enough CTAs for four waves of eight per SM, at least 8 rows each
-  const int64_t columns = (F / 8 + 255) / 256, want = std::max<int64_t>(1, (int64_t)sm_count() * 32 / columns);
-  return std::max<int64_t>(8, (M + want - 1) / want);
+  // Rows per CTA: enough CTAs for two waves of four per SM, at least two rows a thread.  Shorter ones keep the bias sums busy: 32760 x 128 of two
+  // and eight rows a thread 29 and 20 us; longer ones the GPU idle: 1101 x 4616 12.9 and 15.0.
+  const int64_t columns = (F / 8 + ACT_COLS - 1) / ACT_COLS, want = std::max<int64_t>(1, (int64_t)sm_count() * 8 / columns);
+  return std::max<int64_t>(2, ((M + want - 1) / want + ACT_ROWS - 1) / ACT_ROWS) * ACT_ROWS;
 }
 
 }  // namespace gated
@@ -803,16 +819,16 @@ extern "C" int ksb_gated_linear_backward(const ksb_gated_linear_grads* a, void* 
   e.stretch = gated::row_stretch(M, F);
   const int stretches = (int)((M + e.stretch - 1) / e.stretch);
   const bool bf16 = a->dtype == KSB_BF16;
-  const dim3 grid((unsigned)((F / 8 + 255) / 256), (unsigned)stretches);
+  const dim3 grid((unsigned)((F / 8 + gated::ACT_COLS - 1) / gated::ACT_COLS), (unsigned)stretches);
   if (int rc = launch_kernel("gated linear", bf16 ? reinterpret_cast<const void*>(gated::act_grad_kernel<__nv_bfloat16>) : reinterpret_cast<const void*>(gated::act_grad_kernel<__half>),
-                             grid, dim3(256), 0, st, 1, true, e))
+                             grid, dim3(gated::ACT_COLS, gated::ACT_ROWS), 0, st, 1, true, e))
     return rc;
   if (biases) {
     const float* parts = e.parts;
     const int cols = (int)F;
     void *dbg = a->db_gate, *dbu = a->db_up;
     if (int rc = launch_kernel("gated linear", bf16 ? reinterpret_cast<const void*>(gated::bias_grad_kernel<__nv_bfloat16>) : reinterpret_cast<const void*>(gated::bias_grad_kernel<__half>),
-                               dim3((unsigned)((2 * F + 31) / 32)), dim3(256), 0, st, 1, true, parts, stretches, cols, dbg, dbu))
+                               dim3((unsigned)((2 * F + 31) / 32)), dim3(32 * gated::TAKERS), 0, st, 1, true, parts, stretches, cols, dbg, dbu))
       return rc;
   }
   if (a->dx) {
