@@ -20,7 +20,9 @@
 // MN-major with 128-byte swizzle.
 //
 // Measured (bf16): 32760 x 1536 -> 8960 1155 us (1560 TFLOP/s, the library's product alone 1450; 1390 us once the card is at its power limit);
-// forward and backward pass of 16380 x 5120 x 13824 11.5 - 12.1 ms (1200 TFLOP/s; the gradients read both operands column by column).
+// forward and backward pass of 16380 x 5120 x 13824 11.4 - 12.1 ms (1150 - 1220 TFLOP/s, at the power limit).  8192 x 4096 x 4096 1432 (with what the
+// backward pass is kept), dx 1494, weights' gradients 1492 TFLOP/s: operands that are read column by column cost nothing.  A pair's step of 64
+// columns takes 0.36 - 0.37 us whether its tile is 256, 224 or 192 wide (512 x 4096 x 10240), so narrower tiles for even waves gained 3 % at best.
 // 77 x 4096 x 10240 34 us, where the weights alone are 26: a product of 128 rows costs some 115 cycles however few its columns are, so
 // tiles of as many columns as there are CTAs for are taken (FLEX).
 #include <algorithm>
