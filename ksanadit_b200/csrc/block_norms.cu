@@ -18,8 +18,9 @@
 // row does.  A thread copies what it will read itself (cp.async) some rows ahead into a ring in shared memory: HBM is kept busy
 // through the exchanges of a row's sums, of which there are two to four, one after the other.
 //
-// Measured (bf16, RMS): forward 2 x 32760 x 1536 141 us (5.7 TB/s), 75600 x 5120 485 us (6.4 TB/s); backward 243 us (5.0) and 889 us (5.2 TB/s;
-// bound by issue slots: two exchanges or other numbers of warps and chunks were slower, below).  One row 6 us, all of it launch.
+// Measured (bf16, RMS): forward 2 x 32760 x 1536 134 us (6.0 TB/s), 75600 x 5120 485 us (6.4 TB/s); backward 242 us (5.0) and 889 us (5.2 TB/s: without
+// the barrier of a row's exchange, as a probe, 762; two exchanges, other numbers of warps and chunks, a barrier in two halves were slower).  One
+// row 6 us, all of it launch.
 #include <algorithm>
 
 #include "../../include/ksana_b200.h"
@@ -663,7 +664,8 @@ __global__ void __launch_bounds__(backward_threads<NC>, 1) backward_kernel(const
 }
 
 // Adds up the stretches' sums, in order: 32 columns per CTA, 16 threads per column, which take turns over the stretches of a
-// modulation row, or over the modulation rows where there are many.
+// modulation row, or over the modulation rows where there are many.  Without gradients of the weights, which are sums over all of them, the
+// modulation rows have CTAs of their own (backward pass of 3 x 777 x 2056 25.0 and 22.4 us, of 8 x 777 x 2048 51.4 and 42.9).
 constexpr int FINISH = 16;
 template <typename T> __global__ void __launch_bounds__(32 * FINISH) finish_kernel(const __grid_constant__ Params p, const __grid_constant__ Grads q) {
   __shared__ float part[3][FINISH][33];
@@ -698,7 +700,7 @@ template <typename T> __global__ void __launch_bounds__(32 * FINISH) finish_kern
   };
   float s[3];
   if (by_sample) {
-    for (int b = j; b < q.samples; b += FINISH) {
+    for (int b = blockIdx.y * FINISH + j; b < q.samples; b += gridDim.y * FINISH) {
       sums(b, 0, 1, s);
       write(b, s[0], s[1], s[2]);
     }
@@ -712,7 +714,7 @@ template <typename T> __global__ void __launch_bounds__(32 * FINISH) finish_kern
       dwn += part[1][k][lane];
     }
   } else {
-    for (int b = 0; b < q.samples; ++b) {
+    for (int b = blockIdx.y; b < q.samples; b += gridDim.y) {
       sums(b, j, FINISH, s);
 #pragma unroll
       for (int i = 0; i < 3; ++i) part[i][j][lane] = s[i];
@@ -823,7 +825,8 @@ template <typename T> static int backward(const Params& p, const Grads& q, const
   const dim3 grid((unsigned)((p.C + 31) / 32)), block(32, FINISH);
   if (!s.whole) {
     if (!q.dgate && !q.dscale && !q.dshift && !q.dpost_w && !q.dpre_w) return 0;
-    return launch_kernel("sandwich norm sums", reinterpret_cast<const void*>(finish_kernel<T>), grid, block, 0, st, 1, true, p, q);
+    const unsigned apart = q.dpost_w || q.dpre_w ? 1 : q.samples < FINISH ? q.samples : (q.samples + FINISH - 1) / FINISH;
+    return launch_kernel("sandwich norm sums", reinterpret_cast<const void*>(finish_kernel<T>), dim3(grid.x, apart), block, 0, st, 1, true, p, q);
   }
   if (!q.dpost_w && !q.dpre_w) return 0;
   return launch_kernel("sandwich norm sums", reinterpret_cast<const void*>(finish_weights_kernel), grid, block, 0, st, 1, true, p, q, s.ctas);
