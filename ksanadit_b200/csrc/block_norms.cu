@@ -158,6 +158,12 @@ template <typename T> __device__ __forceinline__ V8 pre_factor(const Params& p, 
 __device__ __forceinline__ void copy8(uint32_t dst, const void* base, int64_t offset_bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(static_cast<const uint8_t*>(base) + offset_bytes) : "memory");
 }
+// Where every row has a modulation row of its own, the L2 asks for it with the row's copies, some rows ahead of its use.  us without and with:
+// forward 75600 x 1 x 1536 397 and 355, 32760 x 1 x 5120 609 and 583 (1560 rows, which lie in the L2: 35.7 and 38.0, so of many rows only);
+// backward 747 and 669, 1172 and 1066, 97.8 and 93.5.
+__device__ __forceinline__ void ask_for(const void* base, int64_t offset_bytes) {
+  if (base) asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const uint8_t*>(base) + offset_bytes));
+}
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
@@ -286,7 +292,7 @@ __device__ __forceinline__ float2 row_stats(Of& g, const Chunk& chunk, const boo
 }
 
 constexpr int FORWARD_DEPTH = 4;
-template <typename T, int NC, bool LAYER, int THREADS, int CTAS, bool UNIFORM>
+template <typename T, int NC, bool LAYER, int THREADS, int CTAS, bool UNIFORM, bool APART>
 __global__ void __launch_bounds__(THREADS, CTAS) forward_kernel(const __grid_constant__ Params p) {
   extern __shared__ __align__(16) uint8_t ring_bytes[];  // [FORWARD_DEPTH][x, y][NC][threads] 16 bytes
   __shared__ __align__(16) float red[RED_FLOATS];
@@ -308,6 +314,11 @@ __global__ void __launch_bounds__(THREADS, CTAS) forward_kernel(const __grid_con
         if (live[c]) {
           copy8(mine + ((slot * 2) * NC + c) * all * 16, p.x, (static_cast<int64_t>(ahead) * p.ldx + (t + c * nt) * 8) * 2);
           if (p.y) copy8(mine + ((slot * 2 + 1) * NC + c) * all * 16, p.y, (static_cast<int64_t>(ahead) * p.ldy + (t + c * nt) * 8) * 2);
+          if (APART) {
+            ask_for(p.gate, (ahead * p.gate_stride + (t + c * nt) * 8) * 2);
+            ask_for(p.scale, (ahead * p.scale_stride + (t + c * nt) * 8) * 2);
+            ask_for(p.shift, (ahead * p.shift_stride + (t + c * nt) * 8) * 2);
+          }
         }
     }
     ahead += step;
@@ -453,6 +464,10 @@ __global__ void __launch_bounds__(backward_threads<NC>, 1) backward_kernel(const
           if (p.y) copy8(place(slot, 1, c), py, c * nt * 16);
           if (q.dr) copy8(place(slot, 2, c), pr, c * nt * 16);
           if (q.dh) copy8(place(slot, 3, c), ph, c * nt * 16);
+          if (WHOLE && p.rows_per_mod == 1) {
+            ask_for(p.gate, (at * p.gate_stride + (t + c * nt) * 8) * 2);
+            ask_for(p.scale, (at * p.scale_stride + (t + c * nt) * 8) * 2);
+          }
         }
     }
     ahead += step;
@@ -787,13 +802,18 @@ static Plan plan_backward(int64_t M, int64_t C, int64_t rows_per_mod) {
   return s;
 }
 
-template <typename T, int NC, bool LAYER, int THREADS, int CTAS, bool UNIFORM = true> static int forward_as(const Params& p, int threads, int groups, cudaStream_t st) {
-  auto kernel = forward_kernel<T, NC, LAYER, THREADS, CTAS, UNIFORM>;
+template <typename T, int NC, bool LAYER, int THREADS, int CTAS, bool UNIFORM, bool APART> static int forward_kind(const Params& p, int threads, int groups, cudaStream_t st) {
+  auto kernel = forward_kernel<T, NC, LAYER, THREADS, CTAS, UNIFORM, APART>;
   static DeviceOnce limit;
   if (int rc = limit.raise_smem(reinterpret_cast<const void*>(kernel), FORWARD_DEPTH * 2 * NC * THREADS * 16)) return rc;
   const int need = (p.M + groups - 1) / groups, room = sm_count() * CTAS;
   return launch_kernel("sandwich norm", reinterpret_cast<const void*>(kernel), dim3((unsigned)std::min(need, room)), dim3(threads, groups),
                        FORWARD_DEPTH * 2 * NC * threads * groups * 16, st, 1, true, p);
+}
+template <typename T, int NC, bool LAYER, int THREADS, int CTAS> static int forward_as(const Params& p, int threads, int groups, cudaStream_t st) {
+  if (p.rows_per_mod == 1 && p.M > 4096 && (p.gate || p.scale || p.shift)) return forward_kind<T, NC, LAYER, THREADS, CTAS, true, true>(p, threads, groups, st);
+  if (!LAYER && THREADS == 320 && groups * threads == 320 && p.M > 16384) return forward_kind<T, NC, LAYER, THREADS, CTAS, LAYER || THREADS != 320, false>(p, threads, groups, st);  // see uniform
+  return forward_kind<T, NC, LAYER, THREADS, CTAS, true, false>(p, threads, groups, st);
 }
 template <typename T, bool LAYER> static int forward(const Params& p, cudaStream_t st) {
   const int chunks = p.C / 8;
@@ -802,7 +822,6 @@ template <typename T, bool LAYER> static int forward(const Params& p, cudaStream
     return forward_as<T, 1, LAYER, 256, 4>(p, threads, 256 / threads, st);
   }
   const int threads = (chunks + 63) / 64 * 32;
-  if (!LAYER && threads <= 320 && 320 / threads * threads == 320 && p.M > 16384) return forward_as<T, 2, false, 320, 2, false>(p, threads, 320 / threads, st);  // see uniform
   if (threads <= 320) return forward_as<T, 2, LAYER, 320, 2>(p, threads, 320 / threads, st);
   return forward_as<T, 2, LAYER, 512, 1>(p, threads, 1, st);
 }

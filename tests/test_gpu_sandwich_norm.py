@@ -135,7 +135,7 @@ def _compare(name, got, ref, size, rows=0):
 SHAPES = [
     ((1, 8), (1,), True), ((5, 64), (5,), True), ((3, 7, 40), (3, 1), False), ((2, 33, 1536), (2, 1), True), ((2, 65, 1544), (), True), ((1, 130, 5120), (1, 1), True),
     ((2, 5, 8192), (2, 5), False), ((400, 3, 72), (400, 1), True), ((2, 300, 264), (2, 300), True), ((600, 2056), (300,), False), ((3, 777, 520), (3,), True),
-    ((2, 3, 4, 136), (2, 3, 1), True), ((40000, 16), (2,), True), ((16500, 528), (1,), True), ((200, 2, 5200), (200, 1), True)]
+    ((2, 3, 4, 136), (2, 3, 1), True), ((40000, 16), (2,), True), ((16500, 528), (1,), True), ((4100, 264), (4100,), True), ((2, 2100, 1544), (2, 2100), False), ((200, 2, 5200), (200, 1), True)]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
