@@ -17,6 +17,7 @@
 #include <torch/csrc/jit/frontend/tracer.h>
 
 #include <array>
+#include <atomic>
 
 #include "../../include/ksana_b200.h"
 
@@ -38,29 +39,23 @@ struct Library {
   decltype(&ksb_sandwich_norm_workspace) norm_workspace = nullptr;
   decltype(&ksb_sandwich_norm_backward) norm_backward = nullptr;
   decltype(&ksb_last_error) last_error = nullptr;
-  PyObject* ops = nullptr;    // dict of the module that holds STATS
   PyObject* error = nullptr;  // the library's exception
 } lib;
 
-// Kernels queued by a call, or its refusal.  Takes the interpreter.
+std::atomic<int64_t> kernels{0};  // that the calls here have queued
+
+// Kernels queued by a call, or its refusal, for which alone the interpreter is taken: in the engine's thread that takes 4 us.
 void count(int rc, const char* what) {
+  if (rc >= 0) {
+    kernels += rc;
+    return;
+  }
   PyGILState_STATE gil = PyGILState_Ensure();
-  PyObject* r = nullptr;
-  if (rc < 0) {
-    PyErr_Format(lib.error, "%s failed (rc=%d): %s", what, rc, lib.last_error());
-  } else if (PyObject* stats = PyDict_GetItemString(lib.ops, "STATS")) {
-    Ref held(stats);
-    r = PyObject_CallMethod(stats, "count", "i", rc);
-  }
-  if (!r) {
-    if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, "no launch statistics");
-    python_error e;
-    e.persist();
-    PyGILState_Release(gil);
-    throw e;
-  }
-  Py_DECREF(r);
+  PyErr_Format(lib.error, "%s failed (rc=%d): %s", what, rc, lib.last_error());
+  python_error e;
+  e.persist();
   PyGILState_Release(gil);
+  throw e;
 }
 
 int dtype_of(const Tensor& t) { return t.scalar_type() == at::kBFloat16 ? KSB_BF16 : KSB_FP16; }
@@ -71,7 +66,7 @@ void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 // Whether plain calls may take this way at all just now.
 bool watched() {
-  return lib.ops == nullptr || at::impl::torch_function_mode_enabled() || c10::impl::TorchDispatchModeTLS::any_modes_set() || torch::jit::tracer::isTracing();
+  return lib.error == nullptr || at::impl::torch_function_mode_enabled() || c10::impl::TorchDispatchModeTLS::any_modes_set() || torch::jit::tracer::isTracing();
 }
 // A tensor argument, or none (undefined) where that is allowed.  False: not a plain one.
 bool take(PyObject* o, bool optional, Tensor& t) {
@@ -383,7 +378,8 @@ struct SandwichNorm : torch::autograd::Function<SandwichNorm> {
       const bool there = i == X || (i == Y || i == GATE || i == POST ? behind : dh.defined());
       if (!(need >> i & 1) || !there) continue;
       if (i == POST || i == PRE) out[i] = at::empty({c.a.C}, x.options().dtype(at::kFloat));
-      else out[i] = i < GATE ? at::empty(x.sizes(), x.options()) : at::empty({c.a.mod_rows, c.a.C}, x.options());
+      else if (i < GATE) out[i] = at::empty(x.sizes(), x.options());
+      else out[i] = t[i].numel() == c.a.mod_rows * c.a.C ? at::empty(t[i].sizes(), x.options()) : at::empty({c.a.mod_rows, c.a.C}, x.options());
     }
     ksb_sandwich_norm_grads g{};
     g.dr = ptr(dr); g.dh = ptr(dh); g.lddr = g.lddh = c.a.C;
@@ -392,10 +388,9 @@ struct SandwichNorm : torch::autograd::Function<SandwichNorm> {
     const Tensor ws = bytes(lib.norm_workspace(c.a.M, c.a.C, c.a.mod_rows), x);
     count(lib.norm_backward(&c.a, &g, ws.data_ptr(), stream_of(x)), "ksb_sandwich_norm_backward");
     for (int i = GATE; i <= SHIFT; ++i) {
-      if (!out[i].defined()) continue;
+      if (!out[i].defined() || out[i].numel() == t[i].numel()) continue;
       // a tensor with one row for rows that others of the call tell apart
-      if (out[i].numel() != t[i].numel()) out[i] = out[i].to(at::kFloat).sum(0).to(x.scalar_type());
-      out[i] = out[i].view(t[i].sizes());
+      out[i] = out[i].to(at::kFloat).sum(0).to(x.scalar_type()).view(t[i].sizes());
     }
     return last_derivatives(std::move(out), again);
   }
@@ -437,11 +432,13 @@ PyObject* check_captured_leaves(PyObject*, PyObject*) {
   END_HANDLE_TH_ERRORS
 }
 
-// setup(dict with STATS, the library's exception, addresses of the nine entries above in their order)
+PyObject* queued(PyObject*, PyObject*) { return PyLong_FromLongLong(kernels); }
+
+// setup(the library's exception, addresses of the nine entries above in their order)
 PyObject* setup(PyObject*, PyObject* args) {
-  PyObject *ops, *error;
+  PyObject* error;
   unsigned long long at[9];
-  if (!PyArg_ParseTuple(args, "O!O(KKKKKKKKK)", &PyDict_Type, &ops, &error, at, at + 1, at + 2, at + 3, at + 4, at + 5, at + 6, at + 7, at + 8)) return nullptr;
+  if (!PyArg_ParseTuple(args, "O(KKKKKKKKK)", &error, at, at + 1, at + 2, at + 3, at + 4, at + 5, at + 6, at + 7, at + 8)) return nullptr;
   lib.w4 = reinterpret_cast<decltype(lib.w4)>(at[0]);
   lib.gated = reinterpret_cast<decltype(lib.gated)>(at[1]);
   lib.gated_saved = reinterpret_cast<decltype(lib.gated_saved)>(at[2]);
@@ -451,10 +448,8 @@ PyObject* setup(PyObject*, PyObject* args) {
   lib.norm_workspace = reinterpret_cast<decltype(lib.norm_workspace)>(at[6]);
   lib.norm_backward = reinterpret_cast<decltype(lib.norm_backward)>(at[7]);
   lib.last_error = reinterpret_cast<decltype(lib.last_error)>(at[8]);
-  Py_INCREF(ops);
   Py_INCREF(error);
-  Py_XSETREF(lib.error, error);
-  Py_XSETREF(lib.ops, ops);
+  Py_XSETREF(lib.error, error);  // the last: see watched
   Py_RETURN_NONE;
 }
 
@@ -463,6 +458,7 @@ PyCFunction fast(PyObject* (*f)(PyObject*, PyObject* const*, Py_ssize_t)) { retu
 }  // namespace
 
 PyMethodDef op_methods[] = {{"setup", setup, METH_VARARGS, nullptr},
+                            {"queued", queued, METH_NOARGS, nullptr},
                             {"check_captured_leaves", check_captured_leaves, METH_NOARGS, nullptr},
                             {"w4_linear", fast(w4_linear), METH_FASTCALL, nullptr},
                             {"gated_linear", fast(gated_linear), METH_FASTCALL, nullptr},

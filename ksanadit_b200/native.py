@@ -201,12 +201,16 @@ def host_ops():
     if _host_ops is None:
         _host_ops = host_module() or False
         if _host_ops:
-            from . import ops
             lib = _lib.load()
-            _host_ops.setup(vars(ops), _lib.KsanaB200Error, tuple(ctypes.cast(getattr(lib, n), c_void_p).value for n in (
+            _host_ops.setup(_lib.KsanaB200Error, tuple(ctypes.cast(getattr(lib, n), c_void_p).value for n in (
                 "ksb_w4_linear", "ksb_gated_linear", "ksb_gated_linear_saved", "ksb_gated_linear_workspace", "ksb_gated_linear_backward", "ksb_sandwich_norm",
                 "ksb_sandwich_norm_workspace", "ksb_sandwich_norm_backward", "ksb_last_error")))
     return _host_ops
+
+
+def queued_by_host_ops():
+    """Kernels that the extension's plain calls have queued."""
+    return _host_ops.queued() if _host_ops else 0
 
 
 def check_captured_leaves():

@@ -21,17 +21,26 @@ class LaunchStats:
     """Counts the CUDA kernels this library launches and, when ``timing`` is on, brackets every call of a
     chosen entry point with CUDA events on the launching stream (used by the benchmark's roofline)."""
 
-    def __init__(self):
+    def __init__(self, elsewhere=lambda: 0):
+        self._elsewhere = elsewhere  # what is counted without Python
         self.kernels = 0
         self.timing = False
         self.events: dict = {}
+
+    @property
+    def kernels(self):
+        return self._kernels + self._elsewhere()
+
+    @kernels.setter
+    def kernels(self, n):
+        self._kernels = n - self._elsewhere()
 
     def reset(self):
         self.kernels = 0
         self.events = {}
 
     def count(self, n):
-        self.kernels += n
+        self._kernels += n
 
     def timed(self, tag, fn):
         if not self.timing:
@@ -48,7 +57,7 @@ class LaunchStats:
         return {t: (len(ev), sum(a.elapsed_time(b) for a, b in ev)) for t, ev in self.events.items()}
 
 
-STATS = LaunchStats()
+STATS = LaunchStats(native.queued_by_host_ops)
 
 
 def _dt(t: torch.Tensor) -> int:
