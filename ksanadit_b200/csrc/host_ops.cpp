@@ -68,12 +68,14 @@ void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 bool watched() {
   return lib.error == nullptr || at::impl::torch_function_mode_enabled() || c10::impl::TorchDispatchModeTLS::any_modes_set() || torch::jit::tracer::isTracing();
 }
+// A forward-mode derivative goes with the tensor, whether or not it requires a gradient.
+bool has_tangent(const Tensor& t) { return t._fw_grad(0).defined(); }
 // A tensor argument, or none (undefined) where that is allowed.  False: not a plain one.
 bool take(PyObject* o, bool optional, Tensor& t) {
   if (o == Py_None) return optional;
   if (!plain_tensor(o)) return false;
   t = THPVariable_Unpack(o);
-  return true;
+  return !has_tangent(t);
 }
 // x [.., K] of a half type on the current GPU: rows a constant distance apart, on 16-byte boundaries
 bool rows(const Tensor& x, int64_t& M, int64_t& K, int64_t& ld) {
@@ -100,6 +102,7 @@ std::vector<int64_t> with_last(const Tensor& x, int64_t n) {
 // an incoming gradient as contiguous rows
 Tensor dense(const Tensor& d) {
   if (!d.defined()) return d;
+  TORCH_CHECK(!has_tangent(d), "the operators of a gated half have no forward-mode derivatives");
   Tensor c = d.contiguous();
   return aligned(c) ? c : c.clone();
 }

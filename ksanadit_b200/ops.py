@@ -10,6 +10,7 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib, native
 
@@ -651,6 +652,13 @@ def _one_device(x, *ts):
             raise _lib.KsanaB200Error(f"all tensors of a call must be on one GPU: found {t.device} beside {x.device}")
 
 
+def _no_tangents(*ts):
+    """Raises for dual tensors: a kernel sees their values alone, and a result without its tangent would count as a constant."""
+    for t in ts:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise _lib.KsanaB200Error("the operators of a gated half have no forward-mode derivatives")
+
+
 def _rows(x, K):
     """x [..., K] as rows [M, K] with adjacent elements, a constant distance apart and on 16-byte boundaries (a copy where it is not)."""
     x2 = x if x.dim() == 2 else x.reshape(-1, K)
@@ -670,6 +678,7 @@ def w4_linear(x, weight, weight_scale, weight_zero=None, bias=None, out_features
         out = host.w4_linear(x, weight, weight_scale, weight_zero, bias, out_features)
         if out is not None:  # a plain call
             return out
+    _no_tangents(x, weight_scale, bias)
     dt, K = _dt(x), x.shape[-1]
     if weight.dim() != 3 or weight.dtype != torch.uint8 or weight.shape[2] != 512 or not weight.is_contiguous():
         raise _lib.KsanaB200Error("the packed weight must be a contiguous [ceil(N/16), ceil(K/64), 512] uint8 tensor")
@@ -763,6 +772,7 @@ def _once(backward):
     @functools.wraps(backward)
     def run(ctx, *grads):
         again = torch.is_grad_enabled()
+        _no_tangents(*grads)
         native.check_captured_leaves()
         with torch.no_grad():
             out = backward(ctx, *grads)
@@ -829,13 +839,15 @@ def sandwich_norm(x, y=None, *, gate=None, scale=None, shift=None, post_weight=N
     x, y [..., C] of one half type; N: RMSNorm (``kind="rms"``) or LayerNorm (``"layer"``) over the last axis.  gate, scale, shift: half,
     [C], [1, C], or one row per leading index up to some axis ([B, 1, C], [B, C] or [B, L, C] for x [B, L, C]; any number that divides M
     for x [M, C]).  post_weight, pre_weight: fp32 [C].  All optional; without y, r is x itself; with ``pre=False``, h is None.  C % 8 == 0, at
-    most 8192.  fp32 arithmetic, one rounding per result; h is the norm of the unrounded r.  Differentiable in all tensors."""
+    most 8192.  fp32 arithmetic, one rounding per result; h is the norm of the unrounded r.  Differentiable in all tensors
+    (reverse mode only, once)."""
     host = native.host_ops()
     if host and kind in ("rms", "layer"):
         rh = host.sandwich_norm(x, y, gate, scale, shift, post_weight, pre_weight, residual_scale, pre, kind == "layer", eps)
         if rh is not None:  # a plain call
             return rh if y is not None else (x, rh[1])
     tensors = (x, y, gate, scale, shift, post_weight, pre_weight)
+    _no_tangents(*tensors)
     if kind not in ("rms", "layer"):
         raise _lib.KsanaB200Error(f"kind must be 'rms' or 'layer', got {kind!r}")
     _dt(x)
@@ -919,12 +931,14 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, act="silu"):
 
     x [..., K], w_gate and w_up [F, K], b_gate and b_up [F] or None, all of one half type -> h [..., F].  act: ``"silu"`` or ``"gelu_tanh"``.
     K and F must be multiples of 8.  fp32 sums, one rounding of h.  Differentiable in all tensors: for the backward pass the two projections are
-    kept in 24 bits each; its products take their gradients in the half type."""
+    kept in 24 bits each; its products take their gradients in the half type.  Reverse mode only, once."""
     host = native.host_ops()
     if host and act in ACTIVATIONS:
         h = host.gated_linear(x, w_gate, w_up, b_gate, b_up, ACTIVATIONS[act])
         if h is not None:  # a plain call
             return h
+    tensors = (x, w_gate, w_up, b_gate, b_up)
+    _no_tangents(*tensors)
     if act not in ACTIVATIONS:
         raise _lib.KsanaB200Error(f"act must be one of {sorted(ACTIVATIONS)}, got {act!r}")
     _dt(x)
@@ -938,7 +952,6 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, act="silu"):
     for b in (b_gate, b_up):
         if b is not None and (b.shape != (F,) or b.dtype != x.dtype or b.stride(0) != 1 or b.data_ptr() % 16 != 0):
             raise _lib.KsanaB200Error(f"biases must hold {F} adjacent values of x's type, {x.dtype}, on a 16-byte boundary")
-    tensors = (x, w_gate, w_up, b_gate, b_up)
     _one_device(*tensors)
     if _elsewhere(x.device):
         with torch.cuda.device(x.device):

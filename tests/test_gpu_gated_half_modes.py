@@ -1,0 +1,69 @@
+"""Modes of torch that the operators of a gated half cannot follow are errors of the call, and what they can follow is not refused."""
+
+import pytest
+import torch
+import torch.autograd.forward_ad as fwd
+
+from ksanadit_b200 import _lib, ops, w4
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(params=["extension", "python"], autouse=True)
+def way(request, monkeypatch):
+    """Every test both ways: plain calls through the extension, and all calls through Python."""
+    from ksanadit_b200 import native
+    if request.param == "python":
+        monkeypatch.setattr(native, "host_ops", lambda: False)
+    else:
+        assert native.host_ops()
+    return request.param
+
+
+def _n(*shape, dtype=torch.bfloat16, seed=0):
+    return torch.randn(*shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed)).to(dtype)
+
+
+def calls():
+    """name -> (function of its tensors, the tensors that a derivative could be asked of)"""
+    packed, scale, _ = w4.quantize_w4(_n(48, 64, dtype=torch.float32), 64)
+    return {
+        "gated": (lambda *t: ops.gated_linear(*t), (_n(20, 16), _n(24, 16, seed=1), _n(24, 16, seed=2), _n(24), _n(24))),
+        "norms": (lambda x, y, g, sc, sh, wp, wn: ops.sandwich_norm(x, y, gate=g, scale=sc, shift=sh, post_weight=wp, pre_weight=wn),
+                  (_n(20, 16), _n(20, 16), _n(16), _n(16), _n(16), _n(16, dtype=torch.float32), _n(16, dtype=torch.float32))),
+        "w4": (lambda x, s, b: ops.w4_linear(x, packed, s, None, b), (_n(2, 64), scale, _n(48))),
+    }
+
+
+@pytest.mark.parametrize("name", ["gated", "norms", "w4"])
+def test_forward_mode_is_refused(name):
+    f, tensors = calls()[name]
+    for i, t in enumerate(tensors):
+        with fwd.dual_level():
+            for needs in (False, True) if name != "w4" else (False,):
+                dual = fwd.make_dual(t.detach().clone().requires_grad_(needs), torch.ones_like(t))
+                with pytest.raises(_lib.KsanaB200Error, match="forward-mode"):
+                    f(*tensors[:i], dual, *tensors[i + 1:])
+            f(*tensors)  # without a dual tensor a level changes nothing
+
+
+@pytest.mark.parametrize("name", ["gated", "norms"])
+def test_forward_over_reverse_is_refused(name):
+    f, tensors = calls()[name]
+    leaves = [t.detach().clone().requires_grad_(True) for t in tensors]
+    out = f(*leaves)
+    out = out if name == "gated" else out[0]
+    with fwd.dual_level():
+        d = fwd.make_dual(torch.ones_like(out), torch.ones_like(out))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(out, leaves[:2], d)
+
+
+def test_registered_operators_refuse_forward_mode():
+    import ksanadit_b200.torch_ops  # noqa: F401
+    x, w = _n(20, 16), _n(24, 16)
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        for call in (lambda: torch.ops.ksana_b200.gated_linear(dual, w, w), lambda: torch.ops.ksana_b200.sandwich_norm(dual, x)):
+            with pytest.raises(RuntimeError):
+                call()
