@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import sys
 
 import torch
 from torch.autograd import forward_ad
@@ -659,6 +660,13 @@ def _no_tangents(*ts):
             raise _lib.KsanaB200Error("the operators of a gated half have no forward-mode derivatives")
 
 
+def _not_recorded(name):
+    """Raises while a call is recorded (``torch.jit.trace``, ``make_fx``): of a launch the record would keep the output's allocation alone."""
+    proxies = sys.modules.get("torch.fx.experimental.proxy_tensor")
+    if torch.jit.is_tracing() or (proxies is not None and proxies.get_proxy_mode() is not None):
+        raise _lib.KsanaB200Error(f"a record of this call would not hold its kernel: record torch.ops.ksana_b200.{name} (ksanadit_b200.torch_ops)")
+
+
 def _rows(x, K):
     """x [..., K] as rows [M, K] with adjacent elements, a constant distance apart and on 16-byte boundaries (a copy where it is not)."""
     x2 = x if x.dim() == 2 else x.reshape(-1, K)
@@ -678,6 +686,7 @@ def w4_linear(x, weight, weight_scale, weight_zero=None, bias=None, out_features
         out = host.w4_linear(x, weight, weight_scale, weight_zero, bias, out_features)
         if out is not None:  # a plain call
             return out
+    _not_recorded("w4_linear")
     _no_tangents(x, weight_scale, bias)
     dt, K = _dt(x), x.shape[-1]
     if weight.dim() != 3 or weight.dtype != torch.uint8 or weight.shape[2] != 512 or not weight.is_contiguous():
@@ -847,6 +856,7 @@ def sandwich_norm(x, y=None, *, gate=None, scale=None, shift=None, post_weight=N
         if rh is not None:  # a plain call
             return rh if y is not None else (x, rh[1])
     tensors = (x, y, gate, scale, shift, post_weight, pre_weight)
+    _not_recorded("sandwich_norm")
     _no_tangents(*tensors)
     if kind not in ("rms", "layer"):
         raise _lib.KsanaB200Error(f"kind must be 'rms' or 'layer', got {kind!r}")
@@ -938,6 +948,7 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, act="silu"):
         if h is not None:  # a plain call
             return h
     tensors = (x, w_gate, w_up, b_gate, b_up)
+    _not_recorded("gated_linear")
     _no_tangents(*tensors)
     if act not in ACTIVATIONS:
         raise _lib.KsanaB200Error(f"act must be one of {sorted(ACTIVATIONS)}, got {act!r}")

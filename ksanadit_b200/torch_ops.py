@@ -8,9 +8,10 @@ operators with known output shapes instead of ctypes calls it cannot trace:
     torch.ops.ksana_b200.sandwich_norm(x, y, gate, scale, shift, post_weight, pre_weight, residual_scale, kind, eps) -> (r, h) like x
     torch.ops.ksana_b200.w4_linear(x, weight, weight_scale, weight_zero, bias, out_features) -> [..., out_features] in x.dtype
 
-The real implementations are the CUDA kernels (no CPU implementation is registered: calling the operators on
-CPU tensors raises); the fake implementations only describe shapes and dtypes.  None has an autograd formula here: gradients are those of
-``ops.gated_linear`` and ``ops.sandwich_norm``, called directly.
+The real implementations are the CUDA kernels (no CPU implementation is registered: calling the operators on CPU tensors raises); the fake
+implementations only describe shapes and dtypes.  None has an autograd formula here: gradients are those of ``ops.gated_linear`` and
+``ops.sandwich_norm``, called directly.  Where ``torch.jit.trace`` or ``make_fx`` records, the last three operators have to be called in this form, and their
+namesakes in ``ops`` raise; ``sandwich_norm`` has no form here without ``y`` or without the norm behind the sum.
 """
 
 from __future__ import annotations

@@ -30,3 +30,14 @@ def test_forward_mode_is_refused(name):
             dual = fwd.make_dual(t, torch.ones_like(t))
             with pytest.raises(_lib.KsanaB200Error, match="forward-mode"):
                 f(*tensors[:i], dual, *tensors[i + 1:])
+
+
+@pytest.mark.parametrize("name", ["gated", "norms", "w4"])
+def test_recording_is_refused(name):
+    """What records a call sees its output's allocation and no kernel that fills it."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    f, tensors = calls()[name]
+    with pytest.raises(_lib.KsanaB200Error, match="torch.ops.ksana_b200"):
+        torch.jit.trace(f, tensors, check_trace=False)
+    with pytest.raises(_lib.KsanaB200Error, match="torch.ops.ksana_b200"):
+        make_fx(f)(*tensors)

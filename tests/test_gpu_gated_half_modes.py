@@ -67,3 +67,35 @@ def test_registered_operators_refuse_forward_mode():
         for call in (lambda: torch.ops.ksana_b200.gated_linear(dual, w, w), lambda: torch.ops.ksana_b200.sandwich_norm(dual, x)):
             with pytest.raises(RuntimeError):
                 call()
+
+
+@pytest.mark.parametrize("name", ["gated", "norms", "w4"])
+def test_recording_is_refused(name):
+    """What records a call sees its output's allocation and no kernel that fills it."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    f, tensors = calls()[name]
+    with torch.no_grad():
+        with pytest.raises(_lib.KsanaB200Error, match="torch.ops.ksana_b200"):
+            torch.jit.trace(f, tensors, check_trace=False)
+        with pytest.raises(_lib.KsanaB200Error, match="torch.ops.ksana_b200"):
+            make_fx(f)(*tensors)
+        f(*tensors)
+
+
+def test_registered_operators_are_recorded():
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    import ksanadit_b200.torch_ops  # noqa: F401
+    t = torch.ops.ksana_b200
+    packed, scale, _ = w4.quantize_w4(_n(48, 64, dtype=torch.float32), 64)
+    w = _n(64, 16, seed=1)
+
+    def f(x, y):
+        r, h = t.sandwich_norm(x, y, x[0], None, None, None, None, 0.5, "rms", 1e-6)
+        return r, t.w4_linear(t.gated_linear(h, w, w, None, None, "silu"), packed, scale, None, None, 48)
+
+    with torch.no_grad():
+        for recorded in (torch.jit.trace(f, (_n(20, 16), _n(20, 16, seed=2))), make_fx(f)(_n(20, 16), _n(20, 16, seed=2))):
+            x, y = _n(20, 16, seed=3), _n(20, 16, seed=4)
+            assert all(torch.equal(a, b) for a, b in zip(recorded(x, y), f(x, y)))
+            assert torch.equal(f(x, y)[0], ops.sandwich_norm(x, y, gate=x[0], residual_scale=0.5)[0])
