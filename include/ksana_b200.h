@@ -440,13 +440,18 @@ typedef struct ksb_sandwich_norm_args {
 } ksb_sandwich_norm_args;
 int ksb_sandwich_norm(const ksb_sandwich_norm_args* args, void* r, void* h, ksb_stream_t stream);
 /* Its gradients: from dr and dh (half, row strides lddr, lddh; one of them may be NULL = zeros) those asked for: dx, dy [M, C], dgate, dscale,
- * dshift [mod_rows, C] half, contiguous; dpost_w, dpre_w fp32 [C].  args: as in the forward call, stats as it wrote them.  Sums over rows
- * are fp32, in an order that depends on the shapes alone.  workspace: ksb_sandwich_norm_workspace bytes. */
+ * dshift [mod_rows, C] half, contiguous; dpost_w, dpre_w fp32 [C].  args: as in the forward call, stats as it wrote them.  one_row: which of
+ * gate, scale and shift have one row where mod_rows is above 1 (stride 0); their gradients are [C], the sum over all rows.  Sums over rows
+ * are fp32, in an order that depends on the shapes alone, rounded once.  workspace: ksb_sandwich_norm_workspace bytes. */
+#define KSB_NORM_ONE_GATE 1
+#define KSB_NORM_ONE_SCALE 2
+#define KSB_NORM_ONE_SHIFT 4
 typedef struct ksb_sandwich_norm_grads {
   const void *dr, *dh;
   void *dx, *dy, *dgate, *dscale, *dshift;
   float *dpost_w, *dpre_w;
   int64_t lddr, lddh;
+  int one_row;
 } ksb_sandwich_norm_grads;
 int64_t ksb_sandwich_norm_workspace(int64_t M, int64_t C, int64_t mod_rows);
 int ksb_sandwich_norm_backward(const ksb_sandwich_norm_args* args, const ksb_sandwich_norm_grads* grads, void* workspace, ksb_stream_t stream);

@@ -68,7 +68,12 @@ struct Grads {
   int chunk_rows;
   int chunks;      // of the rows that share a modulation row
   int samples;     // modulation rows
+  int one_row;     // KSB_NORM_ONE_*: gradients that are sums over all rows, of tensors with one row beside others that have several
 };
+// Whether a launch has sums over all rows to make, besides those over a modulation row's.
+__host__ __device__ __forceinline__ bool sums_all(const Grads& q) {
+  return q.dpost_w || q.dpre_w || ((q.one_row & KSB_NORM_ONE_GATE) && q.dgate) || ((q.one_row & KSB_NORM_ONE_SCALE) && q.dscale) || ((q.one_row & KSB_NORM_ONE_SHIFT) && q.dshift);
+}
 
 __device__ __forceinline__ uint4 load8(const void* base, int64_t offset_bytes) { return *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(base) + offset_bytes); }
 
@@ -407,7 +412,8 @@ struct Sums {
 };
 
 // NC chunks per thread.  WHOLE: a group takes all rows of some modulation rows, and writes the modulation's gradients itself; else a CTA takes
-// a stretch of the rows of one and leaves its sums to finish_kernel.
+// a stretch of the rows of one and leaves its sums to finish_kernel.  ONE (WHOLE): some of gate, scale and shift have one row for all (a form of its
+// own, since the other one lost 1 - 2 % to the questions: 32760 x 1 x 5120 1050 and 1063 us, layer norm 20000 x 1 x 8192 1784 and 1814).
 //
 // With w = dr + rstd_r t and z = A yh, D = w - a1 rh - a0 is linear in its row's a1 = rstd_r mean(t rh) and a0 = rstd_r mean(t), and so are the sums
 // that dy takes: sum(e yh) = sum(w z) - a1 sum(rh z) - a0 sum(z), sum(e) = sum(w A) - a1 sum(rh A) - a0 sum(A).  So a row has one exchange, of
@@ -415,7 +421,7 @@ struct Sums {
 //
 // Up to 5120 columns a thread has one chunk and up to twenty warps share a row: eight warps of three chunks, which leaves the exchanges less to do
 // but the schedulers two warps each, took 1040 us for 75600 x 5120, twelve of two 1058, twenty of one 903.
-template <typename T, int NC, bool LAYER, bool WHOLE>
+template <typename T, int NC, bool LAYER, bool WHOLE, bool ONE>
 __global__ void __launch_bounds__(backward_threads<NC>, 1) backward_kernel(const __grid_constant__ Params p, const __grid_constant__ Grads q) {
   extern __shared__ __align__(16) uint8_t ring_bytes[];  // [DEPTH][x, y, dr, dh][NC][threads] 16 bytes and the factors; in the end the groups' sums
   __shared__ __align__(16) float red[RED_FLOATS];
@@ -498,7 +504,9 @@ __global__ void __launch_bounds__(backward_threads<NC>, 1) backward_kernel(const
     put_factor(0, c, fill8(0.f));
     put_factor(1, c, fill8(0.f));
   }
-  // WHOLE: a modulation row's gradients, and its part of the weights'
+  // WHOLE: a modulation row's gradients, and its part of the weights'.  What a tensor with one row takes (acc.p: the gate and the weight
+  // behind it, acc.q: the scale and the weight ahead, acc.s: the shift) runs on instead, through all rows.
+  const bool one_gate = ONE && q.one_row & KSB_NORM_ONE_GATE, one_scale = ONE && q.one_row & KSB_NORM_ONE_SCALE, one_shift = ONE && q.one_row & KSB_NORM_ONE_SHIFT;
   auto flush = [&]() {
     const F2 a = both(p.a);
 #pragma unroll
@@ -507,7 +515,7 @@ __global__ void __launch_bounds__(backward_threads<NC>, 1) backward_kernel(const
         const int ch = t + c * nt;
         V8 f, o;
         auto out = [&](void* to) { *reinterpret_cast<uint4*>(static_cast<T*>(to) + static_cast<int64_t>(mod) * p.C + ch * 8) = pack8<T>(o); };
-        if (p.y) {
+        if (p.y && !one_gate) {
           if (q.dpost_w) {
             f = p.gate ? unpack8<T>(load8(p.gate, (mod * p.gate_stride + ch * 8) * 2)) : fill8(1.f);
 #pragma unroll
@@ -521,24 +529,26 @@ __global__ void __launch_bounds__(backward_threads<NC>, 1) backward_kernel(const
           }
         }
         if (q.dh) {
-          if (q.dpre_w) {
+          if (q.dpre_w && !one_scale) {
             f = p.scale ? unpack8<T>(load8(p.scale, (mod * p.scale_stride + ch * 8) * 2)) : fill8(0.f);
 #pragma unroll
             for (int i = 0; i < 4; ++i) wn[c][i] = fma2(add(both(1.f), f[i]), acc[c].q[i], wn[c][i]);
           }
-          if (q.dscale) {
+          if (q.dscale && !one_scale) {
             f = weight8(p.pre_w, ch);
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[i] = mul(f[i], acc[c].q[i]);
             out(q.dscale);
           }
-          if (q.dshift) {
+          if (q.dshift && !one_shift) {
             o = acc[c].s;
             out(q.dshift);
           }
         }
       }
-      acc[c].p = acc[c].q = acc[c].s = fill8(0.f);
+      if (!one_gate) acc[c].p = fill8(0.f);
+      if (!one_scale) acc[c].q = fill8(0.f);
+      if (!one_shift) acc[c].s = fill8(0.f);
     }
   };
   int slot = 0;
@@ -654,8 +664,8 @@ __global__ void __launch_bounds__(backward_threads<NC>, 1) backward_kernel(const
   copies_wait<0>();
 
   // What is left to the second kernel: the groups' sums, added up in the order of the groups where there are several.
-  constexpr int KINDS = WHOLE ? 2 : 3;
-  if (WHOLE && !q.dpost_w && !q.dpre_w) return;
+  constexpr int KINDS = WHOLE && !ONE ? 2 : 3;
+  if (WHOLE && !sums_all(q)) return;
   float* to = q.parts + static_cast<int64_t>(blockIdx.x) * KINDS * p.C;
   float* sums = blockDim.y == 1 ? to : reinterpret_cast<float*>(ring_bytes);
   for (int y = 0; y < (int)blockDim.y; ++y) {
@@ -666,7 +676,7 @@ __global__ void __launch_bounds__(backward_threads<NC>, 1) backward_kernel(const
       if (live[c]) {
 #pragma unroll
         for (int k = 0; k < KINDS; ++k) {
-          const V8& v = WHOLE ? (k == 0 ? wp[c] : wn[c]) : (k == 0 ? acc[c].p : k == 1 ? acc[c].q : acc[c].s);
+          const V8& v = WHOLE && !ONE ? (k == 0 ? wp[c] : wn[c]) : k == 0 ? (!WHOLE || one_gate ? acc[c].p : wp[c]) : k == 1 ? (!WHOLE || one_scale ? acc[c].q : wn[c]) : acc[c].s;
           F2* at = reinterpret_cast<F2*>(sums + k * p.C + (t + c * nt) * 8);
 #pragma unroll
           for (int i = 0; i < 4; ++i) at[i] = y == 0 ? v[i] : add(at[i], v[i]);
@@ -683,24 +693,28 @@ __global__ void __launch_bounds__(backward_threads<NC>, 1) backward_kernel(const
 // modulation rows have CTAs of their own (backward pass of 3 x 777 x 2056 25.0 and 22.4 us, of 8 x 777 x 2048 51.4 and 42.9).
 constexpr int FINISH = 16;
 template <typename T> __global__ void __launch_bounds__(32 * FINISH) finish_kernel(const __grid_constant__ Params p, const __grid_constant__ Grads q) {
-  __shared__ float part[3][FINISH][33];
+  __shared__ float part[5][FINISH][33];
   const int lane = threadIdx.x, j = threadIdx.y, col = blockIdx.x * 32 + lane;
   const bool live = col < p.C;
   pdl_wait();
   pdl_release();
   const bool by_sample = q.samples >= FINISH;
   const float wp = p.post_w && live ? p.post_w[col] : 1.f, wn = p.pre_w && live ? p.pre_w[col] : 1.f;
-  float dwp = 0.f, dwn = 0.f;
+  const bool one_gate = q.one_row & KSB_NORM_ONE_GATE, one_scale = q.one_row & KSB_NORM_ONE_SCALE, one_shift = q.one_row & KSB_NORM_ONE_SHIFT;
+  float all[5] = {0.f, 0.f, 0.f, 0.f, 0.f};  // over all rows: of the two weights', and of gate, scale and shift where they have one row
   auto write = [&](int b, float sp, float sq, float ss) {
     if (!live) return;
     const float gate = p.gate ? HalfOps<T>::to_f(static_cast<const T*>(p.gate)[b * p.gate_stride + col]) : 1.f;
     const float scale = p.scale ? HalfOps<T>::to_f(static_cast<const T*>(p.scale)[b * p.scale_stride + col]) : 0.f;
     const int64_t at = static_cast<int64_t>(b) * p.C + col;
-    if (q.dgate) static_cast<T*>(q.dgate)[at] = HalfOps<T>::from_f(p.a * wp * sp);
-    if (q.dscale) static_cast<T*>(q.dscale)[at] = HalfOps<T>::from_f(wn * sq);
-    if (q.dshift) static_cast<T*>(q.dshift)[at] = HalfOps<T>::from_f(ss);
-    dwp = fmaf(p.a * gate, sp, dwp);
-    dwn = fmaf(1.f + scale, sq, dwn);
+    if (q.dgate && !one_gate) static_cast<T*>(q.dgate)[at] = HalfOps<T>::from_f(p.a * wp * sp);
+    if (q.dscale && !one_scale) static_cast<T*>(q.dscale)[at] = HalfOps<T>::from_f(wn * sq);
+    if (q.dshift && !one_shift) static_cast<T*>(q.dshift)[at] = HalfOps<T>::from_f(ss);
+    all[0] = fmaf(p.a * gate, sp, all[0]);
+    all[1] = fmaf(1.f + scale, sq, all[1]);
+    all[2] += sp;
+    all[3] += sq;
+    all[4] += ss;
   };
   auto sums = [&](int b, int first, int step, float (&s)[3]) {
     const float* from = q.parts + (static_cast<int64_t>(b) * q.chunks + first) * 3 * p.C + col;
@@ -719,15 +733,15 @@ template <typename T> __global__ void __launch_bounds__(32 * FINISH) finish_kern
       sums(b, 0, 1, s);
       write(b, s[0], s[1], s[2]);
     }
-    part[0][j][lane] = dwp;
-    part[1][j][lane] = dwn;
+#pragma unroll
+    for (int i = 0; i < 5; ++i) part[i][j][lane] = all[i];
     __syncthreads();
     if (j != 0 || !live) return;
-    dwp = dwn = 0.f;
-    for (int k = 0; k < FINISH; ++k) {
-      dwp += part[0][k][lane];
-      dwn += part[1][k][lane];
-    }
+#pragma unroll
+    for (int i = 0; i < 5; ++i) all[i] = 0.f;
+    for (int k = 0; k < FINISH; ++k)
+#pragma unroll
+      for (int i = 0; i < 5; ++i) all[i] += part[i][k][lane];
   } else {
     for (int b = blockIdx.y; b < q.samples; b += gridDim.y) {
       sums(b, j, FINISH, s);
@@ -745,34 +759,51 @@ template <typename T> __global__ void __launch_bounds__(32 * FINISH) finish_kern
     }
     if (j != 0 || !live) return;
   }
-  if (q.dpost_w) q.dpost_w[col] = dwp;
-  if (q.dpre_w) q.dpre_w[col] = dwn;
+  if (q.dpost_w) q.dpost_w[col] = all[0];
+  if (q.dpre_w) q.dpre_w[col] = all[1];
+  if (q.dgate && one_gate) static_cast<T*>(q.dgate)[col] = HalfOps<T>::from_f(p.a * wp * all[2]);
+  if (q.dscale && one_scale) static_cast<T*>(q.dscale)[col] = HalfOps<T>::from_f(wn * all[3]);
+  if (q.dshift && one_shift) static_cast<T*>(q.dshift)[col] = HalfOps<T>::from_f(all[4]);
 }
 
-// The weights' gradients from the CTAs' sums of a WHOLE launch.
-__global__ void __launch_bounds__(32 * FINISH) finish_weights_kernel(const __grid_constant__ Params p, const __grid_constant__ Grads q, int count) {
-  __shared__ float part[2][FINISH][33];
+// What is summed over all rows, from the CTAs' sums of a WHOLE launch (ONE: as there, a third sum among them).
+template <typename T, bool ONE> __global__ void __launch_bounds__(32 * FINISH) finish_all_kernel(const __grid_constant__ Params p, const __grid_constant__ Grads q, int count) {
+  constexpr int KINDS = ONE ? 3 : 2;
+  __shared__ float part[KINDS][FINISH][33];
   const int lane = threadIdx.x, j = threadIdx.y, col = blockIdx.x * 32 + lane;
   pdl_wait();
   pdl_release();
-  float a = 0.f, b = 0.f;
+  float v[KINDS];
+#pragma unroll
+  for (int k = 0; k < KINDS; ++k) v[k] = 0.f;
   if (col < p.C)
 #pragma unroll 4
     for (int c = j; c < count; c += FINISH) {
-      a += q.parts[static_cast<int64_t>(c) * 2 * p.C + col];
-      b += q.parts[static_cast<int64_t>(c) * 2 * p.C + p.C + col];
+      const float* from = q.parts + static_cast<int64_t>(c) * KINDS * p.C + col;
+      v[0] += from[0];
+      v[1] += from[p.C];
+      if (ONE) v[KINDS - 1] += from[2 * p.C];
     }
-  part[0][j][lane] = a;
-  part[1][j][lane] = b;
+#pragma unroll
+  for (int k = 0; k < KINDS; ++k) part[k][j][lane] = v[k];
   __syncthreads();
   if (j != 0 || col >= p.C) return;
-  a = b = 0.f;
-  for (int k = 0; k < FINISH; ++k) {
-    a += part[0][k][lane];
-    b += part[1][k][lane];
+#pragma unroll
+  for (int k = 0; k < KINDS; ++k) v[k] = 0.f;
+#pragma unroll
+  for (int i = 0; i < FINISH; ++i)
+#pragma unroll
+    for (int k = 0; k < KINDS; ++k) v[k] += part[k][i][lane];
+  if constexpr (ONE) {  // a gate or scale with one row has waited until here: see flush
+    const bool one_gate = q.one_row & KSB_NORM_ONE_GATE, one_scale = q.one_row & KSB_NORM_ONE_SCALE, one_shift = q.one_row & KSB_NORM_ONE_SHIFT;
+    if (q.dgate && one_gate) static_cast<T*>(q.dgate)[col] = HalfOps<T>::from_f(p.a * (p.post_w ? p.post_w[col] : 1.f) * v[0]);
+    if (q.dscale && one_scale) static_cast<T*>(q.dscale)[col] = HalfOps<T>::from_f((p.pre_w ? p.pre_w[col] : 1.f) * v[1]);
+    if (q.dshift && one_shift) static_cast<T*>(q.dshift)[col] = HalfOps<T>::from_f(v[KINDS - 1]);
+    if (one_gate) v[0] *= p.a * HalfOps<T>::to_f(static_cast<const T*>(p.gate)[col]);
+    if (one_scale) v[1] *= 1.f + HalfOps<T>::to_f(static_cast<const T*>(p.scale)[col]);
   }
-  if (q.dpost_w) q.dpost_w[col] = a;
-  if (q.dpre_w) q.dpre_w[col] = b;
+  if (q.dpost_w) q.dpost_w[col] = v[0];
+  if (q.dpre_w) q.dpre_w[col] = v[1];
 }
 
 // How the backward pass shares out the rows: a CTA per SM, of as many groups as its threads hold.
@@ -780,7 +811,7 @@ struct Plan {
   int each, threads, groups, ctas, chunks;  // each: chunks per thread
   int64_t chunk_rows;
   bool whole;
-  int64_t floats(int C) const { return static_cast<int64_t>(ctas) * (whole ? 2 : 3) * C; }
+  int64_t floats(int C) const { return static_cast<int64_t>(ctas) * 3 * C; }
 };
 static Plan plan_backward(int64_t M, int64_t C, int64_t rows_per_mod) {
   Plan s{};
@@ -826,29 +857,30 @@ template <typename T, bool LAYER> static int forward(const Params& p, cudaStream
   return forward_as<T, 2, LAYER, 512, 1>(p, threads, 1, st);
 }
 
-template <typename T, int NC, bool LAYER, bool WHOLE> static int backward_as(const Params& p, const Grads& q, const Plan& s, cudaStream_t st) {
-  auto kernel = backward_kernel<T, NC, LAYER, WHOLE>;
+template <typename T, int NC, bool LAYER, bool WHOLE, bool ONE> static int backward_as(const Params& p, const Grads& q, const Plan& s, cudaStream_t st) {
+  auto kernel = backward_kernel<T, NC, LAYER, WHOLE, ONE>;
   constexpr int bytes = (backward_depth<NC, LAYER> + 1) * 64 * NC;  // a thread: the ring, and the factors
   static DeviceOnce limit;
   if (int rc = limit.raise_smem(reinterpret_cast<const void*>(kernel), bytes * backward_threads<NC>)) return rc;
   return launch_kernel("sandwich norm gradient", reinterpret_cast<const void*>(kernel), dim3((unsigned)s.ctas), dim3(s.threads, s.groups), bytes * s.threads * s.groups, st, 1, true, p, q);
 }
-template <typename T, bool LAYER, bool WHOLE> static int backward_of(const Params& p, const Grads& q, const Plan& s, cudaStream_t st) {
-  return s.each == 1 ? backward_as<T, 1, LAYER, WHOLE>(p, q, s, st) : backward_as<T, 4, LAYER, WHOLE>(p, q, s, st);
+template <typename T, bool LAYER, bool WHOLE, bool ONE> static int backward_of(const Params& p, const Grads& q, const Plan& s, cudaStream_t st) {
+  return s.each == 1 ? backward_as<T, 1, LAYER, WHOLE, ONE>(p, q, s, st) : backward_as<T, 4, LAYER, WHOLE, ONE>(p, q, s, st);
+}
+template <typename T, bool LAYER> static int backward_form(const Params& p, const Grads& q, const Plan& s, cudaStream_t st) {
+  if (!s.whole) return backward_of<T, LAYER, false, false>(p, q, s, st);
+  return q.one_row ? backward_of<T, LAYER, true, true>(p, q, s, st) : backward_of<T, LAYER, true, false>(p, q, s, st);
 }
 template <typename T> static int backward(const Params& p, const Grads& q, const Plan& s, bool layer, cudaStream_t st) {
-  int rc;
-  if (layer) rc = s.whole ? backward_of<T, true, true>(p, q, s, st) : backward_of<T, true, false>(p, q, s, st);
-  else rc = s.whole ? backward_of<T, false, true>(p, q, s, st) : backward_of<T, false, false>(p, q, s, st);
-  if (rc) return rc;
+  if (int rc = layer ? backward_form<T, true>(p, q, s, st) : backward_form<T, false>(p, q, s, st)) return rc;
   const dim3 grid((unsigned)((p.C + 31) / 32)), block(32, FINISH);
   if (!s.whole) {
     if (!q.dgate && !q.dscale && !q.dshift && !q.dpost_w && !q.dpre_w) return 0;
-    const unsigned apart = q.dpost_w || q.dpre_w ? 1 : q.samples < FINISH ? q.samples : (q.samples + FINISH - 1) / FINISH;
+    const unsigned apart = sums_all(q) ? 1 : q.samples < FINISH ? q.samples : (q.samples + FINISH - 1) / FINISH;
     return launch_kernel("sandwich norm sums", reinterpret_cast<const void*>(finish_kernel<T>), dim3(grid.x, apart), block, 0, st, 1, true, p, q);
   }
-  if (!q.dpost_w && !q.dpre_w) return 0;
-  return launch_kernel("sandwich norm sums", reinterpret_cast<const void*>(finish_weights_kernel), grid, block, 0, st, 1, true, p, q, s.ctas);
+  if (!sums_all(q)) return 0;
+  return launch_kernel("sandwich norm sums", q.one_row ? reinterpret_cast<const void*>(finish_all_kernel<T, true>) : reinterpret_cast<const void*>(finish_all_kernel<T, false>), grid, block, 0, st, 1, true, p, q, s.ctas);
 }
 
 static int check(const Params& p, int dtype, int64_t C, int64_t mod_rows) {
@@ -904,12 +936,19 @@ extern "C" int ksb_sandwich_norm_backward(const ksb_sandwich_norm_args* a, const
   norms::Params p{};
   if (int rc = norm_params(p, a)) return rc;
   if (!g) return fail(KSB_ERR_INVALID, "null pointer");
+  // one row of a tensor is all of its rows: what a call with a single modulation row does anyway
+  const int one_row = a->mod_rows > 1 ? g->one_row : 0;
+  if ((g->one_row & ~(KSB_NORM_ONE_GATE | KSB_NORM_ONE_SCALE | KSB_NORM_ONE_SHIFT)) != 0 || ((one_row & KSB_NORM_ONE_GATE) && (!p.gate || p.gate_stride != 0)) ||
+      ((one_row & KSB_NORM_ONE_SCALE) && (!p.scale || p.scale_stride != 0)) || ((one_row & KSB_NORM_ONE_SHIFT) && (!p.shift || p.shift_stride != 0)))
+    return fail(KSB_ERR_INVALID, "one_row names a tensor that is not there or has several rows");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (p.M == 0) {  // sums over no rows
     if ((g->dpost_w && cudaMemsetAsync(g->dpost_w, 0, p.C * 4, st) != cudaSuccess) || (g->dpre_w && cudaMemsetAsync(g->dpre_w, 0, p.C * 4, st) != cudaSuccess))
       return fail(KSB_ERR_CUDA, "cannot clear the sums");
-    for (void* m : {g->dgate, g->dscale, g->dshift})
-      if (m && cudaMemsetAsync(m, 0, (size_t)a->mod_rows * p.C * 2, st) != cudaSuccess) return fail(KSB_ERR_CUDA, "cannot clear the sums");
+    void* const mods[3] = {g->dgate, g->dscale, g->dshift};
+    for (int i = 0; i < 3; ++i)
+      if (mods[i] && cudaMemsetAsync(mods[i], 0, (size_t)(one_row >> i & 1 ? 1 : a->mod_rows) * p.C * 2, st) != cudaSuccess)
+        return fail(KSB_ERR_CUDA, "cannot clear the sums");
     return 0;
   }
   norms::Grads q{};
@@ -926,6 +965,7 @@ extern "C" int ksb_sandwich_norm_backward(const ksb_sandwich_norm_args* a, const
   q.chunk_rows = (int)s.chunk_rows;
   q.chunks = s.chunks;
   q.samples = (int)a->mod_rows;
+  q.one_row = one_row;
   const int before = launch_count();
   if (int rc = a->dtype == KSB_BF16 ? norms::backward<__nv_bfloat16>(p, q, s, a->layer != 0, st) : norms::backward<__half>(p, q, s, a->layer != 0, st)) return rc;
   return launch_count() - before;

@@ -382,19 +382,16 @@ struct SandwichNorm : torch::autograd::Function<SandwichNorm> {
       if (!(need >> i & 1) || !there) continue;
       if (i == POST || i == PRE) out[i] = at::empty({c.a.C}, x.options().dtype(at::kFloat));
       else if (i < GATE) out[i] = at::empty(x.sizes(), x.options());
-      else out[i] = t[i].numel() == c.a.mod_rows * c.a.C ? at::empty(t[i].sizes(), x.options()) : at::empty({c.a.mod_rows, c.a.C}, x.options());
+      else out[i] = at::empty(t[i].sizes(), x.options());
     }
     ksb_sandwich_norm_grads g{};
+    for (int i = GATE; i <= SHIFT; ++i)  // one row for rows that others of the call tell apart
+      if (t[i].defined() && c.a.mod_rows > 1 && t[i].numel() == c.a.C) g.one_row |= 1 << (i - GATE);
     g.dr = ptr(dr); g.dh = ptr(dh); g.lddr = g.lddh = c.a.C;
     g.dx = ptr(out[X]); g.dy = ptr(out[Y]); g.dgate = ptr(out[GATE]); g.dscale = ptr(out[SCALE]); g.dshift = ptr(out[SHIFT]);
     g.dpost_w = static_cast<float*>(ptr(out[POST])); g.dpre_w = static_cast<float*>(ptr(out[PRE]));
     const Tensor ws = bytes(lib.norm_workspace(c.a.M, c.a.C, c.a.mod_rows), x);
     count(lib.norm_backward(&c.a, &g, ws.data_ptr(), stream_of(x)), "ksb_sandwich_norm_backward");
-    for (int i = GATE; i <= SHIFT; ++i) {
-      if (!out[i].defined() || out[i].numel() == t[i].numel()) continue;
-      // a tensor with one row for rows that others of the call tell apart
-      out[i] = out[i].to(at::kFloat).sum(0).to(x.scalar_type()).view(t[i].sizes());
-    }
     return last_derivatives(std::move(out), again);
   }
 };

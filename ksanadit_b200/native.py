@@ -262,7 +262,8 @@ class NormArgs(ctypes.Structure):
 
 
 class NormGrads(ctypes.Structure):
-    _fields_ = [(n, c_void_p) for n in ("dr", "dh", "dx", "dy", "dgate", "dscale", "dshift", "dpost_w", "dpre_w")] + [("lddr", c_int64), ("lddh", c_int64)]
+    _fields_ = [(n, c_void_p) for n in ("dr", "dh", "dx", "dy", "dgate", "dscale", "dshift", "dpost_w", "dpre_w")] + \
+        [("lddr", c_int64), ("lddh", c_int64), ("one_row", c_int)]
 
 
 class GatedGrads(ctypes.Structure):

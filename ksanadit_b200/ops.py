@@ -818,24 +818,20 @@ class _SandwichNorm(torch.autograd.Function):
             dy = torch.empty(y.shape, dtype=x.dtype, device=device) if y is not None and need[1] else None
             # without dh, what belongs to the norm behind the sum has no gradient
             there = (y is not None, dh is not None, dh is not None)
-            dmods = [torch.empty(mod_rows, C, dtype=x.dtype, device=device) if n and t is not None and ok else None
-                     for n, t, ok in zip(need[2:5], (gate, scale, shift), there)]
+            one_row = [t is not None and t.numel() == C and mod_rows > 1 for t in (gate, scale, shift)]  # one row for rows that others of the call tell apart
+            dmods = [torch.empty(1 if one else mod_rows, C, dtype=x.dtype, device=device) if n and t is not None and ok else None
+                     for n, t, ok, one in zip(need[2:5], (gate, scale, shift), there, one_row)]
             dpost, dpre = (torch.empty(C, dtype=torch.float32, device=device) if n and w is not None and ok else None
                            for n, w, ok in zip(need[5:7], (post_weight, pre_weight), there))
             lib = _lib.load()
             args = native.NormArgs(x2.data_ptr(), _p(y2), mods[0][0], mods[1][0], mods[2][0], _p(post_weight), _p(pre_weight), stats.data_ptr(), M, C, mod_rows,
                                    x2.stride(0), 0 if y2 is None else y2.stride(0), mods[0][1], mods[1][1], mods[2][1], _dt(x), int(layer), eps, residual_scale)
             grads = native.NormGrads(_p(dr2), _p(dh2), _p(dx), _p(dy), _p(dmods[0]), _p(dmods[1]), _p(dmods[2]), _p(dpost), _p(dpre),
-                                     0 if dr2 is None else dr2.stride(0), 0 if dh2 is None else dh2.stride(0))
+                                     0 if dr2 is None else dr2.stride(0), 0 if dh2 is None else dh2.stride(0), sum(one << i for i, one in enumerate(one_row)))
             ws = native.workspace(lib.ksb_sandwich_norm_workspace(M, C, mod_rows), device)
             STATS.count(native.queued(lib.ksb_sandwich_norm_backward(ctypes.addressof(args), ctypes.addressof(grads), ws.data_ptr(), _stream()),
                                       "ksb_sandwich_norm_backward"))
-            # a tensor with one row for rows that others of the call tell apart
-            out = []
-            for d, t in zip(dmods, (gate, scale, shift)):
-                if d is not None and d.numel() != t.numel():
-                    d = d.float().sum(0).to(t.dtype) if t.numel() else torch.empty_like(t)
-                out.append(None if d is None else d.view(t.shape))
+            out = [None if d is None else d.view(t.shape) if t.numel() else torch.empty_like(t) for d, t in zip(dmods, (gate, scale, shift))]
         return (dx, dy, *out, dpost, dpre, None, None, None, None, None)
 
 
