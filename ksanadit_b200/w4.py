@@ -54,25 +54,42 @@ def untile_groups(v: torch.Tensor, N: int) -> torch.Tensor:
     return v.transpose(1, 2).reshape(-1, v.shape[1])[:N].contiguous()
 
 
+def _scales(span: torch.Tensor, levels: int, dtype) -> torch.Tensor:
+    """span / levels per group in ``dtype``: a group of zeros takes the least normal number, any would do.
+
+    Below the normal numbers a step of the type is a large part of the scale.  One that was rounded down so far that its levels no longer reach
+    the group's ends is taken a step up: a value is then never more than half a level off."""
+    f = torch.finfo(dtype)
+    least = f.smallest_normal * f.eps
+    scale = (span / levels).to(dtype)
+    if not bool(scale.isfinite().all()):
+        raise _lib.KsanaB200Error(f"a group's scale is not finite in {dtype}: its weights are too large, or not finite themselves")
+    # a group that the least scale cannot tell from zeros: that is nothing beside weights 4096 times as large, and else the weight is lost
+    lost = (scale == 0) & (span > span.amax() / 4096) if span.numel() else scale != scale
+    if bool(lost.any()):
+        raise _lib.KsanaB200Error(f"the weights are too small for scales of {dtype}: use bfloat16 ones")
+    scale = torch.where(scale.float() * (levels + 0.5) < span, (scale.float() + least).to(dtype), scale)
+    return torch.where(span == 0, torch.full_like(scale, f.smallest_normal), scale)
+
+
 def quantize_w4(w: torch.Tensor, group: int = 128, zeros: bool = False, dtype=torch.bfloat16):
     """Rounds a weight [N, K] to 4 bits per group of ``group`` columns -> (packed, scale, zero or None) as ``ops.w4_linear`` takes them.
 
     Without zero points a group's values are scale * (-7 .. 7), scale = absmax / 7; with them they reach from the group's least
     value (or 0) to its largest (or 0) in 15 steps.  The scale is rounded to ``dtype`` first and the values against the
-    rounded one."""
+    rounded one.  Raises where ``dtype`` has no scale for the weights: fp16 ones reach down to values of some 1e-7."""
     if w.dim() != 2 or group not in GROUPS or w.shape[1] % group != 0:
         raise _lib.KsanaB200Error(f"quantize_w4 needs a [N, K] weight whose K is in whole groups of {GROUPS}, got {tuple(w.shape)} and {group}")
     if dtype not in (torch.bfloat16, torch.float16):
         raise TypeError(f"expected bfloat16 or float16 scales, got {dtype}")
     N, K = w.shape
     wf = w.float().view(N, K // group, group)
-    tiny = float(torch.finfo(dtype).tiny)  # all zeros: any scale will do
     if zeros:
         low, high = wf.amin(-1).clamp(max=0), wf.amax(-1).clamp(min=0)
-        scale = ((high - low) / 15).clamp(min=tiny).to(dtype)
+        scale = _scales(high - low, 15, dtype)
         zero = torch.round(-low / scale.float()).clamp(0, 15)
     else:
-        scale = (wf.abs().amax(-1) / 7).clamp(min=tiny).to(dtype)
+        scale = _scales(wf.abs().amax(-1), 7, dtype)
         zero = torch.full_like(scale, 8, dtype=torch.float32)
     q = torch.round(wf / scale.float()[..., None] + zero[..., None]).clamp(0, 15).to(torch.uint8).view(N, K)
     return pack_w4(q), tile_groups(scale), tile_groups(zero.to(torch.uint8)) if zeros else None
