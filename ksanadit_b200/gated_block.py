@@ -7,8 +7,8 @@
 
 KsanaDiT's own blocks (ksana/models/wan/wan_model.py:317-321, ksana/models/qwen/transformer.py:225-234) have a plain GELU
 feed-forward and no norm behind a half; models of this form run there as eager torch.  In a stack of halves the norm behind one and the
-norm ahead of the next are one pass over the tokens.  Everything but the 4-bit modulation is differentiable, so the same module is fine-tuned
-and served; for serving, ``down`` may be a ``B200Fp8Linear``.
+norm ahead of the next are one pass over the tokens.  Everything but the 4-bit modulation is differentiable (an embedding that needs a
+gradient through it is refused), so the same module is fine-tuned and served; for serving, ``down`` may be a ``B200Fp8Linear``.
 """
 
 from __future__ import annotations
@@ -39,11 +39,11 @@ class B200GatedFeedForward(torch.nn.Module):
         self.modulation = B200W4Linear(dim, 3 * dim, True, group, device=device, dtype=dtype) if modulation else None
 
     def vectors(self, temb):
-        """(shift, scale, gate), [B, 1, dim] each, of the timestep embedding [B, dim].  No gradients: the weights are frozen."""
+        """(shift, scale, gate), [B, 1, dim] each, of the timestep embedding [B, dim].  The 4-bit weights are frozen, and their product
+        has no backward pass: an embedding that needs a gradient is refused (detach it where the gradient through the modulation is not wanted)."""
         if self.modulation is None:
             raise _lib.KsanaB200Error("this half has no modulation of its own: pass its vectors")
-        with torch.no_grad():
-            return self.modulation(torch.nn.functional.silu(temb))[:, None].chunk(3, -1)
+        return self.modulation(torch.nn.functional.silu(temb))[:, None].chunk(3, -1)
 
     def inner(self, h):
         """The half between its norms."""
