@@ -888,7 +888,8 @@ static int check(const Params& p, int dtype, int64_t C, int64_t mod_rows) {
   if (C <= 0 || C % 8 != 0) return fail(KSB_ERR_INVALID, "bad shape M=%d C=%lld (C %% 8 == 0)", p.M, (long long)C);
   if (C > KSB_NORM_MAX_C) return fail(KSB_ERR_UNSUPPORTED, "C=%lld is above %d", (long long)C, KSB_NORM_MAX_C);
   if (mod_rows < 1 || (p.M > 0 && p.M % mod_rows != 0)) return fail(KSB_ERR_INVALID, "mod_rows must divide M");
-  const bool strides = (p.M <= 1 || (p.ldx >= C && (!p.y || p.ldy >= C))) && p.ldx % 8 == 0 && p.ldy % 8 == 0 && p.gate_stride % 8 == 0 && p.scale_stride % 8 == 0 && p.shift_stride % 8 == 0;
+  // the distance between rows of a tensor that has one row, or none, is nobody's
+  const bool strides = (p.M <= 1 || (p.ldx >= C && (!p.y || p.ldy >= C) && p.ldx % 8 == 0 && p.ldy % 8 == 0)) && p.gate_stride % 8 == 0 && p.scale_stride % 8 == 0 && p.shift_stride % 8 == 0;
   const bool aligned = aligned16(p.x) && aligned16(p.y) && aligned16(p.gate) && aligned16(p.scale) && aligned16(p.shift) && aligned16(p.post_w) && aligned16(p.pre_w) && aligned16(p.stats);
   if (!strides || !aligned) return fail(KSB_ERR_INVALID, "tensors must be 16-byte aligned, their rows multiples of 8 elements apart");
   if (p.M > 0 && !p.y && (p.gate || p.post_w)) return fail(KSB_ERR_INVALID, "gate and post_w belong to y");
@@ -958,7 +959,7 @@ extern "C" int ksb_sandwich_norm_backward(const ksb_sandwich_norm_args* a, const
   if (!p.x || !p.stats || !workspace || (!q.dr && !q.dh)) return fail(KSB_ERR_INVALID, "null pointer");
   for (const void* t : {q.dr, q.dh, (const void*)q.dx, (const void*)q.dy, (const void*)q.dgate, (const void*)q.dscale, (const void*)q.dshift, (const void*)workspace})
     if (!aligned16(t)) return fail(KSB_ERR_INVALID, "unaligned pointer");
-  if (q.lddr % 8 != 0 || q.lddh % 8 != 0 || (p.M > 1 && ((q.dr && q.lddr < p.C) || (q.dh && q.lddh < p.C)))) return fail(KSB_ERR_INVALID, "rows of dr and dh must be multiples of 8 elements apart");
+  if (p.M > 1 && (q.lddr % 8 != 0 || q.lddh % 8 != 0 || (q.dr && q.lddr < p.C) || (q.dh && q.lddh < p.C))) return fail(KSB_ERR_INVALID, "rows of dr and dh must be multiples of 8 elements apart");
   if (!p.y && (q.dy || q.dgate || q.dpost_w)) return fail(KSB_ERR_INVALID, "dy, dgate and dpost_w belong to y");
   if (!q.dh && (q.dscale || q.dshift || q.dpre_w)) return fail(KSB_ERR_INVALID, "dscale, dshift and dpre_w belong to dh");
   const norms::Plan s = norms::plan_backward(p.M, p.C, p.rows_per_mod);
