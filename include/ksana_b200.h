@@ -412,7 +412,8 @@ int ksb_qwen_block_forward(const ksb_qwen_block* block, const ksb_qwen_call* cal
  * the weight's way from memory.
  *   out[m, n] = sum_g scale[n, g] * (sum_{k in g} (q[n, k] - zero[n, g]) * x[m, k]) + bias[n],  groups of 32, 64 or 128 columns
  * x: [M, K] half (row stride ldx); out: [M, N] half (row stride ldo); bias: half [N] or NULL; K in whole groups, at most KSB_W4_MAX_K;
- * sums of a group and over groups in fp32, one rounding at the end.  Up to 16 rows share one pass over the weight.
+ * sums of a group and over groups in fp32, one rounding at the end, in an order that depends on the shapes alone (M among them).  Up to 16 rows
+ * share one pass over the weight where shared memory has room for them: 16 of K = 13824 with N = 30720 take two passes.
  * weight: q packed as [ceil(N/16)][ceil(K/64)][512] bytes.  Byte ((r * 4 + t) * 16 + 8 * b + 4 * h + i) of tile (n, k) holds of
  *   row 16 n + 8 h + r the columns 64 k + 32 b + 8 t + c with c = {0, 4, 1, 5}[i] in its low and c + 2 in its high four bits
  * scale: half [ceil(N/16)][K/group][16]; zero: uint8 of the same layout, 0..15, or NULL for 8.

@@ -396,7 +396,6 @@ extern "C" int ksb_w4_linear(const void* x, int dtype, int64_t M, int64_t K, int
   const int tiles = (int)((K + w4::TILE_K - 1) / w4::TILE_K), step_tiles = w4::step_tiles(group);
   p.steps = tiles / step_tiles;
   p.groups = (int)(K / group);
-  // K is shared by a cluster where that fills the GPU, or makes room for the rows of x.
   auto plan = [&](int rows, int split) {
     const int clusters = std::min(units, cluster_room(split)), sums = w4::TILE_N * (rows > 8 ? 16 : 8) * 4;
     p.x_at = w4::WARPS * w4::depth(rows > 8 ? 2 : 1) * w4::slot_bytes(group, zero != nullptr);
@@ -408,14 +407,29 @@ extern "C" int ksb_w4_linear(const void* x, int dtype, int64_t M, int64_t K, int
     p.sums_at = p.x_at + rows * p.pitch;
     return p.sums_at + kept <= w4::SMEM_LIMIT - w4::fixed_bytes(rows > 8 ? 2 : 1) ? (int)(p.sums_at + kept) : 0;
   };
+  // K is shared by a cluster where that fills the GPU, or makes room for the rows of x.
+  int split = 1;
+  auto fit = [&](int rows) {
+    split = 1;
+    while (split < 8 && 2 * split * units <= sm_count() && 2 * split <= p.steps) split *= 2;
+    int smem;
+    while ((smem = plan(rows, split)) == 0 && split < 8 && 2 * split <= p.steps) split *= 2;
+    return smem;
+  };
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   int launches = 0;
   for (int64_t m0 = 0; m0 < M; ++launches) {
-    const int64_t left = M - m0, passes = (left + 15) / 16;
-    int rows = (int)((left + passes - 1) / passes), split = 1, smem = 0;
-    while (split < 8 && 2 * split * units <= sm_count() && 2 * split <= p.steps) split *= 2;
-    while ((smem = plan(rows, split)) == 0 && split < 8 && 2 * split <= p.steps) split *= 2;
-    while (smem == 0 && rows > 1) smem = plan(rows = (rows + 1) / 2, split = 1);  // the kept sums of very many row tiles
+    // As few passes over the weight as there is room for (x, and with a shared K the row tiles' sums), of equal sizes where those fit: nine to
+    // sixteen rows may fit where eight do not, whose rings are deeper.  16 x 13824 -> 30720 takes 92 us in two passes; in three, as it was where
+    // fewer rows were tried without clusters, 134.
+    const int64_t left = M - m0;
+    int rows = 0, smem = 0;
+    for (int most = (int)std::min<int64_t>(16, left); smem == 0 && most > 0; --most) {
+      const int64_t passes = (left + most - 1) / most;
+      rows = (int)((left + passes - 1) / passes);
+      smem = fit(rows);
+      if (smem == 0 && rows < most) smem = fit(rows = most);
+    }
     if (smem == 0) return fail(KSB_ERR_UNSUPPORTED, "no room for a row of %lld columns", (long long)K);
     p.M = rows;
     p.x = static_cast<const uint8_t*>(x) + m0 * ldx * 2;

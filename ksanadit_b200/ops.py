@@ -680,7 +680,8 @@ def w4_linear(x, weight, weight_scale, weight_zero=None, bias=None, out_features
 
     out[m, n] = sum over groups of scale * sum (q - zero) x, plus bias; sums in fp32, one rounding.  N: ``out_features`` (default: 16
     per tile row, or the bias's length).  The group is K / weight_scale.shape[1]: 32, 64 or 128.  Up to 16 rows of x share one pass over
-    the weight, more are taken 16 at a time: for many rows ``B200Fp8Linear`` is the faster class.  No gradients."""
+    the weight (fewer where both K and N are large), more take more passes: for many rows ``B200Fp8Linear`` is the faster class.  The order of a row's
+    sums goes by the shapes, the number of rows among them.  No gradients."""
     host = native.host_ops()
     if host:
         out = host.w4_linear(x, weight, weight_scale, weight_zero, bias, out_features)
