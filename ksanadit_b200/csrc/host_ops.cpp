@@ -126,13 +126,15 @@ variable_list last_derivatives(variable_list&& out, bool again) {
 }
 // A leaf's accumulation node keeps the stream that it was made on for as long as any graph of the leaf lives.  One of the default stream cannot take
 // part in a capture, and its failure inside the engine can end the process; here it is an error of this call, ahead of any launch.
+// Leaves whose gradients the pass does not ask for take no part.
 void leaves_can_be_captured() {
   cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
   if (cudaStreamIsCapturing(c10::cuda::getCurrentCUDAStream().stream(), &status) != cudaSuccess || status == cudaStreamCaptureStatusNone) return;
   const auto node = torch::autograd::get_current_node();
   if (!node) return;
-  for (const auto& edge : node->next_edges()) {
-    if (!edge.function || !dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get())) continue;
+  for (size_t i = 0; i < node->num_outputs(); ++i) {
+    const auto& edge = node->next_edge(i);
+    if (!edge.function || !dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get()) || !node->task_should_compute_output(i)) continue;
     const auto stream = edge.function->stream();
     TORCH_CHECK(!stream || !stream->device().is_cuda() || c10::cuda::CUDAStream(*stream) != c10::cuda::getDefaultCUDAStream(stream->device_index()),
                 "a backward pass is captured while a graph of the same leaves that was made on the default stream is alive: release its outputs first");

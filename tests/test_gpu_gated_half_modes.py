@@ -99,3 +99,29 @@ def test_registered_operators_are_recorded():
             x, y = _n(20, 16, seed=3), _n(20, 16, seed=4)
             assert all(torch.equal(a, b) for a, b in zip(recorded(x, y), f(x, y)))
             assert torch.equal(f(x, y)[0], ops.sandwich_norm(x, y, gate=x[0], residual_scale=0.5)[0])
+
+
+def _captured(step):
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    graph.replay()
+    torch.cuda.synchronize()
+    return out
+
+
+def test_capture_beside_an_eager_graph_of_other_leaves():
+    """An eager graph of a weight lives; a captured backward pass that does not ask for the weight's gradient has nothing to do with it."""
+    x = _n(20, 16).requires_grad_(True)
+    w = [_n(24, 16, seed=i).requires_grad_(True) for i in (1, 2)]
+    p = _n(16, dtype=torch.float32).requires_grad_(True)
+    plain = lambda: torch.autograd.grad(ops.gated_linear(x, *w).sum(), [x])  # noqa: E731
+    normed = lambda: torch.autograd.grad(ops.sandwich_norm(x, pre_weight=p)[1].sum(), [x])  # noqa: E731
+    want = [plain()[0], normed()[0]]
+    eager = ops.gated_linear(x.detach(), *w), ops.sandwich_norm(x.detach(), pre_weight=p)[1]
+    got = [_captured(plain)[0], _captured(normed)[0]]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert all(t.grad_fn is not None for t in eager)
+    with pytest.raises(RuntimeError, match="release its outputs"):
+        _captured(lambda: torch.autograd.grad(ops.gated_linear(x, *w).sum(), w))
+    _lib.assert_device_ok()
