@@ -346,6 +346,7 @@ __global__ void __launch_bounds__(Cfg<KIND, CTAS, TN, FLEX>::THREADS, 1) gemm_ke
             const int row = row0 + lane;
             for (int c = 0; c < OUT_N; c += 8) {
               uint32_t v[8], w[8];
+              __syncwarp();  // lanes without a row come from the last turn by another way, and the loads are the whole warp's
               tmem_ld8(t_row + c, v);
               tmem_ld8(t_row + OUT_N + c, w);
               tmem_wait_ld();
