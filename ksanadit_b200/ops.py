@@ -655,6 +655,8 @@ def _one_device(x, *ts):
 
 def _no_tangents(*ts):
     """Raises for dual tensors: a kernel sees their values alone, and a result without its tangent would count as a constant."""
+    if getattr(forward_ad, "_current_level", 0) < 0:  # no dual tensors: 2 us of asking each
+        return
     for t in ts:
         if t is not None and forward_ad.unpack_dual(t).tangent is not None:
             raise _lib.KsanaB200Error("the operators of a gated half have no forward-mode derivatives")
