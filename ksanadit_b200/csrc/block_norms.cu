@@ -178,9 +178,12 @@ constexpr int PLACES = 8;
 constexpr int RED_FLOATS = 2 * PLACES * 64;  // groups x warps, in fours, are at most 64
 // Every lane's v, all the same, for the compiler to know it: counts and addresses then leave the vector registers, and branches take one
 // instruction.  It is asked for (of the rows' counts, of the warps') where it gained.  us without and with: forward 30000 x 1536 70.9 and 65.0, x 4096
-// 169 and 155, 5000 x 5120 40.9 and 37.7, layer norm 2 x 32760 x 5120 646 and 582; but CTAs of all 320 threads with many rows, which
-// come to the copy's rate without it, lose: 75600 x 5120 485 and 531, 30000 x 2560 102 and 114.  Backward: four chunks, 20000 x 8192 442 and 365,
-// 75600 x 1 x 1536 877 and 744, layer norm 2 x 32760 x 5120 875 and (of the warps alone) 832; but 75600 x 5120 889 and 1081, 30000 x 1536 123 and 134.
+// 169 and 155, 5000 x 5120 40.9 and 37.7, 75600 x 768 95 and 87, x 2056 232 and 213, x 4616 504 and 470, layer norm 2 x 32760 x 5120 646 and 582.  RMS norms
+// by CTAs of all 320 threads whose lanes all have columns come to the copy's rate without it, and with many rows lose a tenth: 75600 x 5120 483 and 530,
+// x 2560 244 and 277, x 1024 106 and 116; so much from some 25000 rows of 1024 columns, 16000 of 2560, 11000 of 5120.  (After a tenth of a second
+// of nothing but such calls the two forms change places at 75600 x 5120, 531 and 490; the cause is not known.)
+// Backward: four chunks, 20000 x 8192 442 and 365, 75600 x 1 x 1536 877 and 744, layer norm 2 x 32760 x 5120 875 and (of the warps alone) 832; but
+// 75600 x 5120 889 and 1081, 30000 x 1536 123 and 134.
 template <bool ASKED> __device__ __forceinline__ int uniform(int v) { return ASKED ? __shfl_sync(0xffffffffu, v, 0) : v; }
 
 template <bool UNIFORM> struct Group {
@@ -843,7 +846,9 @@ template <typename T, int NC, bool LAYER, int THREADS, int CTAS, bool UNIFORM, b
 }
 template <typename T, int NC, bool LAYER, int THREADS, int CTAS> static int forward_as(const Params& p, int threads, int groups, cudaStream_t st) {
   if (p.rows_per_mod == 1 && p.M > 4096 && (p.gate || p.scale || p.shift)) return forward_kind<T, NC, LAYER, THREADS, CTAS, true, true>(p, threads, groups, st);
-  if (!LAYER && THREADS == 320 && groups * threads == 320 && p.M > 16384) return forward_kind<T, NC, LAYER, THREADS, CTAS, LAYER || THREADS != 320, false>(p, threads, groups, st);  // see uniform
+  // see uniform; a 32nd of the lanes may be idle (75600 x 992 100 and 114 us, x 896 98 and 90)
+  if (!LAYER && THREADS == 320 && groups * threads == 320 && p.C / 8 * 32 >= 31 * NC * threads && p.M > 16384)
+    return forward_kind<T, NC, LAYER, THREADS, CTAS, LAYER || THREADS != 320, false>(p, threads, groups, st);
   return forward_kind<T, NC, LAYER, THREADS, CTAS, true, false>(p, threads, groups, st);
 }
 template <typename T, bool LAYER> static int forward(const Params& p, cudaStream_t st) {
