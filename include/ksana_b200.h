@@ -406,7 +406,7 @@ int64_t ksb_qwen_block_workspace(const ksb_qwen_block* block, int64_t text_token
 int ksb_qwen_block_forward(const ksb_qwen_block* block, const ksb_qwen_call* call, int first, int last, void* workspace, ksb_stream_t stream);
 
 /* Operators of blocks whose halves are normed on both sides and whose feed-forward is gated, with the gradients that fine-tuning
- * needs.  They have no counterpart in KsanaDiT, which runs such models through eager torch. ------------------------------------ */
+ * needs.  They have no counterpart in KsanaDiT, none of whose models has such a half. ------------------------------------------- */
 
 /* Products of a few rows with a weight held in 4 bits: the one-row Linears of a block (timestep embedding, modulation), whose time is
  * the weight's way from memory.

@@ -77,7 +77,7 @@ __host__ __device__ __forceinline__ bool sums_all(const Grads& q) {
 
 __device__ __forceinline__ uint4 load8(const void* base, int64_t offset_bytes) { return *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(base) + offset_bytes); }
 
-// Two fp32 numbers in one register pair; one instruction works on both (backward pass of 75600 x 5120: 914 us, one by one 921).
+// Two fp32 numbers in one register pair; one instruction works on both (backward pass of 75600 x 5120: 0.8 % less than one by one).
 typedef unsigned long long F2;
 __device__ __forceinline__ F2 pair(float x, float y) {
   F2 r;
@@ -219,7 +219,7 @@ template <bool UNIFORM> struct Group {
     return collect(at);
   }
   // N sums in one exchange.  Of eight, lanes first share out the sums and only then add up one each, the warps' sums as well: 9 and 2 shuffles
-  // instead of 40, and 5 loads instead of 40 (32760 x 2 x 5120: 936 us instead of 1090).  Of three that would only lengthen the way (903 -> 1133).
+  // instead of 40, and 5 loads instead of 40 (32760 x 2 x 5120: a seventh less).  Of three that would only lengthen the way (75600 x 5120: a quarter more).
   template <int N> __device__ __forceinline__ void sums(float (&v)[N]) const {
     constexpr bool SHARED_OUT = N == 8;
     if (SHARED_OUT) {
@@ -423,7 +423,8 @@ struct Sums {
 // three sums for RMS norms (a0 = 0) and of eight for layer norms, instead of two, one after the other.
 //
 // Up to 5120 columns a thread has one chunk and up to twenty warps share a row: eight warps of three chunks, which leaves the exchanges less to do
-// but the schedulers two warps each, took 1040 us for 75600 x 5120, twelve of two 1058, twenty of one 903.
+// but the schedulers two warps each, took 15 % longer for 75600 x 5120 than twenty of one (889 us now), twelve of two 17 %.  NC = 4 with WHOLE has 240 - 376
+// bytes of spills at 255 registers: 20000 x 1 x 8192 1745 us, layer norm 1784.
 template <typename T, int NC, bool LAYER, bool WHOLE, bool ONE>
 __global__ void __launch_bounds__(backward_threads<NC>, 1) backward_kernel(const __grid_constant__ Params p, const __grid_constant__ Grads q) {
   extern __shared__ __align__(16) uint8_t ring_bytes[];  // [DEPTH][x, y, dr, dh][NC][threads] 16 bytes and the factors; in the end the groups' sums
@@ -580,7 +581,7 @@ __global__ void __launch_bounds__(backward_threads<NC>, 1) backward_kernel(const
     F2 tr = both(0.f), wz = tr, rz = tr, ts = tr, zs = tr, wa = tr, ra = tr, as = tr;
     const uint32_t src = mine + slot * 4 * NC * all * 16;
     auto from = [&](int which, int c, bool there) { return unpack8<T>(live[c] && there ? ld_shared_v4(src + (which * NC + c) * all * 16) : none); };
-    // the factors are read where they are used: held, they would push others out of the registers (903 -> 1110 us)
+    // the factors are read where they are used: held, they would push others out of the registers (75600 x 5120: 23 % more)
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       yh[c] = from(1, c, p.y != nullptr);

@@ -6,8 +6,8 @@
     x = x + residual_scale * gate * N(y) * post_norm
 
 KsanaDiT's own blocks (ksana/models/wan/wan_model.py:317-321, ksana/models/qwen/transformer.py:225-234) have a plain GELU
-feed-forward and no norm behind a half; models of this form run there as eager torch.  In a stack of halves the norm behind one and the
-norm ahead of the next are one pass over the tokens.  Everything but the 4-bit modulation is differentiable (an embedding that needs a
+feed-forward and no norm behind a half: this module is for models beside them.  In a stack of halves the norm behind one and the norm
+ahead of the next are one pass over the tokens.  Everything but the 4-bit modulation is differentiable (an embedding that needs a
 gradient through it is refused), so the same module is fine-tuned and served; for serving, ``down`` may be a ``B200Fp8Linear``.
 """
 
