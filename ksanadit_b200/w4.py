@@ -72,6 +72,7 @@ def _scales(span: torch.Tensor, levels: int, dtype) -> torch.Tensor:
     return torch.where(span == 0, torch.full_like(scale, f.smallest_normal), scale)
 
 
+@torch.no_grad()
 def quantize_w4(w: torch.Tensor, group: int = 128, zeros: bool = False, dtype=torch.bfloat16):
     """Rounds a weight [N, K] to 4 bits per group of ``group`` columns -> (packed, scale, zero or None) as ``ops.w4_linear`` takes them.
 

@@ -70,3 +70,11 @@ def test_products_with_small_scales(std, dtype, zeros):
     # one rounding of the result, half a step of the type's least number where it is tiny, and the sum's (256 / 16 + 48 of 2^-22)
     f = torch.finfo(dtype)
     assert bool(((out.double() - ref).abs() <= f.eps / 2 * ref.abs() + f.smallest_normal * f.eps / 2 + 64 * 2.0 ** -22 * (1 + f.eps) * size).all())
+
+
+def test_a_parameter_is_quantised_without_a_graph():
+    lin = torch.nn.Linear(64, 16)
+    for zeros in (False, True):
+        parts = w4.quantize_w4(lin.weight, 64, zeros)
+        assert not any(t is not None and t.requires_grad for t in parts)
+        assert all(a is b or torch.equal(a, b) for a, b in zip(parts, w4.quantize_w4(lin.weight.detach(), 64, zeros)))
