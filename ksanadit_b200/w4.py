@@ -26,6 +26,8 @@ def pack_w4(q: torch.Tensor) -> torch.Tensor:
     """Values 0..15 [N, K] (uint8) -> the packed weight [ceil(N/16), ceil(K/64), 512] that ``ops.w4_linear`` reads."""
     if q.dim() != 2 or q.dtype != torch.uint8:
         raise _lib.KsanaB200Error("pack_w4 needs a 2-D uint8 tensor")
+    if q.numel() and int(q.max()) > 15:  # it would change its neighbour
+        raise _lib.KsanaB200Error(f"pack_w4 needs values 0 .. 15, found {int(q.max())}")
     N, K = q.shape
     nt, kt = _tiles(N, TILE_N), _tiles(K, TILE_K)
     full = torch.full((nt * TILE_N, kt * TILE_K), 8, dtype=torch.uint8, device=q.device)

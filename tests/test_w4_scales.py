@@ -78,3 +78,13 @@ def test_a_parameter_is_quantised_without_a_graph():
         parts = w4.quantize_w4(lin.weight, 64, zeros)
         assert not any(t is not None and t.requires_grad for t in parts)
         assert all(a is b or torch.equal(a, b) for a, b in zip(parts, w4.quantize_w4(lin.weight.detach(), 64, zeros)))
+
+
+def test_values_of_more_than_four_bits_are_refused():
+    q = torch.randint(0, 16, (17, 64), dtype=torch.uint8, generator=torch.Generator().manual_seed(0))
+    q[16, 63] = 15
+    w4.pack_w4(q)
+    for bad in (16, 255):
+        q[16, 63] = bad
+        with pytest.raises(_lib.KsanaB200Error, match="15"):
+            w4.pack_w4(q)
